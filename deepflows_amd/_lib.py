@@ -128,6 +128,9 @@ _SIGS = {
     "dfhip_sgd_step": [c_int, PP, PP, PP, I64P, c_double, c_double, c_double, c_int, c_double],
     "dfhip_sgd_hyper": [P, c_double, c_double, c_double, c_int, c_double],
     "dfhip_sgd_step_dev": [c_int, PP, PP, PP, I64P, P],
+    "dfhip_clip_grad_norm": [c_int, PP, PP, I64P, c_double, c_int, c_double, P],
+    "dfhip_rms_norm_forward": [P] * 6 + [c_int64, c_int64, c_float],
+    "dfhip_rms_norm_backward": [P] * 7 + [c_int64, c_int64],
     "dfhip_pack": [c_int, PP, I64P, P],
     "dfhip_unpack": [c_int, PP, I64P, P],
     "dfhip_comm_unique_id": [c_char_p],

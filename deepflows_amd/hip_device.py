@@ -738,6 +738,23 @@ class HipModule:
         mb = _ptr_table(momentum_buf) if momentum_buf else None
         _lib.check(self._lib.dfhip_sgd_step_dev(n, _ptr_table(params), _ptr_table(grads), mb, sizes, hyper.ptr))
 
+    def clip_grad_norm(self, grads, outs, norm, max_norm, infinity=False, grad_scale=1.0):
+        """outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); norm[0] = the norm over all of them, times grad_scale."""
+        n = len(grads)
+        sizes = (c_int64 * n)(*[g.size for g in grads])
+        _lib.check(self._lib.dfhip_clip_grad_norm(n, _ptr_table(grads), _ptr_table(outs), sizes, float(max_norm),
+                                                  0 if infinity else 2, float(grad_scale), norm.ptr))
+
+    def rms_norm_forward(self, x, residual, weight, y, h, rstd, rows, width, eps):
+        g = lambda a: a.ptr if a is not None else None
+        _lib.check(self._lib.dfhip_rms_norm_forward(x.ptr, g(residual), g(weight), y.ptr, g(h), g(rstd), rows, width,
+                                                    float(eps)))
+
+    def rms_norm_backward(self, dy, h, rstd, weight, add, dx, dweight, rows, width):
+        g = lambda a: a.ptr if a is not None else None
+        _lib.check(self._lib.dfhip_rms_norm_backward(dy.ptr, h.ptr, rstd.ptr, g(weight), g(add), g(dx), g(dweight), rows,
+                                                     width))
+
     def pack(self, srcs, flat):
         n = len(srcs)
         sizes = (c_int64 * n)(*[s.size for s in srcs])

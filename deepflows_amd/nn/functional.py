@@ -440,6 +440,99 @@ def log_softmax(input: Tensor, dim=None, keepdims=False):
     return shifted - tensor.log(tensor.sum(tensor.exp(shifted), dim, True))
 
 
+# ---- root-mean-square normalisation ------------------------------------------------------------------
+class _ResidualSum(_FusedNode):
+    """h = x + residual of `rms_norm`, formed inside the normalisation's launch: both inputs receive h's gradient as it is"""
+
+    def __init__(self, x, residual, hd):
+        super().__init__(hd, [x, residual])
+
+    def grad_fn(self, node, grad):
+        return grad
+
+
+class _RMSNormFused(_FusedNode):
+    """x / sqrt(mean(x^2) + eps) * weight over the last axis: one forward launch (dfhip_rms_norm_forward, issued by
+    `rms_norm`), one backward launch for the input's and the weight's gradient together (and one that adds the weight's partial
+    rows up).  The gradient the input already holds -- a residual stream's other reader -- is added in that launch."""
+
+    fuses_accumulation = True
+
+    def __init__(self, x, weight, yd, rstd):
+        self.x, self.weight = x, weight
+        self._saved = (x.data.compact(), weight.data.compact() if weight is not None else None, rstd)
+        self._dw = None                          # (upstream gradient, weight gradient) left behind by the input's turn
+        super().__init__(yd, [x, weight])
+
+    def _launch(self, grad, want_dx, held):
+        xd, wd, rstd = self._saved
+        dev = grad.device
+        dx = _new(xd.shape, dev) if want_dx else None
+        dw = _grad_out(self.weight, self.weight.shape, dev) if self.weight is not None and self.weight.requires_grad else None
+        h = lambda t: t._handle if t is not None else None
+        width = int(xd.shape[-1])
+        dev.mod.rms_norm_backward(grad.compact()._handle, xd._handle, rstd._handle, h(wd), h(held), h(dx), h(dw),
+                                  xd.size // width, width)
+        return dx, dw
+
+    def grad_fn(self, node, grad, held=None):
+        if node is self.x:
+            dx, dw = self._launch(grad, True, held.compact() if held is not None else None)
+            self._dw = (grad, dw)
+            return dx
+        ready, self._dw = self._dw, None         # (handed out once: another sweep over a retained graph starts afresh)
+        if ready is not None and ready[0] is grad:
+            return ready[1]
+        return self._launch(grad, False, None)[1]
+
+
+def rms_norm(input: Tensor, weight=None, eps: float = 1e-6, residual=None):
+    """Root-mean-square normalisation over the last axis: input / sqrt(mean(input^2) + eps) * weight.
+
+    With `residual` (a tensor of input's shape) the sum h = input + residual is normalised and (y, h) come back: h is what the
+    next residual sum starts from.  weight: None or a tensor with as many elements as the last axis.  Zero rows are allowed."""
+    input = realize(input)
+    residual = realize(residual) if residual is not None else None
+    if input.ndim < 1 or int(input.shape[-1]) < 1:
+        raise ValueError(f"rms_norm: the last axis must have at least one element, got shape {tuple(input.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"rms_norm: eps must be >= 0, got {eps}")
+    shape = tuple(int(v) for v in input.shape)
+    width = shape[-1]
+    if weight is not None and (int(weight.size) != width or int(weight.shape[-1]) != width):
+        raise ValueError(f"rms_norm: weight of shape {tuple(weight.shape)} for a last axis of {width}")
+    if weight is input:
+        raise ValueError("rms_norm: weight and input are one tensor")
+    if residual is not None and tuple(int(v) for v in residual.shape) != shape:
+        raise ValueError(f"rms_norm: residual of shape {tuple(residual.shape)} for an input of shape {shape}")
+    for other in (weight, residual):
+        if other is not None and other.device != input.device:
+            raise ValueError("rms_norm: all tensors must be on one device")
+    mod = input.device.mod
+    if _fused(input) and hasattr(mod, "rms_norm_forward"):
+        dev = input.device
+        xd = input.data.compact()
+        y = _new(shape, dev)
+        grad = is_grad_enable() and any(t is not None and t.requires_grad for t in (input, weight, residual))
+        rows = y.size // width
+        rstd = _new((rows,), dev) if grad else None
+        h = lambda t: t._handle if t is not None else None
+        hd = _new(shape, dev) if residual is not None else None
+        wd = weight.data.compact() if weight is not None else None
+        rd = residual.data.compact() if residual is not None else None
+        mod.rms_norm_forward(xd._handle, h(rd), h(wd), y._handle, h(hd), h(rstd), rows, width, eps)
+        summed = _ResidualSum(input, residual, hd) if residual is not None else input
+        out = _RMSNormFused(summed, weight, y, rstd)
+    else:
+        summed = input + residual if residual is not None else input
+        axis = len(shape) - 1
+        mean = tensor.sum(summed * summed, axes=axis, keepdims=True) / width
+        out = summed / (mean + eps) ** 0.5
+        if weight is not None:
+            out = out * weight
+    return (out, summed) if residual is not None else out
+
+
 # ---- losses --------------------------------------------------------------------------------------
 def nll_loss(input: Tensor, target: Tensor, reduction: str = 'mean'):
     nll = -input * target

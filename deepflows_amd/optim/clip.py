@@ -1,0 +1,87 @@
+"""Clipping the gradients of a network by their common norm (extension; the reference has none)."""
+import math
+
+from .. import backend_api
+from ..backend_selection import BackendTensor
+from ..parallel import _ArrayView
+from ..tensor import Tensor
+
+_ALIGN = 64         # a gradient's place in the common array begins at a multiple of this many elements (256 bytes)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, grad_scale=1.0, error_if_nonfinite=False):
+    """Scales the gradients of `parameters` down to a common norm of at most `max_norm`; returns that norm as it was before, a
+    tensor of shape (1,).
+
+    norm_type 2: the square root of the sum of all squares, held in double; norm_type inf: the largest magnitude.  Every
+    gradient is multiplied by min(1, max_norm / (norm + 1e-6)); a NaN or an infinity in one of them shows in the norm and in all.
+    Parameters without a gradient are passed over, one that is listed twice counts once.  `grad_scale` is the factor the
+    optimizer applies when it steps (`optimizer.grad_scale`, 1/world behind a gradient exchange): the norm is that of the scaled
+    gradients.  error_if_nonfinite reads the norm back and raises RuntimeError instead of scaling, which a captured step cannot.
+
+    Gradients are not modified in place: p.grad is replaced (nodes of a retained graph and parameters with a common gradient
+    keep reading the arrays they have)."""
+    params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    max_norm, norm_type, grad_scale = float(max_norm), float(norm_type), float(grad_scale)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grad_norm_: max_norm must be >= 0, got {max_norm}")
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f"clip_grad_norm_: norm_type is 2 or inf, got {norm_type}")
+    if not 0.0 <= grad_scale < math.inf:
+        raise ValueError(f"clip_grad_norm_: grad_scale must be finite and >= 0, got {grad_scale}")
+    seen, live, grads = set(), [], []
+    for p in params:
+        g = p.grad
+        if g is None or id(p) in seen:
+            continue
+        seen.add(id(p))
+        live.append(p)
+        grads.append((g.data if isinstance(g, Tensor) else g).compact())
+    device = grads[0].device if grads else (params[0].device if params else backend_api.default_device())
+    for g in grads:
+        if g.device != device:
+            raise ValueError("clip_grad_norm_: the gradients are on different devices")
+    mod = device.mod
+    if error_if_nonfinite and getattr(mod, "capturing", False):
+        raise RuntimeError("clip_grad_norm_: error_if_nonfinite reads the norm back, which a captured step cannot")
+    if not hasattr(mod, "clip_grad_norm"):
+        return _primitive(live, grads, device, max_norm, norm_type, grad_scale, error_if_nonfinite)
+    norm = BackendTensor.make((1,), device=device)
+    places, end = [], 0
+    for g in grads:
+        places.append(end)
+        end += -(-g._handle.size // _ALIGN) * _ALIGN
+    flat = mod.Array(end)
+    outs = [_ArrayView(flat, at, g._handle.size) for at, g in zip(places, grads)]
+    mod.clip_grad_norm([g._handle for g in grads], outs, norm._handle, max_norm, norm_type == math.inf, grad_scale)
+    if error_if_nonfinite:
+        _refuse_nonfinite(float(norm.numpy()[0]))
+    for p, g, out in zip(live, grads, outs):
+        p.grad = _like(p.grad, BackendTensor.make(g.shape, device=device, handle=out))
+    return Tensor(norm)
+
+
+def _like(old, new):
+    return Tensor(new) if isinstance(old, Tensor) else new
+
+
+def _refuse_nonfinite(norm):
+    if not math.isfinite(norm):
+        raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {norm}")
+
+
+def _primitive(live, grads, device, max_norm, norm_type, grad_scale, error_if_nonfinite):
+    """the same over the device primitives, a scalar read back per gradient"""
+    if norm_type == math.inf:
+        parts = [float((g.maximum(-g)).max().numpy().reshape(-1)[0]) for g in grads if g.size]
+        total = math.nan if any(math.isnan(v) for v in parts) else max(parts, default=0.0)
+    else:
+        total = math.sqrt(sum(float((g * g).sum().numpy().reshape(-1)[0]) for g in grads if g.size))
+    total *= grad_scale
+    if error_if_nonfinite:
+        _refuse_nonfinite(total)
+    coef = max_norm / (total + 1e-6)
+    coef = 1.0 if coef > 1.0 else coef
+    for p, g in zip(live, grads):
+        p.grad = _like(p.grad, g * coef)
+    return Tensor(device.full((1,), total))

@@ -377,6 +377,20 @@ int dfhip_bn_relu_maxpool2_backward(const float* x, const float* y, const float*
                                     float* dx, float* dgamma, float* dbeta, int N, int C, int H, int W,
                                     float eps);
 
+/* Root-mean-square normalisation over the last axis, with the residual's addition in front of it (extension; kin of
+ * dfhip_bn2d_forward_train with its residual): per row of `width` elements
+ *     h = x + residual (residual NULL: h = x),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight (weight NULL: 1).
+ * y (rows, width); h (rows, width) is written when a residual is given, ignored otherwise; rstd (rows) feeds the backward
+ * pass and may be NULL.  The mean of the squares is held in double.  No output may overlap an input. */
+int dfhip_rms_norm_forward(const float* x, const float* residual, const float* weight, float* y, float* h, float* rstd,
+                           int64_t rows, int64_t width, float eps);
+/* Its gradient, from the h and rstd of the forward pass: with n = h * rstd and g = dy * weight
+ *     dx = rstd * (g - n * mean(g * n)) + add,   dweight = column sums of dy * n.
+ * dx is the gradient of x AND of the residual; add (may be NULL) is the gradient h received from its other readers.  dx or
+ * dweight may be NULL.  The column sums are added in a fixed order.  No output may overlap an input. */
+int dfhip_rms_norm_backward(const float* dy, const float* h, const float* rstd, const float* weight, const float* add,
+                            float* dx, float* dweight, int64_t rows, int64_t width);
+
 /* Input pipeline on the device.
  * dfhip_upload_async / dfhip_upload_wait: double-buffered pinned upload on a copy stream, so the
  * H2D of batch k+1 overlaps the training step of batch k (utils/data/dataloader.py:60-139 hands
@@ -544,6 +558,16 @@ int dfhip_sgd_hyper(float* hyper_dev, double lr, double momentum, double weight_
                     double grad_scale);
 int dfhip_sgd_step_dev(int n_tensors, float* const* params, const float* const* grads,
                        float* const* momentum_buf, const int64_t* sizes, const float* hyper_dev);
+
+/* The norm over all gradients of a network and the gradients scaled down to a largest norm (extension; the reference has no
+ * clipping).  total = grad_scale * sqrt(sum of g^2 over all tensors) (DFHIP_NORM_2) or grad_scale * max |g|
+ * (DFHIP_NORM_INF); outs[i] = grads[i] * min(1, max_norm / (total + 1e-6)); norm[0] = total.  The sum of squares is held in
+ * double.  outs[i] may be grads[i].  A NaN or an infinity in any gradient shows in `norm` and in the outputs.  grad_scale is
+ * the factor an optimizer step applies later (1/world for data parallel): it enters `total`, not `outs`. */
+#define DFHIP_NORM_2 2
+#define DFHIP_NORM_INF 0
+int dfhip_clip_grad_norm(int n_tensors, const float* const* grads, float* const* outs, const int64_t* sizes, double max_norm,
+                         int norm_type, double grad_scale, float* norm);
 
 /* Pack / unpack a list of tensors into one flat bucket (gradient all-reduce payload).   */
 int dfhip_pack(int n_tensors, const float* const* srcs, const int64_t* sizes, float* flat);

@@ -1,0 +1,77 @@
+"""CPU: F.rms_norm, nn.RMSNorm and optim.clip_grad_norm_ on the NumPy oracle device (their compositions over the device
+primitives), and what they refuse."""
+import math
+
+import numpy as np
+import pytest
+
+from conftest import assert_close
+
+
+def test_rms_norm_composition(cpu_oracle):
+    from deepflows_amd import nn, tensor
+    from deepflows_amd.tensor import Tensor
+    rng = np.random.default_rng(0)
+    x, r, c = (rng.standard_normal((4, 10)).astype(np.float32) for _ in range(3))
+    norm = nn.RMSNorm(10, eps=1e-3, device=cpu_oracle)
+    xt = Tensor(x, device=cpu_oracle, requires_grad=True)
+    y, h = norm(xt, Tensor(r, device=cpu_oracle))
+    s = (x + r).astype(np.float64)
+    inv = 1 / np.sqrt((s * s).mean(-1, keepdims=True) + 1e-3)
+    assert_close(h.numpy(), x + r, 1e-7)
+    assert_close(y.numpy(), s * inv, 1e-6)
+    (tensor.sum(y * Tensor(c, device=cpu_oracle))).reshape(1).backward()
+    assert_close(xt.grad.numpy(), inv * (c - s * inv * (c * s * inv).mean(-1, keepdims=True)), 1e-5)
+    assert_close(norm.weight.grad.numpy(), (c * s * inv).sum(0), 1e-5)
+    assert "weight" in norm.state_dict()
+
+
+def test_rms_norm_refusals(cpu_oracle):
+    from deepflows_amd import nn
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x = Tensor(np.ones((3, 8), np.float32), device=cpu_oracle)
+    with pytest.raises(ValueError):
+        F.rms_norm(x, Tensor(np.ones(7, np.float32), device=cpu_oracle))
+    with pytest.raises(ValueError):
+        F.rms_norm(x, None, eps=float("nan"))
+    with pytest.raises(ValueError):
+        F.rms_norm(x, None, residual=Tensor(np.ones((2, 8), np.float32), device=cpu_oracle))
+    with pytest.raises(ValueError):
+        nn.RMSNorm(0, device=cpu_oracle)
+
+
+def _params(dev, arrays):
+    from deepflows_amd import nn
+    from deepflows_amd.tensor import Tensor
+    out = []
+    for a in arrays:
+        p = nn.Parameter(Tensor(np.zeros(a.shape), device=dev))
+        p.grad = Tensor(a, device=dev).data
+        out.append(p)
+    return out
+
+
+@pytest.mark.parametrize("kind", [2, math.inf])
+def test_clip_composition(cpu_oracle, kind):
+    from deepflows_amd import optim
+    rng = np.random.default_rng(1)
+    arrays = [rng.standard_normal(s).astype(np.float32) for s in ((3, 4), (1, 7), (5,))]
+    params = _params(cpu_oracle, arrays)
+    total = optim.clip_grad_norm_(params, 0.5, norm_type=kind, grad_scale=0.5)
+    flat = np.concatenate([a.reshape(-1) for a in arrays]).astype(np.float64)
+    want = 0.5 * (np.sqrt((flat ** 2).sum()) if kind == 2 else np.abs(flat).max())
+    assert_close(total.numpy(), [want], 1e-6)
+    for a, p in zip(arrays, params):
+        assert_close(p.grad.numpy(), a * min(1.0, 0.5 / (want + 1e-6)), 1e-6)
+
+
+def test_clip_refusals(cpu_oracle):
+    from deepflows_amd import optim
+    params = _params(cpu_oracle, [np.ones(3, np.float32)])
+    for kw in ({"max_norm": -1.0}, {"max_norm": 1.0, "norm_type": 3.0}, {"max_norm": 1.0, "grad_scale": -0.1}):
+        with pytest.raises(ValueError):
+            optim.clip_grad_norm_(params, **kw)
+    params[0].grad.fill(np.inf)
+    with pytest.raises(RuntimeError):
+        optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
