@@ -129,6 +129,8 @@ _SIGS = {
     "dfhip_sgd_hyper": [P, c_double, c_double, c_double, c_int, c_double],
     "dfhip_sgd_step_dev": [c_int, PP, PP, PP, I64P, P],
     "dfhip_clip_grad_norm": [c_int, PP, PP, I64P, c_double, c_int, c_double, P],
+    "dfhip_linear_ce_forward": [P] * 8 + [c_int64] * 4 + [c_double, c_int],
+    "dfhip_scale_by": [P, P, P, c_int64],
     "dfhip_rms_norm_forward": [P] * 6 + [c_int64, c_int64, c_float],
     "dfhip_rms_norm_backward": [P] * 7 + [c_int64, c_int64],
     "dfhip_pack": [c_int, PP, I64P, P],

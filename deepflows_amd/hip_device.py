@@ -745,6 +745,15 @@ class HipModule:
         _lib.check(self._lib.dfhip_clip_grad_norm(n, _ptr_table(grads), _ptr_table(outs), sizes, float(max_norm),
                                                   0 if infinity else 2, float(grad_scale), norm.ptr))
 
+    def linear_ce_forward(self, x, w, bias, target, loss, dx, dw, db, rows, width, classes, ignore_index, label_smoothing, mean):
+        """cross entropy of x . w + bias for class indices, and the gradients (each may be None) for an upstream gradient of 1"""
+        g = lambda a: a.ptr if a is not None else None
+        _lib.check(self._lib.dfhip_linear_ce_forward(x.ptr, w.ptr, g(bias), target.ptr, loss.ptr, g(dx), g(dw), g(db), rows,
+                                                     width, classes, int(ignore_index), float(label_smoothing), int(mean)))
+
+    def scale_by(self, src, scalar, dst):
+        _lib.check(self._lib.dfhip_scale_by(src.ptr, scalar.ptr, dst.ptr, dst.size))
+
     def rms_norm_forward(self, x, residual, weight, y, h, rstd, rows, width, eps):
         g = lambda a: a.ptr if a is not None else None
         _lib.check(self._lib.dfhip_rms_norm_forward(x.ptr, g(residual), g(weight), y.ptr, g(h), g(rstd), rows, width,

@@ -604,6 +604,80 @@ def cross_entropy(input: Tensor, target: Tensor, reduction: str = 'mean', dim: i
     assert 0, "reduction must be mean or sum."
 
 
+class _LinearCrossEntropyFused(_FusedNode):
+    """cross entropy of a linear layer (dfhip_linear_ce_forward): the launches of the forward pass leave the gradients for an
+    upstream gradient of 1 behind -- what loss.backward() seeds --, grad_fn hands them out, or their product with another one."""
+
+    def __init__(self, x, weight, bias, target, mean, ignore_index, label_smoothing):
+        self.x, self.w, self.b = x, weight, bias
+        dev = x.device
+        rows, width = (int(v) for v in x.shape)
+        grads = [_new(p.shape, dev) if p is not None and is_grad_enable() and p.requires_grad else None
+                 for p in (x, weight, bias)]
+        h = lambda t: t._handle if t is not None else None
+        out = _new((1,), dev)
+        xd, wd, td = x.data.compact(), weight.data.compact(), target.data.compact()
+        bd = bias.data.compact() if bias is not None else None
+        dev.mod.linear_ce_forward(xd._handle, wd._handle, h(bd), td._handle, out._handle, *[h(g) for g in grads], rows, width,
+                                  int(weight.shape[1]), ignore_index, label_smoothing, mean)
+        self._unit = grads
+        super().__init__(out, [x, weight, bias])
+
+    def grad_fn(self, node, grad):
+        unit = self._unit[0 if node is self.x else (1 if node is self.w else 2)]
+        if getattr(grad, "is_unit_seed", False):
+            return unit
+        out = _new(unit.shape, unit.device)
+        unit.device.mod.scale_by(unit._handle, grad.compact()._handle, out._handle)
+        return out
+
+
+def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, reduction: str = 'mean',
+                         ignore_index: int = -100, label_smoothing: float = 0.0):
+    """cross_entropy(linear(input, weight, bias), target) for many classes: the logits are never kept.
+
+    input (N, D), weight (D, V), bias None or V elements, target (N,): class indices as whole numbers (fp32, the device's only
+    type, holds them exactly up to 2^24 classes).  Rows whose target is `ignore_index` are not counted; 'mean' divides by the
+    number of counted rows, and a batch without one has loss 0 and zero gradients.  label_smoothing e: the target distribution is
+    (1 - e) onehot + e / V.  On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it
+    in time to raise would stall the device); elsewhere it raises ValueError."""
+    input = realize(input)
+    if input.ndim != 2 or weight.ndim != 2 or int(input.shape[1]) != int(weight.shape[0]):
+        raise ValueError(f"linear_cross_entropy: input {tuple(input.shape)} and weight {tuple(weight.shape)} do not match")
+    rows, classes = int(input.shape[0]), int(weight.shape[1])
+    if classes < 1 or int(input.shape[1]) < 1:
+        raise ValueError("linear_cross_entropy: at least one class and one input feature are needed")
+    if bias is not None and (int(bias.size) != classes or int(bias.shape[-1]) != classes):
+        raise ValueError(f"linear_cross_entropy: bias of shape {tuple(bias.shape)} for {classes} classes")
+    if tuple(int(v) for v in target.shape) != (rows,):
+        raise ValueError(f"linear_cross_entropy: target of shape {tuple(target.shape)} for {rows} rows (class indices, one a row)")
+    if target.requires_grad:
+        raise ValueError("linear_cross_entropy: the class indices cannot require a gradient")
+    if reduction not in ('mean', 'sum'):
+        raise ValueError("reduction must be mean or sum.")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"linear_cross_entropy: label_smoothing must be in [0, 1], got {label_smoothing}")
+    if int(ignore_index) != ignore_index:
+        raise ValueError(f"linear_cross_entropy: ignore_index must be a whole number, got {ignore_index}")
+    if input is weight or (bias is not None and (bias is input or bias is weight)):
+        raise ValueError("linear_cross_entropy: input, weight and bias must be different tensors")
+    for other in (weight, bias, target):
+        if other is not None and other.device != input.device:
+            raise ValueError("linear_cross_entropy: all tensors must be on one device")
+    mean = reduction == 'mean'
+    if _fused(input) and hasattr(input.device.mod, "linear_ce_forward"):
+        return _LinearCrossEntropyFused(input, weight, bias, target, mean, int(ignore_index), float(label_smoothing))
+    t = target.numpy()
+    counted = t != ignore_index
+    if np.any(counted & ~((t >= 0) & (t < classes) & (t == np.floor(t)))):
+        raise ValueError(f"linear_cross_entropy: a target is neither a class index below {classes} nor {ignore_index}")
+    q = np.zeros((rows, classes), dtype=np.float32)
+    q[counted] = label_smoothing / classes
+    q[np.nonzero(counted)[0], t[counted].astype(np.int64)] += 1.0 - label_smoothing
+    nll = tensor.sum(-log_softmax(linear(input, weight, bias), 1) * Tensor(q, device=input.device))
+    return nll * (1.0 / max(1, int(counted.sum()))) if mean else nll
+
+
 # ---- im2col building blocks (primitive path; functional.py:249-313) ---------------------------------
 class _im2col2d(tensor.UnaryOperator):
     def __init__(self, x, kernel_size, stride):

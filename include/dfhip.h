@@ -494,6 +494,22 @@ int dfhip_mlp2_ce_forward(const float* x, const float* w1, const float* b1, cons
 int dfhip_mlp2_ce_backward(const float* x, const float* h, const float* dz1, const float* dlogits, float* dw1, float* db1,
                            float* dw2, float* db2, const float* rowloss, float* loss, int M, int K, int HD, int P);
 
+/* Softmax cross entropy of a linear layer over many classes without keeping its logits, with its gradient (extension; the
+ * composition it stands for is nn/functional.py:8-12 followed by :104-115, there with dense targets as large as the logits):
+ *     l = x (rows, width) . w (width, classes) + bias (classes or NULL)
+ *     row loss = lse(l) - (1 - e) l[target] - e / classes * sum(l),  e = label_smoothing
+ *     loss (1) = sum of the row losses of the counted rows, divided by their number (at least 1) when mean != 0
+ * and, for an upstream gradient of 1, dx (rows, width), dw (width, classes), db (classes); each may be NULL.
+ * target (rows): class indices as whole numbers in fp32; rows with target == ignore_index are not counted: no loss, zeros in dx,
+ * nothing added to dw and db.  A target that is neither ignore_index nor a whole number in [0, classes) makes the loss and the
+ * gradients it reaches NaN.  At most 2^24 classes.  Without counted rows the loss and the gradients are 0.
+ * Scratch memory comes from the pool and does not grow with rows x classes.  No output may overlap an input. */
+int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, const float* target, float* loss, float* dx,
+                            float* dw, float* db, int64_t rows, int64_t width, int64_t classes, int64_t ignore_index,
+                            double label_smoothing, int mean);
+/* dst = src * scalar[0]: a stored gradient for an upstream gradient other than 1 */
+int dfhip_scale_by(const float* src, const float* scalar, float* dst, int64_t n);
+
 /* Dropout in training mode as one launch each way (nn/modules/dropout.py:31 `x * mask / (1 - p)`, the mask drawn on the
  * host): backward = 0: y = (x * mask) / keep; backward = 1 (x is the upstream gradient): y = (x / keep) * mask -- the two
  * primitive nodes' results bit for bit (backend_tensor.py:551-586, tensor.py:640-676).  keep = 1 - p. */

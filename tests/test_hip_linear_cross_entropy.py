@@ -1,0 +1,353 @@
+"""GPU: cross entropy of a linear layer over many classes without its logits (F.linear_cross_entropy,
+nn.LinearCrossEntropyLoss; dfhip_linear_ce_forward) against the definition in 64 bits.
+
+Tolerances, from the arithmetic (u = 2^-24).  A product of K terms a b is formed from operands that carry at most 2^-22 relative
+each (or a floor of 2^-39 of the array's largest magnitude A, B) and summed in fp32 in at most 3 K roundings, independent of each
+other: |error| <= (12 + 6 sqrt(3 K)) u sum|a b| + 2^-38 (A sum|b| + B sum|a|), six standard deviations.
+  E   = the largest such error of a row's logits, plus u |l| for the bias;
+  row loss: the log-sum-exp and the target's logit move by at most E each, the sums over V (depth V / 256 + 20) and the last
+        operations add u (V / 256 + 40) (1 + |lse - l_t|), the smoothing term another E + u (V/256 + 20) mean|l - m|;
+  dl  = p - q: p (2 E + (V / 256 + 40) u), 4 u for the subtractions from values up to 1, 2^-22 |dl| + 2^-38 for its operand form;
+  dx, dW, db: the product's own error plus the sum of |other operand| times dl's error."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _product_error(a, b):
+    """bound on the error of a . b (64-bit copies of fp32 operands), elementwise"""
+    K = a.shape[1]
+    aa, bb = np.abs(a), np.abs(b)
+    fl = 2.0 ** -38 * (aa.max(initial=0.0) * bb.sum(0)[None, :] + bb.max(initial=0.0) * aa.sum(1)[:, None])
+    return (12 + 6 * np.sqrt(3 * K)) * U * (aa @ bb) + fl
+
+
+def _reference(x, w, b, t, mean=True, ignore=-100, e=0.0):
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    N, V = x.shape[0], w.shape[1]
+    l = x @ w
+    E = _product_error(x, w)
+    if b is not None:
+        l = l + b.astype(np.float64).reshape(1, -1)
+    E = (E + U * np.where(np.isfinite(l), np.abs(l), 0.0)).max(1, keepdims=True)
+    counted = (t != ignore)
+    m = l.max(1, keepdims=True)
+    p = np.exp(l - m)
+    z = p.sum(1, keepdims=True)
+    lse = np.log(z) + m
+    p = p / z
+    q = np.full((N, V), e / V)
+    at = np.where(counted, t, 0).astype(np.int64)
+    q[np.arange(N), at] += 1 - e
+    lt = l[np.arange(N), at][:, None]
+    row = lse - (1 - e) * lt - (e * l.mean(1, keepdims=True) if e else 0.0)
+    trow = 3 * E + U * (V / 256 + 60) * (1 + np.abs(lse - lt)) + (U * (V / 256 + 30) * np.abs(l - m).mean(1, keepdims=True) if e else 0.0)
+    count = max(1, int(counted.sum())) if mean else 1
+    keep = counted[:, None].astype(np.float64)
+    loss = float((row * keep).sum() / count)
+    tloss = float((trow * keep).sum() / count) + U * (N / 256 + 12) * float((np.abs(row) * keep).sum() / count) + 1e-30
+    dl = (p - q) * keep
+    td = (p * (2 * E + (V / 256 + 40) * U) + 4 * U * (p + q) + 2.0 ** -22 * np.abs(dl) + 2.0 ** -38) * keep
+    dx, dw, db = dl @ w.T / count, x.T @ dl / count, dl.sum(0) / count
+    tdx = (_product_error(dl, w.T) + td @ np.abs(w).T) / count + 4 * U * np.abs(dx)
+    tdw = (_product_error(x.T, dl) + np.abs(x).T @ td) / count + 4 * U * np.abs(dw)
+    tdb = (td.sum(0) + (N / 64 + 30) * U * np.abs(dl).sum(0)) / count + 4 * U * np.abs(db)
+    tiny = 1e-30
+    return (loss, tloss), (dx, tdx + tiny), (dw, tdw + tiny), (db, tdb + tiny)
+
+
+def _within(got, want, tol, what):
+    got = np.asarray(got, np.float64).reshape(np.shape(want))
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (f"{what}: {bad.sum()} of {bad.size} off; worst {np.abs(got - want)[bad].max():.3e} "
+                           f"against {np.asarray(tol)[bad].min() if np.ndim(tol) else tol:.3e}")
+
+
+def _data(N, D, V, seed, ignored=0.0, ignore=-100, bias=True):
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((N, D)).astype(np.float32)
+    w = (rng.standard_normal((D, V)) * 1.5 / np.sqrt(D)).astype(np.float32)
+    b = rng.standard_normal((1, V)).astype(np.float32) if bias else None
+    t = rng.integers(0, V, N).astype(np.float32)
+    t[rng.random(N) < ignored] = ignore
+    return x, w, b, t
+
+
+def _run(dev, x, w, b, t, scale=None, **kw):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    xt, wt = Tensor(x, device=dev, requires_grad=True), Tensor(w, device=dev, requires_grad=True)
+    bt = Tensor(b, device=dev, requires_grad=True) if b is not None else None
+    loss = F.linear_cross_entropy(xt, wt, bt, Tensor(t, device=dev), **kw)
+    assert tuple(loss.shape) == (1,)
+    value = float(loss.numpy()[0])
+    (loss if scale is None else loss * scale).backward()
+    out = value, xt.grad.numpy(), wt.grad.numpy(), (bt.grad.numpy() if b is not None else None)
+    Graph.free_graph_all()
+    return out
+
+
+def _check(dev, x, w, b, t, scale=None, **kw):
+    got = _run(dev, x, w, b, t, scale, **kw)
+    ref = _reference(x, w, b, t, kw.get("reduction", "mean") == "mean", kw.get("ignore_index", -100), kw.get("label_smoothing", 0.0))
+    s = 1.0 if scale is None else abs(scale)
+    _within(got[0], ref[0][0], ref[0][1], "loss")
+    for g, (want, tol), what in zip(got[1:], ref[1:], ("dx", "dw", "db")):
+        if g is not None:
+            _within(g, (scale or 1.0) * want, s * tol + 2 * U * s * np.abs(want), what)
+
+
+SHAPES = [(1, 1, 1), (1, 1, 2), (3, 5, 7), (1, 64, 1000), (2, 33, 31), (31, 32, 33), (64, 256, 1000), (130, 100, 257), (257, 129, 511),
+          (300, 48, 4099), (65, 300, 640), (1000, 17, 129), (33, 1031, 77), (512, 512, 512), (640, 256, 2100), (7, 40, 20011)]
+
+
+@pytest.mark.parametrize("N,D,V", SHAPES)
+def test_values_and_gradients(hip_device, N, D, V):
+    _check(hip_device, *_data(N, D, V, N + D + V))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 1.0])
+@pytest.mark.parametrize("ignore", [-100, 3])
+def test_smoothing_reductions_and_rows_that_are_not_counted(hip_device, reduction, smoothing, ignore):
+    x, w, b, t = _data(150, 70, 333, 5, ignored=0.3, ignore=ignore)
+    _check(hip_device, x, w, b, t, reduction=reduction, label_smoothing=smoothing, ignore_index=ignore)
+
+
+def test_without_a_bias(hip_device):
+    _check(hip_device, *_data(90, 64, 700, 6, bias=False))
+
+
+@pytest.mark.parametrize("scale", [0.5, -3.0])
+def test_an_upstream_gradient_other_than_one(hip_device, scale):
+    _check(hip_device, *_data(50, 40, 300, 7), scale=scale)
+
+
+def test_no_row_is_counted(hip_device):
+    x, w, b, t = _data(20, 16, 50, 8)
+    t[:] = -100
+    loss, dx, dw, db = _run(hip_device, x, w, b, t)
+    assert loss == 0.0 and not dx.any() and not dw.any() and not db.any()
+
+
+def test_rows_that_are_not_counted_leave_their_inputs_alone(hip_device):
+    """what stands in a row that is not counted does not matter for the others, nor does it reach its own gradient"""
+    x, w, b, t = _data(70, 32, 200, 9, ignored=0.4)
+    first = _run(hip_device, x, w, b, t)
+    y = x.copy()
+    y[t == -100] *= 3.0
+    second = _run(hip_device, y, w, b, t)
+    ref = _reference(x, w, b, t)
+    _within(second[0], ref[0][0], 2 * ref[0][1], "loss")
+    assert not second[1][t == -100].any() and not first[1][t == -100].any()
+    for g, (want, tol) in zip(second[1:], ref[1:]):
+        _within(g, want, 4 * tol, "gradient")
+
+
+def test_bad_targets_show(hip_device):
+    x, w, b, t = _data(40, 24, 100, 10)
+    for bad in (100.0, -1.0, 2.5, np.nan, np.inf, 1e9):
+        u = t.copy()
+        u[17] = bad
+        loss, dx, dw, db = _run(hip_device, x, w, b, u)
+        assert np.isnan(loss) and np.all(np.isnan(dx[17])) and np.all(np.isnan(dw)) and np.all(np.isnan(db))
+        assert np.all(np.isfinite(np.delete(dx, 17, axis=0)))
+
+
+def test_classes_masked_by_the_bias(hip_device):
+    """a bias of -inf, or of the type's lowest value, takes a class out: probability 0, gradient 0"""
+    x, w, b, t = _data(60, 48, 300, 11)
+    out = np.zeros(300, bool)
+    out[5::7] = True
+    t = np.array([v if not out[int(v)] else 0.0 for v in t], np.float32)
+    ref = _reference(x, w[:, ~out], b[:, ~out], np.searchsorted(np.nonzero(~out)[0], t).astype(np.float32))
+    for low in (-np.inf, np.finfo(np.float32).min):
+        c = b.copy()
+        c[0, out] = low
+        loss, dx, dw, db = _run(hip_device, x, w, c, t)
+        _within(loss, ref[0][0], ref[0][1], "loss")
+        _within(dx, ref[1][0], 2 * ref[1][1], "dx")
+        _within(dw[:, ~out], ref[2][0], 2 * ref[2][1], "dw")
+        assert not dw[:, out].any() and not db[0, out].any()
+
+
+def test_a_row_that_is_not_finite_stays_in_its_row(hip_device):
+    x, w, b, t = _data(45, 30, 90, 12)
+    for bad in (np.nan, np.inf):
+        y = x.copy()
+        y[11, 3] = bad
+        loss, dx, _, _ = _run(hip_device, y, w, b, t, reduction="sum")
+        assert np.isnan(loss) and np.all(np.isnan(dx[11]))
+        ref = _reference(np.delete(x, 11, 0), w, b, np.delete(t, 11), mean=False)
+        _within(np.delete(dx, 11, 0), ref[1][0], 2 * ref[1][1], "dx")
+
+
+@pytest.mark.parametrize("sx,sw", [(1e-15, 1e15), (1e12, 1e-12), (1e-30, 1.0), (1.0, 1e-30), (0.0, 1.0), (1.0, 0.0)])
+def test_operands_of_any_magnitude(hip_device, sx, sw):
+    x, w, b, t = _data(40, 60, 130, 13)
+    _check(hip_device, (x * np.float32(sx)), (w * np.float32(sw)), b, t)
+
+
+def test_large_logits(hip_device):
+    """probabilities of 0 and 1 to the last bit"""
+    x, w, b, t = _data(64, 50, 400, 14)
+    _check(hip_device, 20 * x, 5 * w, b, t)
+
+
+def test_strided_operands_and_a_flat_bias(hip_device):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x, w, b, t = _data(33, 20, 60, 15)
+    dev = hip_device
+    loss = F.linear_cross_entropy(Tensor(np.ascontiguousarray(x.T), device=dev).transpose(),
+                                  Tensor(np.ascontiguousarray(w.T), device=dev).transpose(), Tensor(b.reshape(-1), device=dev),
+                                  Tensor(t, device=dev))
+    ref = _reference(x, w, b, t)
+    _within(float(loss.numpy()[0]), ref[0][0], ref[0][1], "loss")
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_one_gradient_at_a_time(hip_device, which):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    x, w, b, t = _data(80, 48, 210, 16)
+    ts = [Tensor(a, device=hip_device, requires_grad=k == which) for k, a in enumerate((x, w, b))]
+    F.linear_cross_entropy(*ts, Tensor(t, device=hip_device)).backward()
+    want, tol = _reference(x, w, b, t)[1 + which]
+    _within(ts[which].grad.numpy(), want, tol, "gradient")
+    assert all(ts[k].grad is None for k in range(3) if k != which)
+    Graph.free_graph_all()
+
+
+def test_evaluation_and_training_agree(hip_device):
+    from deepflows_amd import nn
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.tensor import Graph, Tensor
+    x, w, b, t = _data(100, 64, 900, 17, ignored=0.2)
+    fc = nn.Linear(64, 900, device=hip_device)
+    fc.weight.data, fc.bias.data = Tensor(w, device=hip_device).data, Tensor(b, device=hip_device).data
+    crit = nn.LinearCrossEntropyLoss(fc, label_smoothing=0.05)
+    xt, tt = Tensor(x, device=hip_device), Tensor(t, device=hip_device)
+    train = crit(xt, tt)
+    with no_grad():
+        held_out = crit(xt, tt)
+    ref = _reference(x, w, b, t, e=0.05)
+    for v in (train, held_out):
+        _within(float(v.numpy()[0]), ref[0][0], ref[0][1], "loss")
+    Graph.free_graph_all()
+
+
+def test_several_pieces_of_rows(hip_device):
+    """more rows x classes than one piece holds (512 MB of logits): 140 M of them"""
+    _check(hip_device, *_data(1400, 20, 100003, 18, ignored=0.1), label_smoothing=0.1)
+
+
+def test_no_rows(hip_device):
+    from deepflows_amd.backend_selection import BackendTensor
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    w = Tensor(np.ones((4, 6), np.float32), device=hip_device, requires_grad=True)
+    b = Tensor(np.ones((1, 6), np.float32), device=hip_device, requires_grad=True)
+    loss = F.linear_cross_entropy(Tensor(BackendTensor.make((0, 4), device=hip_device)), w, b,
+                                  Tensor(BackendTensor.make((0,), device=hip_device)))
+    loss.backward()
+    assert float(loss.numpy()[0]) == 0.0 and not w.grad.numpy().any() and not b.grad.numpy().any()
+    Graph.free_graph_all()
+
+
+def test_gradients_against_differences(hip_device):
+    rng = np.random.default_rng(19)
+    x, w, b, t = _data(6, 9, 14, 19)
+    _, dx, dw, db = _run(hip_device, x, w, b, t, label_smoothing=0.2)
+
+    def value(x, w, b):
+        return _reference(x, w, b, t, e=0.2)[0][0]
+
+    args = [a.astype(np.float64) for a in (x, w, b)]
+    for k, got in enumerate((dx, dw, db)):
+        for _ in range(6):
+            at = tuple(int(rng.integers(0, s)) for s in args[k].shape)
+            up, dn = [a.copy() for a in args], [a.copy() for a in args]
+            up[k][at] += 1e-5
+            dn[k][at] -= 1e-5
+            slope = (value(*up) - value(*dn)) / 2e-5
+            # (differences in 64 bits: 1e-10; fp32 values of at most order 1 with sums of 14 and 9 terms: 64 u)
+            assert abs(got[at] - slope) <= 64 * U * (1 + abs(slope))
+
+
+def test_two_sweeps_over_a_retained_graph_and_a_held_gradient(hip_device):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    x, w, b, t = _data(30, 20, 50, 20)
+    ts = [Tensor(a, device=hip_device, requires_grad=True) for a in (x, w, b)]
+    loss = F.linear_cross_entropy(*ts, Tensor(t, device=hip_device))
+    loss.backward(retain_graph=True)
+    first = [p.grad.numpy().copy() for p in ts]
+    loss.backward()                                            # (added to what the leaves hold)
+    for p, g in zip(ts, first):
+        assert np.array_equal(p.grad.numpy(), 2 * g)
+    Graph.free_graph_all()
+
+
+def test_inside_a_captured_graph(hip_device):
+    """two graphs over different shapes captured one after the other, replayed in turn on changed inputs with eager calls between"""
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    mod = hip_device.mod
+    made = []
+    for k, (N, D, V) in enumerate([(96, 64, 1500), (40, 100, 333)]):
+        x, w, b, t = _data(N, D, V, 30 + k, ignored=0.2)
+        leaves = [Tensor(a, device=hip_device, requires_grad=True) for a in (x, w, b)]
+        tt = Tensor(t, device=hip_device)
+
+        def step(leaves=leaves, tt=tt):
+            for p in leaves:
+                p.grad = None
+            loss = F.linear_cross_entropy(*leaves, tt, label_smoothing=0.1)
+            loss.backward()
+            return [loss.data] + [p.grad for p in leaves]
+
+        step()
+        mod.capture_begin()
+        got = step()
+        made.append((leaves, tt, step, got, mod.capture_end(keep=got), (N, D, V)))
+    for r in range(3):
+        for k, (leaves, tt, step, got, graph, shape) in enumerate(made):
+            x, w, b, t = _data(*shape, 100 + 10 * r + k, ignored=0.1)
+            for p, a in zip(leaves + [tt], (x, w, b, t)):
+                mod.from_numpy(a, p.data._handle)
+        for m in made:
+            m[4].replay()
+        replayed = [[g.numpy().copy() for g in m[3]] for m in made]
+        for m, rep in zip(made, replayed):
+            for a, c in zip(rep, m[2]()):
+                assert np.array_equal(a, c.numpy())
+    for m in made:
+        m[4].destroy()
+    Graph.free_graph_all()
+
+
+def test_refusals(hip_device):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x, w, b, t = (Tensor(a, device=hip_device) for a in _data(8, 6, 10, 21))
+    bad = lambda shape: Tensor(np.zeros(shape, np.float32), device=hip_device)
+    for args, kw in [((x, bad((7, 10)), b, t), {}), ((x, w, bad((1, 9)), t), {}), ((x, w, b, bad((7,))), {}),
+                     ((x, w, b, bad((8, 10))), {}), ((bad((2, 4, 6)), w, b, t), {}), ((x, w, b, t), {"reduction": "none"}),
+                     ((x, w, b, t), {"label_smoothing": 1.5}), ((x, w, b, t), {"label_smoothing": float("nan")}),
+                     ((x, w, b, t), {"ignore_index": 0.5})]:
+        with pytest.raises(ValueError):
+            F.linear_cross_entropy(*args, **kw)
+    s = bad((6, 6))
+    with pytest.raises(ValueError):
+        F.linear_cross_entropy(s, s, None, bad((6,)))
+    mod = hip_device.mod
+    h = lambda v: v.data._handle
+    one = bad((1,))
+    for rows, width, classes, ign, sm in [(-1, 6, 10, -100, 0.0), (8, 0, 10, -100, 0.0), (8, 6, 0, -100, 0.0),
+                                          (8, 6, (1 << 24) + 1, -100, 0.0), (8, 6, 10, 1 << 25, 0.0), (8, 6, 10, -100, -0.1)]:
+        with pytest.raises(ValueError):
+            mod.linear_ce_forward(h(x), h(w), None, h(t), h(one), None, None, None, rows, width, classes, ign, sm, True)

@@ -75,3 +75,39 @@ def test_clip_refusals(cpu_oracle):
     params[0].grad.fill(np.inf)
     with pytest.raises(RuntimeError):
         optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.2])
+def test_linear_cross_entropy_composition(cpu_oracle, smoothing):
+    from deepflows_amd import nn
+    from deepflows_amd.tensor import Tensor
+    rng = np.random.default_rng(2)
+    x, t = rng.standard_normal((6, 5)).astype(np.float32), np.array([0, 6, -100, 3, 3, -100], np.float32)
+    fc = nn.Linear(5, 7, device=cpu_oracle)
+    xt = Tensor(x, device=cpu_oracle, requires_grad=True)
+    loss = nn.LinearCrossEntropyLoss(fc, label_smoothing=smoothing)(xt, Tensor(t, device=cpu_oracle))
+    l = x.astype(np.float64) @ fc.weight.numpy() + fc.bias.numpy()
+    lp = l - l.max(1, keepdims=True)
+    lp -= np.log(np.exp(lp).sum(1, keepdims=True))
+    q = np.full((6, 7), smoothing / 7)
+    q[np.arange(6), np.where(t < 0, 0, t).astype(int)] += 1 - smoothing
+    q[t < 0] = 0
+    assert_close(loss.numpy(), [-(lp * q).sum() / 4], 1e-6)
+    loss.backward()
+    dl = np.where((t < 0)[:, None], 0, np.exp(lp) - q) / 4
+    assert_close(xt.grad.numpy(), dl @ fc.weight.numpy().T, 1e-5)
+    assert_close(fc.weight.grad.numpy(), x.T @ dl, 1e-5)
+    assert_close(fc.bias.grad.numpy(), dl.sum(0, keepdims=True), 1e-5)
+
+
+def test_linear_cross_entropy_refusals(cpu_oracle):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    new = lambda *s: Tensor(np.zeros(s, np.float32), device=cpu_oracle)
+    x, w, b, t = new(4, 3), new(3, 5), new(1, 5), new(4)
+    for args, kw in [((x, new(4, 5), b, t), {}), ((x, w, new(1, 4), t), {}), ((x, w, b, new(4, 5)), {}),
+                     ((x, w, b, t), {"reduction": "none"}), ((x, w, b, t), {"label_smoothing": -0.1}),
+                     ((x, w, b, Tensor(np.full(4, 5.0), device=cpu_oracle)), {}),
+                     ((x, w, b, Tensor(np.full(4, 0.5), device=cpu_oracle)), {})]:
+        with pytest.raises(ValueError):
+            F.linear_cross_entropy(*args, **kw)
