@@ -1,0 +1,247 @@
+// fp32 products on the fp16 matrix cores: every operand is held as TWO fp16 values whose sum carries 22 bits of it, and a
+// product is formed from three of the four partial products, accumulated in fp32.
+//
+//   v 2^-e = hi + lo,  hi = fp16(v 2^-e),  lo = fp16(v 2^-e - hi):  |error| <= 2^-22 |v| (and 2^-39 of the array's largest
+//   magnitude A, with e chosen so that A 2^-e lies in [2^13, 2^14): from there down to 2^-17 A both halves are normal numbers)
+//   a b = hi hi' + hi lo' + lo hi'  (+ lo lo' <= 2^-22 |a b|, left out)
+// (the scheme is published: Ootomo and Yokota, "Recovering single precision accuracy from Tensor Cores while surpassing the FP32
+// theoretical peak performance", 2022).  Against fp32 MFMA (157 TFLOP/s) the fp16 rate is 16 times as high, a third of it is left:
+// measured error and time beside the caller, dfhip_vocab.hip.
+//
+// STORAGE ("split array"): a padded row-major array of 4-byte cells, columns in blocks of 32: 128 bytes that hold the block's 32
+// hi halves, then its 32 lo halves.  A cell takes as much room as the fp32 value it stands for, so an fp32 array can be converted
+// in place block by block, and ONE copy of an array serves as either operand of a product:
+//   the reduction runs along the rows of the storage ("K along"): a tile is 128-byte pieces of BM rows, read as 16-byte fragments;
+//   the reduction runs across them ("K across"): a tile is 32 rows of 4 BM bytes, read with the transposing LDS loads
+//   (ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 halves, each lane receives the 4 rows of its column).
+//
+// KERNEL: workgroup tile BM x BN, K step 32, two LDS buffers filled by 16-byte global-to-LDS copies that are issued a step ahead;
+// one barrier a step.  32 x 32 x 16 MFMA; a wave owns (BM / WM) x (BN / WN).  LDS positions are XOR-permuted at 16-byte
+// granularity by the ROW (the copy's source address is permuted, its LDS side is linear): 16 lanes that read the same piece of 16
+// rows, or 32 lanes that read 4 rows transposed, touch every bank once.
+// LDS reads: three products share two fragments a side, so the LDS moves half the bytes an fp16 GEMM of the same rate would.
+#pragma once
+#include "dfhip_internal.h"
+
+namespace dfhip_split {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTop = 13;                 // the largest magnitude of an operand is scaled into [2^13, 2^14)
+constexpr int kPad = 256;                // rows and columns of a split array are padded with zeros to a multiple of this
+
+__host__ __device__ inline int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
+
+// one scaled value as hi + lo; what is not finite stays in hi alone
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  const float r = v - (float)hi;
+  lo = (_Float16)(r == r ? r : 0.0f);    // (inf - inf, NaN: no low half)
+}
+
+enum { EPI_BIAS = 0, EPI_SLAB = 1, EPI_STORE = 2, EPI_ADD = 3 };
+
+struct Gemm {
+  const char *a, *b;                     // split arrays
+  int64_t lda, ldb;                      // bytes a storage row
+  int tiles_m, tiles_n, splits;
+  int ksteps, ksteps_split;              // steps of 32 along the reduction, in all and for one split
+  float* c;
+  int64_t ldc, slab;                     // elements; EPI_SLAB: elements between two splits' results
+  int m, n;                              // EPI_STORE / EPI_ADD: what lies outside is not written; EPI_BIAS: columns with a bias
+  const float* bias;                     // EPI_BIAS, or NULL
+  const int* exp_a;                      // result = 2^(exp_a + exp_b + exp_c) * scale * accumulator; each NULL or on the device
+  const int* exp_b;
+  int exp_c;
+  const float* scale;
+};
+
+template <int BM, int NW, bool ACROSS>
+struct Loader {
+  static constexpr int J = BM / 8 / NW;  // 1024-byte copies a wave and step
+  const char* p[J];
+  int64_t step;
+  __device__ __forceinline__ void init(const char* base, int64_t ld, int64_t r0, int kstep0, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < J; i++) {
+      const int j = wave * J + i;
+      if (ACROSS) {
+        const int o = j * 1024 + lane * 16;
+        const int k = o / (BM * 4);
+        const int c = ((o % (BM * 4)) >> 4) ^ ((k & 3) << 2);
+        p[i] = base + ((int64_t)kstep0 * 32 + k) * ld + r0 * 4 + c * 16;
+      } else {
+        const int row = 8 * j + (lane >> 3);
+        const int c = (lane & 7) ^ ((row >> 1) & 7);
+        p[i] = base + (r0 + row) * ld + (int64_t)kstep0 * 128 + c * 16;
+      }
+    }
+    step = ACROSS ? 32 * ld : 128;
+  }
+  __device__ __forceinline__ void issue(char* lds, int wave) {
+#pragma unroll
+    for (int i = 0; i < J; i++) {
+      // (written out because the compiler, which cannot tell the two buffers apart, waits for the builtin's copies in front of
+      // the next LDS read; there is no output register, nothing else here uses m0, and the kernel's own wait and barrier order
+      // the copies)
+      const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
+                                                         (unsigned)(wave * J + i) * 1024u);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p[i]) : "memory");
+      p[i] += step;
+    }
+  }
+};
+
+// fragments of T tiles of 32 rows (columns) from row w0 of an LDS tile of BM, for the half step kk (16 of the 32), plane 0 hi / 1 lo
+template <int BM, bool ACROSS>
+struct Reader {
+  int off[4];
+  __device__ __forceinline__ void init(int w0, int lane) {
+    if (ACROSS) {
+      const int k = (lane >> 5) * 8 + ((lane & 15) >> 2);
+      const int x = (lane & 15) >> 2;              // k & 3
+      const int q = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+#pragma unroll
+      for (int par = 0; par < 2; par++)
+#pragma unroll
+        for (int plane = 0; plane < 2; plane++)
+          off[par * 2 + plane] = k * (BM * 4) + (w0 >> 6) * 256 + (((8 * par + 4 * plane + q) ^ (x << 2)) << 4) + (lane & 1) * 8;
+    } else {
+      const int x = ((lane & 31) >> 1) & 7;
+#pragma unroll
+      for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+        for (int plane = 0; plane < 2; plane++)
+          off[kk * 2 + plane] = (w0 + (lane & 31)) * 128 + (((plane * 4 + kk * 2 + (lane >> 5)) ^ x) << 4);
+    }
+  }
+  // tile i, counted from w0 (w0 is a multiple of 64 where the reduction runs across)
+  __device__ __forceinline__ half8 get(const char* lds, int i, int kk, int plane) const {
+    if (ACROSS) {
+      const char* s = lds + off[(i & 1) * 2 + plane] + (i >> 1) * 256 + kk * 16 * (BM * 4);
+      const short4v v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)s);
+      const short4v v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(s + 4 * (BM * 4)));
+      typedef short short8v __attribute__((ext_vector_type(8)));
+      const short8v v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(half8, v);
+    }
+    return *reinterpret_cast<const half8*>(lds + off[kk * 2 + plane] + i * 4096);
+  }
+};
+
+template <int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
+  constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (rows fastest), so that the
+  // tiles that share a column of B meet in one L2
+  const int total = g.tiles_m * g.tiles_n * g.splits, per = (total + 7) >> 3;
+  const int tile = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  if (((int)blockIdx.x >> 3) >= per || tile >= total) return;
+  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m % g.tiles_n, z = tile / (g.tiles_m * g.tiles_n);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int k0 = z * g.ksteps_split, steps = min(g.ksteps - k0, g.ksteps_split);
+  const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+
+  Loader<BM, NW, AX> la;
+  Loader<BN, NW, BX> lb;
+  la.init(g.a, g.lda, m0, k0, wave, lane);
+  lb.init(g.b, g.ldb, n0, k0, wave, lane);
+  Reader<BM, AX> ra;
+  Reader<BN, BX> rb;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+
+  if (steps > 0) {
+    la.issue(lds, wave);
+    lb.issue(lds + ABYTES, wave);
+  }
+  for (int s = 0; s < steps; s++) {
+    // this wave's copies of step s have landed and its reads of step s - 1 are back; behind the barrier everybody's are
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const char* cur = lds + (s & 1) * STAGE;
+    char* nxt = lds + ((s + 1) & 1) * STAGE;
+    if (s + 1 < steps) {
+      la.issue(nxt, wave);
+      lb.issue(nxt + ABYTES, wave);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) {
+      half8 ah[TM], al[TM], bh[TN], bl[TN];
+#pragma unroll
+      for (int i = 0; i < TM; i++) { ah[i] = ra.get(cur, i, kk, 0); al[i] = ra.get(cur, i, kk, 1); }
+#pragma unroll
+      for (int j = 0; j < TN; j++) { bh[j] = rb.get(cur + ABYTES, j, kk, 0); bl[j] = rb.get(cur + ABYTES, j, kk, 1); }
+      // (the same accumulator comes up again after TM * TN products)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+    }
+  }
+
+  int e = g.exp_c;
+  if (g.exp_a) e += g.exp_a[0];
+  if (g.exp_b) e += g.exp_b[0];
+  const float sc = g.scale ? g.scale[0] : 1.0f;
+  float* c = g.c + (EPI == EPI_SLAB ? (int64_t)z * g.slab : 0);
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    const int64_t n = n0 + wn + j * 32 + (lane & 31);
+    float b = 0.0f;
+    if (EPI == EPI_BIAS && g.bias && n < g.n) b = g.bias[n];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int64_t m = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        const float v = acc[i][j][r];
+        if (EPI == EPI_BIAS) c[m * g.ldc + n] = ldexpf(v, e) + b;
+        if (EPI == EPI_SLAB) c[m * g.ldc + n] = v;
+        if (EPI == EPI_STORE && m < g.m && n < g.n) c[m * g.ldc + n] = ldexpf(v, e) * sc;
+        if (EPI == EPI_ADD && m < g.m && n < g.n) c[m * g.ldc + n] += ldexpf(v, e) * sc;
+      }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
+int launch(const Gemm& g) {
+  constexpr int lds = 2 * (BM + BN) * 128;
+  static bool set = false;
+  if (lds > 65536 && !set) {
+    DF_HIP(hipFuncSetAttribute((const void*)k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>,
+                               hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    set = true;
+  }
+  const int64_t total = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  DF_CHECK_ARG(total > 0 && total < (1 << 28), "split product: %lld tiles", (long long)total);
+  DF_LAUNCH((k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WM * WN * 64), lds,
+            dfhip::stream(), g);
+  DF_LAUNCH_CHECK();
+  return DFHIP_OK;
+}
+
+}  // namespace dfhip_split

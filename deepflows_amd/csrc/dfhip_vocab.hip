@@ -7,94 +7,339 @@
 // The rows go through in pieces: the logits of one piece exist at a time, become dl in place and are consumed by the two
 // products, so memory does not grow with rows x classes.  The gradients are formed in the forward pass, for an upstream
 // gradient of 1: nothing is computed twice (recomputing the logits in a backward pass would be a third more products).
+//
+// The three products run on the fp16 matrix cores with fp32 accuracy (dfhip_splitgemm.h): x and W are converted once a call,
+// dl where it is formed.  The launches of a call:
+//   k_lce_scan     the largest magnitudes of x and W (finite elements only)
+//   k_lce_split    x, W -> split arrays; the number of counted rows
+//   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> [k_lce_colsum] -> dx
+//                  product -> dW product (both [+ k_lce_slabs where the reduction is cut])
+//   k_lce_finish   loss, db
 #include <math.h>
 
 #include <algorithm>
 
-#include "dfhip_internal.h"
+#include "dfhip_splitgemm.h"
 
 using namespace dfhip;
+using namespace dfhip_split;
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kScan = 512;                                 // workgroups (= partial maxima) a tensor
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;        // the logits of one piece of the rows
 
-// per call: 0 number of counted rows
-__global__ __launch_bounds__(kThreads) void k_lce_count(const float* __restrict__ target, int64_t rows, float ignore,
-                                                        float* __restrict__ ctl) {
-  __shared__ int sh[kThreads / 64];
-  int n = 0;
-  for (int64_t i = threadIdx.x; i < rows; i += kThreads) n += target[i] != ignore ? 1 : 0;
-#pragma unroll
-  for (int off = 32; off; off >>= 1) n += __shfl_xor(n, off);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
-  __syncthreads();
-  if (threadIdx.x == 0) ctl[0] = (float)(sh[0] + sh[1] + sh[2] + sh[3]);
-}
+// what the launches of one call hand to each other
+struct Ctl {
+  float scale;                                             // 1 / number of counted rows, or 1
+  int ex, ew;                                              // x = 2^ex * split array, W likewise
+  int pad;
+  float max_x[kScan], max_w[kScan];
+};
 
-template <class F>
-__device__ __forceinline__ float block_reduce(float v, float* sh, F f) {
+template <int T, class X, class F>
+__device__ __forceinline__ X block_reduce(X v, X* sh, F f) {
 #pragma unroll
   for (int off = 32; off; off >>= 1) v = f(v, __shfl_xor(v, off));
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
   v = sh[0];
-  for (int w = 1; w < kThreads / 64; w++) v = f(v, sh[w]);
+#pragma unroll
+  for (int w = 1; w < T / 64; w++) v = f(v, sh[w]);
   return v;
 }
+struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Add {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+  __device__ __forceinline__ int operator()(int a, int b) const { return a + b; }
+};
 
-// a workgroup a row: the row's loss, and dl over its logits
-__global__ __launch_bounds__(kThreads) void k_lce_rows(float* __restrict__ logits, const float* __restrict__ target,
-                                                       const float* __restrict__ ctl, float* __restrict__ rowloss, int64_t V,
-                                                       float ignore, float smooth, int mean, int grads) {
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.4028235e38f ? a : 0.0f;                    // (inf and NaN: 0)
+}
+
+// workgroups 0 .. kScan-1: x, kScan .. 2 kScan - 1: W
+__global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__ x, int64_t nx, const float* __restrict__ w,
+                                                       int64_t nw, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
-  float* l = logits + (int64_t)blockIdx.x * V;
-  const float t = target[blockIdx.x];
-  if (t == ignore) {
-    if (threadIdx.x == 0) rowloss[blockIdx.x] = 0.0f;
-    if (grads)
-      for (int64_t v = threadIdx.x; v < V; v += kThreads) l[v] = 0.0f;
+  const bool second = blockIdx.x >= kScan;
+  const float* p = second ? w : x;
+  const int64_t n = second ? nw : nx;
+  const int blk = (int)blockIdx.x & (kScan - 1);
+  float m = 0.0f;
+  int64_t lo = 0;
+  if ((((uintptr_t)p) & 15) == 0) {
+    const float4* p4 = reinterpret_cast<const float4*>(p);
+    const int64_t n4 = n >> 2, step = (int64_t)kScan * kThreads;
+    int64_t i = (int64_t)blk * kThreads + threadIdx.x;
+    for (; i + 3 * step < n4; i += 4 * step) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) v[u] = p4[i + u * step];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        m = fmaxf(fmaxf(m, fmaxf(finite_abs(v[u].x), finite_abs(v[u].y))), fmaxf(finite_abs(v[u].z), finite_abs(v[u].w)));
+    }
+    for (; i < n4; i += step) {
+      const float4 v = p4[i];
+      m = fmaxf(fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y))), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+    }
+    lo = n4 << 2;
+  }
+  for (int64_t i = lo + (int64_t)blk * kThreads + threadIdx.x; i < n; i += (int64_t)kScan * kThreads) m = fmaxf(m, finite_abs(p[i]));
+  m = block_reduce<kThreads>(m, sh, Max());
+  if (threadIdx.x == 0) (second ? ctl->max_w : ctl->max_x)[blk] = m;
+}
+
+// eight columns of one storage row a thread; workgroups [0, bx): x, [bx, bx + bw): W, the last one: the counted rows
+__global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict__ x, int64_t rows, int64_t width,
+                                                        const float* __restrict__ w, int64_t classes, char* __restrict__ xs,
+                                                        char* __restrict__ ws, const float* __restrict__ target, float ignore,
+                                                        int mean, int64_t bx, int64_t bw, Ctl* __restrict__ ctl) {
+  __shared__ float sh[kThreads / 64];
+  __shared__ int shi[kThreads / 64];
+  if (blockIdx.x == bx + bw) {
+    int n = 0;
+    for (int64_t i = threadIdx.x; i < rows; i += kThreads) n += target[i] != ignore ? 1 : 0;
+    n = block_reduce<kThreads>(n, shi, Add());
+    if (threadIdx.x == 0) ctl->scale = mean ? 1.0f / (float)max(n, 1) : 1.0f;
     return;
   }
-  const bool ok = t >= 0.0f && t < (float)V && t == floorf(t);
-  const int64_t ti = ok ? (int64_t)t : 0;
-  float m = -INFINITY;
-  for (int64_t v = threadIdx.x; v < V; v += kThreads) m = fmaxf(m, l[v]);
-  m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
-  float z = 0.0f, s = 0.0f;
-  for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-    z += expf(l[v] - m);
-    s += l[v] - m;
+  const bool second = blockIdx.x >= bx;
+  const float* part = second ? ctl->max_w : ctl->max_x;
+  float m = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kScan / kThreads; u++) m = fmaxf(m, part[threadIdx.x + u * kThreads]);
+  m = block_reduce<kThreads>(m, sh, Max());
+  const int e = m > 0.0f ? ilogbf(m) - kTop : 0;
+  if (threadIdx.x == 0 && blockIdx.x == (second ? bx : 0)) (second ? ctl->ew : ctl->ex) = e;
+  const float* src = second ? w : x;
+  char* dst = second ? ws : xs;
+  const int64_t nr = second ? width : rows, nc = second ? classes : width;
+  const int64_t pr = padded(nr), pc = padded(nc), groups = pr * (pc >> 3);
+  const int64_t nblk = second ? bw : bx;
+  const bool vec = (nc & 3) == 0 && (((uintptr_t)src) & 15) == 0;
+  for (int64_t i = ((int64_t)blockIdx.x - (second ? bx : 0)) * kThreads + threadIdx.x; i < groups; i += nblk * kThreads) {
+    const int64_t r = i / (pc >> 3), c = (i - r * (pc >> 3)) << 3;
+    float v[8];
+    if (r < nr && c + 8 <= nc && vec) {
+      const float4 a = *reinterpret_cast<const float4*>(src + r * nc + c), b = *reinterpret_cast<const float4*>(src + r * nc + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = (r < nr && c + k < nc) ? src[r * nc + c + k] : 0.0f;
+    }
+    half8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      _Float16 h, l;
+      split(ldexpf(v[k], -e), h, l);
+      hi[k] = h; lo[k] = l;
+    }
+    char* d = dst + r * pc * 4 + (c >> 5) * 128 + (c & 31) * 2;
+    *reinterpret_cast<half8*>(d) = hi;
+    *reinterpret_cast<half8*>(d + 64) = lo;
   }
-  z = block_reduce(z, sh, [](float a, float b) { return a + b; });
-  s = block_reduce(s, sh, [](float a, float b) { return a + b; });
-  const float lt = l[ti] - m;
-  __syncthreads();                                 // (every thread has read the target's logit before it is overwritten)
+}
+
+// e^x for x <= 0: 2^(x log2(e)) with the product's rounding error and the constant's own put back to first order (|x| times
+// 2^-24 otherwise), results below 2^-126 as 0.  Half the instructions of expf, whose range checks nothing here needs.
+__device__ __forceinline__ float exp_of(float x) {
+  constexpr double kLog2e = 1.4426950408889634;
+  constexpr float hi = (float)kLog2e, lo = (float)(kLog2e - (double)(float)kLog2e);
+  x = x < -200.0f ? -200.0f : x;                           // (-inf; a NaN stays one)
+  const float t = x * hi, e = fmaf(x, lo, fmaf(x, hi, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, e * 0.6931471805599453f, p);
+}
+
+// A workgroup a row: the row's loss, and dl (times 2^kTop) over its logits as a split array.  `cells` is the padded row, a
+// multiple of 256; a row that is not counted, or lies behind the last one (blockIdx.x >= rows), becomes zeros.
+// U > 0: U groups of eight logits a thread hold the row in registers (T * 8 * U >= cells), one pass over memory each way;
+// U = 0: any length, the row read three times.
+template <int T, int U>
+__global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, const float* __restrict__ target, int rows,
+                                                float* __restrict__ rowloss, int classes, int cells, float ignore, float smooth,
+                                                int grads) {
+  __shared__ float sh[T / 64];
+  float* l = logits + (int64_t)blockIdx.x * cells;
+  const bool exists = (int)blockIdx.x < rows;
+  const float t = exists ? target[blockIdx.x] : ignore;
+  auto store = [&](int c, const float* v) {                // eight cells from column c (a multiple of 8)
+    half8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      _Float16 h, q;
+      split(v[k], h, q);
+      hi[k] = h; lo[k] = q;
+    }
+    char* d = reinterpret_cast<char*>(l) + (c >> 5) * 128 + (c & 31) * 2;
+    *reinterpret_cast<half8*>(d) = hi;
+    *reinterpret_cast<half8*>(d + 64) = lo;
+  };
+  if (t == ignore) {
+    if (threadIdx.x == 0 && exists) rowloss[blockIdx.x] = 0.0f;
+    if (grads)
+      for (int c = threadIdx.x * 4; c < cells; c += T * 4) *reinterpret_cast<float4*>(l + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    return;
+  }
+  const bool ok = t >= 0.0f && t < (float)classes && t == floorf(t);
+  const int ti = ok ? (int)t : 0;
+  const float lt = l[ti];
+  constexpr int UU = U > 0 ? U : 1;
+  const int trips = U > 0 ? 1 : (cells + T * 8 - 1) / (T * 8);
+  float v[UU][8];
+  // (the column is made new for every pass: the compiler otherwise keeps each pass's comparisons of it for the next ones, two
+  // masks a group, and spills)
+  auto first = [&]() {
+    int c0 = (int)threadIdx.x * 8;
+    asm volatile("" : "+v"(c0));
+    return c0;
+  };
+  auto load = [&](int trip) {                              // -inf behind the last class
+    const int c0 = first();
+#pragma unroll
+    for (int u = 0; u < UU; u++) {
+      const int c = (trip * UU + u) * T * 8 + c0;
+      if (c < cells) {
+        const float4 a = *reinterpret_cast<const float4*>(l + c), b = *reinterpret_cast<const float4*>(l + c + 4);
+        v[u][0] = a.x; v[u][1] = a.y; v[u][2] = a.z; v[u][3] = a.w; v[u][4] = b.x; v[u][5] = b.y; v[u][6] = b.z; v[u][7] = b.w;
+      }
+      if (c + 8 > classes)                                 // (a branch that few waves take: a mask a value would cost registers)
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[u][k] = c + k < classes ? v[u][k] : -INFINITY;
+    }
+  };
+  float m = -INFINITY;
+  for (int i = 0; i < trips; i++) {
+    load(i);
+#pragma unroll
+    for (int u = 0; u < UU; u++)
+#pragma unroll
+      for (int k = 0; k < 8; k++) m = fmaxf(m, v[u][k]);   // (passes a NaN over; its exponential makes z one)
+  }
+  m = block_reduce<T>(m, sh, Max());
+  float z = 0.0f, s = 0.0f;
+  for (int i = 0; i < trips; i++) {
+    if (U == 0) load(i);
+    const int c0 = first();
+#pragma unroll
+    for (int u = 0; u < UU; u++) {
+      const int c = (i * UU + u) * T * 8 + c0;
+      if (smooth > 0.0f) {
+        if (c + 8 <= classes) {
+#pragma unroll
+          for (int k = 0; k < 8; k++) s += v[u][k] - m;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; k++) s += c + k < classes ? v[u][k] - m : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        v[u][k] = exp_of(v[u][k] - m);
+        z += v[u][k];
+      }
+    }
+  }
+  z = block_reduce<T>(z, sh, Add());
+  if (smooth > 0.0f) s = block_reduce<T>(s, sh, Add());
   if (threadIdx.x == 0) {
-    float r = logf(z) - (1.0f - smooth) * lt;
-    if (smooth > 0.0f) r -= smooth * (s / (float)V);
+    float r = logf(z) - (1.0f - smooth) * (lt - m);
+    if (smooth > 0.0f) r -= smooth * (s / (float)classes);
     rowloss[blockIdx.x] = ok ? r : NAN;
   }
   if (!grads) return;
-  const float scale = mean ? 1.0f / fmaxf(ctl[0], 1.0f) : 1.0f;
-  const float iz = 1.0f / z, q = smooth / (float)V;
-  for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-    float d = expf(l[v] - m) * iz - q;
-    if (v == ti) d -= 1.0f - smooth;
-    l[v] = ok ? d * scale : NAN;
+  const float top = (float)(1 << kTop), iz = ok ? top / z : NAN, q = top * (smooth / (float)classes), p1 = top * (1.0f - smooth);
+  for (int i = 0; i < trips; i++) {
+    if (U == 0) {
+      load(i);
+#pragma unroll
+      for (int u = 0; u < UU; u++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[u][k] = exp_of(v[u][k] - m);
+    }
+    const int c0 = first();
+#pragma unroll
+    for (int u = 0; u < UU; u++) {
+      const int c = (i * UU + u) * T * 8 + c0;
+      if (c < cells) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[u][k] = fmaf(v[u][k], iz, -q);
+        if ((unsigned)(ti - c) < 8u)
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[u][k] -= c + k == ti ? p1 : 0.0f;
+        if (c + 8 > classes)
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[u][k] = c + k < classes ? v[u][k] : 0.0f;
+        store(c, v[u]);
+      }
+    }
   }
 }
 
-// loss = sum of the row losses (/ the number of counted rows), in a fixed order
-__global__ __launch_bounds__(kThreads) void k_lce_loss(const float* __restrict__ rowloss, const float* __restrict__ ctl,
-                                                       float* __restrict__ loss, int64_t rows, int mean) {
-  __shared__ float sh[kThreads / 64];
+// column sums of a piece's dl: a workgroup takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows
+__global__ __launch_bounds__(kThreads) void k_lce_colsum(const char* __restrict__ dl, int rows, int64_t cells,
+                                                         float* __restrict__ partial) {
+  __shared__ float sh[8][256];
+  const int col = ((int)threadIdx.x & 31) * 8, sub = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 256 + col;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const char* p = dl + (c >> 5) * 128 + (c & 31) * 2;
+  for (int r = (int)blockIdx.y * 8 + sub; r < rows; r += (int)gridDim.y * 8) {
+    const half8 hi = *reinterpret_cast<const half8*>(p + (int64_t)r * cells * 4);
+    const half8 lo = *reinterpret_cast<const half8*>(p + (int64_t)r * cells * 4 + 64);
+#pragma unroll
+    for (int k = 0; k < 8; k++) s[k] += (float)hi[k] + (float)lo[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; k++) sh[sub][col + k] = s[k];
+  __syncthreads();
+  float t = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 8; g++) t += sh[g][threadIdx.x];
+  partial[(int64_t)blockIdx.y * cells + (int64_t)blockIdx.x * 256 + threadIdx.x] = t;
+}
+
+// db (+)= 2^-kTop scale * sum of the partial rows
+__global__ __launch_bounds__(kThreads) void k_lce_db(const float* __restrict__ partial, int n, int64_t cells,
+                                                     float* __restrict__ db, int classes, const Ctl* __restrict__ ctl, int add) {
+  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (c >= classes) return;
   float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows; i += kThreads) s += rowloss[i];
-  s = block_reduce(s, sh, [](float a, float b) { return a + b; });
-  if (threadIdx.x == 0) loss[0] = mean ? s / fmaxf(ctl[0], 1.0f) : s;
+  for (int i = 0; i < n; i++) s += partial[i * cells + c];
+  s = ldexpf(s, -kTop) * ctl->scale;
+  db[c] = add ? db[c] + s : s;
+}
+
+// out (m, n) (+)= 2^(...) scale * sum over the splits, in their order
+__global__ __launch_bounds__(kThreads) void k_lce_slabs(const float* __restrict__ slabs, int splits, int64_t slab, int64_t lds_,
+                                                        float* __restrict__ out, int64_t m, int64_t n,
+                                                        const int* __restrict__ exp_in, const Ctl* __restrict__ ctl, int add) {
+  const int e = exp_in[0] - kTop;
+  const float sc = ctl->scale;
+  const int64_t total = m * n;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t r = i / n, c = i - r * n;
+    const float* p = slabs + r * lds_ + c;
+    float s = 0.0f;
+    for (int z = 0; z < splits; z++) s += p[z * slab];
+    s = ldexpf(s, e) * sc;
+    out[i] = add ? out[i] + s : s;
+  }
+}
+
+// loss = sum of the row losses times the scale, in a fixed order
+__global__ __launch_bounds__(1024) void k_lce_loss(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl,
+                                                   float* __restrict__ loss, int64_t rows) {
+  __shared__ float sh[1024 / 64];
+  float s = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += rowloss[i];
+  s = block_reduce<1024>(s, sh, Add());
+  if (threadIdx.x == 0) loss[0] = s * ctl->scale;
 }
 
 __global__ __launch_bounds__(kThreads) void k_lce_scale(const float* __restrict__ src, const float* __restrict__ scalar,
@@ -106,7 +351,85 @@ __global__ __launch_bounds__(kThreads) void k_lce_scale(const float* __restrict_
 struct Held {                                      // a pool block for the duration of a call (its reuse is stream-ordered)
   float* p = nullptr;
   ~Held() { if (p) (void)dfhip_free(p); }
+  int take(int64_t floats) { return p ? DFHIP_OK : dfhip_malloc(floats, &p); }
 };
+
+// tile of a product of m x n outputs and `steps` steps of 32: 256 x 256 (one workgroup a CU) where that gives every CU work,
+// 128 x 128 (two a CU) otherwise; `cut`: the reduction may be cut into splits of at least 8 steps
+struct Plan { bool big; int splits, steps_split; };
+Plan plan(int64_t m, int64_t n, int steps, bool cut) {
+  const int64_t t256 = df_ceil_div(m, 256) * df_ceil_div(n, 256), t128 = df_ceil_div(m, 128) * df_ceil_div(n, 128);
+  Plan p;
+  p.big = cut ? t256 * steps >= (int64_t)num_cus() * 24 : t256 * 4 >= (int64_t)num_cus() * 3;
+  const int64_t tiles = p.big ? t256 : t128, want = p.big ? num_cus() : 2 * num_cus();
+  int64_t s = cut && tiles < want ? want / tiles : 1;
+  s = std::max<int64_t>(1, std::min<int64_t>(s, steps / 8));
+  p.steps_split = (int)df_ceil_div(steps, s);
+  p.splits = (int)df_ceil_div(steps, p.steps_split);
+  return p;
+}
+
+template <bool AX, bool BX, int EPI>
+int product(Gemm& g, const Plan& p, int64_t m, int64_t n) {
+  const int t = p.big ? 256 : 128;
+  g.tiles_m = (int)df_ceil_div(m, t);
+  g.tiles_n = (int)df_ceil_div(n, t);
+  g.splits = p.splits;
+  g.ksteps_split = p.steps_split;
+  return p.big ? launch<256, 256, 2, 4, AX, BX, EPI>(g) : launch<128, 128, 2, 2, AX, BX, EPI>(g);
+}
+
+// out (m, n) (+)= 2^(e - kTop) scale * a . b; the reduction may be cut, the cut sums meet in `slabs`
+template <bool AX, bool BX>
+int gradient_product(Gemm g, int64_t m, int64_t n, float* out, bool add, const int* e, const Ctl* ctl, Held& slabs,
+                     int64_t& held) {
+  const Plan p = plan(m, n, g.ksteps, true);
+  g.m = (int)m;
+  g.n = (int)n;
+  g.exp_a = e;
+  g.exp_b = nullptr;
+  g.exp_c = -kTop;
+  g.scale = &ctl->scale;
+  g.bias = nullptr;
+  if (p.splits == 1) {
+    g.c = out;
+    g.ldc = n;
+    g.slab = 0;
+    return add ? product<AX, BX, EPI_ADD>(g, p, m, n) : product<AX, BX, EPI_STORE>(g, p, m, n);
+  }
+  g.ldc = padded(n);
+  g.slab = padded(m) * g.ldc;
+  if (held < p.splits * g.slab) {
+    if (slabs.p) { (void)dfhip_free(slabs.p); slabs.p = nullptr; }
+    held = p.splits * g.slab;
+    const int st = slabs.take(held);
+    if (st != DFHIP_OK) return st;
+  }
+  g.c = slabs.p;
+  const int st = product<AX, BX, EPI_SLAB>(g, p, m, n);
+  if (st != DFHIP_OK) return st;
+  DF_LAUNCH(k_lce_slabs, dim3((unsigned)std::min<int64_t>(df_ceil_div(m * n, kThreads), 8192)), dim3(kThreads), 0, stream(),
+            slabs.p, p.splits, g.slab, g.ldc, out, m, n, e, ctl, add ? 1 : 0);
+  DF_LAUNCH_CHECK();
+  return DFHIP_OK;
+}
+
+int rows_pass(float* logits, const float* target, int n, int launch_rows, float* rowloss, int classes, int cells, float ignore,
+              float smooth, int grads) {
+#define ROWS(T, U)                                                                                                        \
+  DF_LAUNCH((k_lce_rows<T, U>), dim3((unsigned)launch_rows), dim3(T), 0, stream(), logits, target, n, rowloss, classes,   \
+            cells, ignore, smooth, grads)
+  if (cells <= 2048) ROWS(256, 1);
+  else if (cells <= 4096) ROWS(256, 2);
+  else if (cells <= 8192) ROWS(1024, 1);
+  else if (cells <= 16384) ROWS(1024, 2);
+  else if (cells <= 32768) ROWS(1024, 4);
+  else if (cells <= 57344) ROWS(1024, 7);
+  else ROWS(1024, 0);
+#undef ROWS
+  DF_LAUNCH_CHECK();
+  return DFHIP_OK;
+}
 
 }  // namespace
 
@@ -118,7 +441,7 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   DF_INIT();
   DF_CHECK_ARG(rows >= 0 && width >= 1 && classes >= 1, "linear_ce_forward: bad extents (%lld, %lld, %lld)", (long long)rows,
                (long long)width, (long long)classes);
-  DF_CHECK_ARG(rows <= 0x7fffffff && width <= 0x7fffffff, "linear_ce_forward: rows and width must be below 2^31");
+  DF_CHECK_ARG(rows <= (1 << 30) && width <= (1 << 24), "linear_ce_forward: at most 2^30 rows and a width of 2^24");
   DF_CHECK_ARG(classes <= (1 << 24), "linear_ce_forward: at most 2^24 classes (their indices are whole numbers held in fp32)");
   DF_CHECK_ARG(ignore_index >= -(1 << 24) && ignore_index <= (1 << 24), "linear_ce_forward: ignore_index must be within 2^24");
   DF_CHECK_ARG(label_smoothing >= 0.0 && label_smoothing <= 1.0, "linear_ce_forward: label_smoothing must be in [0, 1]");
@@ -132,35 +455,79 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     return st;
   }
   const bool grads = dx || dw || db;
-  const int64_t piece = std::min(rows, std::max<int64_t>(1, kPieceBytes / (4 * classes)));
-  Held logits, stats, more;
-  int st = dfhip_malloc(piece * classes, &logits.p);
-  if (st == DFHIP_OK) st = dfhip_malloc(rows + 1, &stats.p);
-  if (st == DFHIP_OK && piece < rows && (dw || db)) st = dfhip_malloc(std::max(dw ? width * classes : 0, classes), &more.p);
+  const int64_t np = padded(rows), dp = padded(width), vp = padded(classes);
+  // pieces of about the same length, a multiple of 256 rows
+  const int64_t cap = std::max<int64_t>(256, kPieceBytes / (4 * vp) / 256 * 256), pieces = df_ceil_div(rows, cap);
+  const int64_t piece = padded(df_ceil_div(rows, pieces));
+  constexpr int kColSlices = 32;
+  Held xs, ws, logits, small, slabs;
+  int64_t held = 0;
+  int st = small.take((int64_t)(sizeof(Ctl) / 4) + rows + (db ? kColSlices * vp : 0));
+  if (st == DFHIP_OK) st = xs.take(np * dp);
+  if (st == DFHIP_OK) st = ws.take(dp * vp);
+  if (st == DFHIP_OK) st = logits.take(piece * vp);
   if (st != DFHIP_OK) return st;
-  float *ctl = stats.p, *rowloss = stats.p + 1;
+  Ctl* ctl = reinterpret_cast<Ctl*>(small.p);
+  float *partial = small.p + sizeof(Ctl) / 4, *rowloss = partial + (db ? kColSlices * vp : 0);
   const float ignore = (float)ignore_index;
-  DF_LAUNCH(k_lce_count, dim3(1), dim3(kThreads), 0, stream(), target, rows, ignore, ctl);
+  ProfScope prof("linear_ce", (grads ? 6.0 : 2.0) * (double)rows * (double)width * (double)classes,
+                 4.0 * (grads ? 2.0 : 1.0) * ((double)rows * width + (double)width * classes));
+
+  DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows * width, w, width * classes, ctl);
   DF_LAUNCH_CHECK();
+  const int64_t bx = std::min<int64_t>(df_ceil_div(np * dp / 8, kThreads), 2048), bw = std::min<int64_t>(df_ceil_div(dp * vp / 8, kThreads), 4096);
+  DF_LAUNCH(k_lce_split, dim3((unsigned)(bx + bw + 1)), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p,
+            (char*)ws.p, target, ignore, mean, bx, bw, ctl);
+  DF_LAUNCH_CHECK();
+
   for (int64_t r0 = 0; r0 < rows; r0 += piece) {
     const int64_t n = std::min(piece, rows - r0);
-    st = dfhip_gemm(x + r0 * width, w, bias, logits.p, n, width, classes, 0, 0);
+    Gemm g = {};
+    g.a = (const char*)xs.p + r0 * dp * 4;
+    g.lda = dp * 4;
+    g.b = (const char*)ws.p;
+    g.ldb = vp * 4;
+    g.ksteps = (int)df_ceil_div(width, 32);
+    g.c = logits.p;
+    g.ldc = vp;
+    g.n = (int)classes;
+    g.bias = bias;
+    g.exp_a = &ctl->ex;
+    g.exp_b = &ctl->ew;
+    st = product<false, true, EPI_BIAS>(g, plan(n, classes, g.ksteps, false), n, classes);
     if (st != DFHIP_OK) return st;
-    DF_LAUNCH(k_lce_rows, dim3((unsigned)n), dim3(kThreads), 0, stream(), logits.p, target + r0, ctl, rowloss + r0, classes,
-              ignore, (float)label_smoothing, mean, grads ? 1 : 0);
-    DF_LAUNCH_CHECK();
-    if (dx) st = dfhip_gemm(logits.p, w, nullptr, dx + r0 * width, n, classes, width, 0, 1);
-    if (st == DFHIP_OK && dw) {
-      st = dfhip_gemm(x + r0 * width, logits.p, nullptr, r0 ? more.p : dw, width, n, classes, 1, 0);
-      if (st == DFHIP_OK && r0) st = dfhip_axpy(dw, more.p, 1.0f, width * classes);
-    }
-    if (st == DFHIP_OK && db) {
-      st = dfhip_reduce_axis(logits.p, r0 ? more.p : db, 1, n, classes, 0, 1.0f);
-      if (st == DFHIP_OK && r0) st = dfhip_axpy(db, more.p, 1.0f, classes);
-    }
+    st = rows_pass(logits.p, target + r0, (int)n, (int)(grads ? df_ceil_div(n, 32) * 32 : n), rowloss + r0, (int)classes, (int)vp,
+                   ignore, (float)label_smoothing, grads ? 1 : 0);
     if (st != DFHIP_OK) return st;
+    if (db) {
+      const int slices = (int)std::min<int64_t>(kColSlices, df_ceil_div(n, 32));
+      DF_LAUNCH(k_lce_colsum, dim3((unsigned)(vp / 256), (unsigned)slices), dim3(kThreads), 0, stream(), (const char*)logits.p, (int)n,
+                vp, partial);
+      DF_LAUNCH_CHECK();
+      DF_LAUNCH(k_lce_db, dim3((unsigned)df_ceil_div(classes, kThreads)), dim3(kThreads), 0, stream(), partial, slices, vp, db,
+                (int)classes, ctl, r0 ? 1 : 0);
+      DF_LAUNCH_CHECK();
+    }
+    if (dx) {
+      g.a = (const char*)logits.p;
+      g.lda = vp * 4;
+      g.b = (const char*)ws.p;
+      g.ldb = vp * 4;
+      g.ksteps = (int)df_ceil_div(classes, 32);
+      st = gradient_product<false, false>(g, n, width, dx + r0 * width, false, &ctl->ew, ctl, slabs, held);
+      if (st != DFHIP_OK) return st;
+    }
+    if (dw) {
+      g.a = (const char*)xs.p + r0 * dp * 4;
+      g.lda = dp * 4;
+      g.b = (const char*)logits.p;
+      g.ldb = vp * 4;
+      g.ksteps = (int)df_ceil_div(n, 32);
+      st = gradient_product<true, true>(g, width, classes, dw, r0 > 0, &ctl->ex, ctl, slabs, held);
+      if (st != DFHIP_OK) return st;
+    }
   }
-  DF_LAUNCH(k_lce_loss, dim3(1), dim3(kThreads), 0, stream(), rowloss, ctl, loss, rows, mean);
+  DF_LAUNCH(k_lce_loss, dim3(1), dim3(1024), 0, stream(), rowloss, ctl, loss, rows);
   DF_LAUNCH_CHECK();
   return DFHIP_OK;
 }
