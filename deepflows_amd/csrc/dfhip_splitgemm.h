@@ -21,6 +21,8 @@
 // rows, or 32 lanes that read 4 rows transposed, touch every bank once.
 // LDS reads: three products share two fragments a side, so the LDS moves half the bytes an fp16 GEMM of the same rate would.
 #pragma once
+#include <algorithm>
+
 #include "dfhip_internal.h"
 
 namespace dfhip_split {
@@ -42,22 +44,47 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(r == r ? r : 0.0f);    // (inf - inf, NaN: no low half)
 }
 
-enum { EPI_BIAS = 0, EPI_SLAB = 1, EPI_STORE = 2, EPI_ADD = 3 };
+enum { EPI_BIAS = 0, EPI_STORE = 1, EPI_ADD = 2 };
 
+// Tiles [0, full) are formed by one workgroup each.  The `rest` tiles behind them -- what would be a last round that leaves most
+// of the chip idle -- are cut along the reduction into `splits` parts of `ksteps_split` steps; their partial tiles go to `parts`
+// and k_split_rest adds them up, in order, and applies the epilogue.
 struct Gemm {
   const char *a, *b;                     // split arrays
   int64_t lda, ldb;                      // bytes a storage row
-  int tiles_m, tiles_n, splits;
-  int ksteps, ksteps_split;              // steps of 32 along the reduction, in all and for one split
+  int tiles_m, full, rest, splits;
+  int ksteps, ksteps_split;              // steps of 32 along the reduction, in all and for a part
   float* c;
-  int64_t ldc, slab;                     // elements; EPI_SLAB: elements between two splits' results
+  int64_t ldc;
   int m, n;                              // EPI_STORE / EPI_ADD: what lies outside is not written; EPI_BIAS: columns with a bias
   const float* bias;                     // EPI_BIAS, or NULL
   const int* exp_a;                      // result = 2^(exp_a + exp_b + exp_c) * scale * accumulator; each NULL or on the device
   const int* exp_b;
   int exp_c;
   const float* scale;
+  float* colsum;                         // or NULL: column sums of b (n), scaled by 2^exp_c * scale; added where EPI_ADD (b across)
+  float* parts;                          // (rest * splits) x (BM * BN + BN)
 };
+
+template <int EPI>
+__device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
+  return EPI == EPI_BIAS && g.bias && n < g.n ? g.bias[n] : 0.0f;
+}
+template <int EPI>
+__device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias, int64_t m, int64_t n, float v) {
+  if (EPI == EPI_BIAS) g.c[m * g.ldc + n] = ldexpf(v, e) + bias;
+  if (EPI == EPI_STORE && m < g.m && n < g.n) g.c[m * g.ldc + n] = ldexpf(v, e) * sc;
+  if (EPI == EPI_ADD && m < g.m && n < g.n) g.c[m * g.ldc + n] += ldexpf(v, e) * sc;
+}
+template <int EPI>
+__device__ __forceinline__ void emit_colsum(const Gemm& g, float sc, int64_t n, float v) {
+  if (n >= g.n) return;
+  v = ldexpf(v, g.exp_c) * sc;
+  g.colsum[n] = EPI == EPI_ADD ? g.colsum[n] + v : v;
+}
+__device__ __forceinline__ int exponent(const Gemm& g) {
+  return g.exp_c + (g.exp_a ? g.exp_a[0] : 0) + (g.exp_b ? g.exp_b[0] : 0);
+}
 
 template <int BM, int NW, bool ACROSS>
 struct Loader {
@@ -140,13 +167,17 @@ __global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (rows fastest), so that the
   // tiles that share a column of B meet in one L2
-  const int total = g.tiles_m * g.tiles_n * g.splits, per = (total + 7) >> 3;
-  const int tile = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-  if (((int)blockIdx.x >> 3) >= per || tile >= total) return;
-  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m % g.tiles_n, z = tile / (g.tiles_m * g.tiles_n);
+  const bool whole = (int)blockIdx.x < (g.full + 7) / 8 * 8;
+  const int id = whole ? (int)blockIdx.x : (int)blockIdx.x - (g.full + 7) / 8 * 8;
+  const int total = whole ? g.full : g.rest * g.splits, per = (total + 7) >> 3;
+  const int item = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || item >= total) return;
+  const int z = whole ? 0 : item / g.rest, tile = whole ? item : g.full + item % g.rest;
+  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int k0 = z * g.ksteps_split, steps = min(g.ksteps - k0, g.ksteps_split);
+  const int k0 = whole ? 0 : z * g.ksteps_split, steps = whole ? g.ksteps : min(g.ksteps - k0, g.ksteps_split);
   const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
+  const bool sums = BX && g.colsum && tm == 0 && wm == 0;
 
   f32x16 acc[TM][TN];
 #pragma unroll
@@ -155,6 +186,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
     for (int j = 0; j < TN; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+  float col[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) col[j] = 0.0f;
 
   Loader<BM, NW, AX> la;
   Loader<BN, NW, BX> lb;
@@ -200,30 +234,90 @@ __global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
       for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+      if (BX && sums) {                            // (a lane holds eight rows of one column)
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+          float t = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 8; k++) t += (float)bh[j][k] + (float)bl[j][k];
+          col[j] += t;
+        }
+      }
     }
   }
 
-  int e = g.exp_c;
-  if (g.exp_a) e += g.exp_a[0];
-  if (g.exp_b) e += g.exp_b[0];
+  const int e = exponent(g);
   const float sc = g.scale ? g.scale[0] : 1.0f;
-  float* c = g.c + (EPI == EPI_SLAB ? (int64_t)z * g.slab : 0);
+  float* part = whole ? nullptr : g.parts + (int64_t)((tile - g.full) * g.splits + z) * (BM * BN + BN);
+  if (BX && sums) {
 #pragma unroll
-  for (int j = 0; j < TN; j++) {
-    const int64_t n = n0 + wn + j * 32 + (lane & 31);
-    float b = 0.0f;
-    if (EPI == EPI_BIAS && g.bias && n < g.n) b = g.bias[n];
+    for (int j = 0; j < TN; j++) {
+      const float t = col[j] + __shfl_xor(col[j], 32);
+      if (lane < 32) {
+        if (whole) emit_colsum<EPI>(g, sc, n0 + wn + j * 32 + lane, t);
+        else part[BM * BN + wn + j * 32 + lane] = t;
+      }
+    }
+  }
+  if (!whole) {
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          part[(wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * BN + wn + j * 32 + (lane & 31)] = acc[i][j][r];
+    return;
+  }
+  float bias[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) bias[j] = bias_of<EPI>(g, n0 + wn + j * 32 + (lane & 31));
+#pragma unroll
+  for (int j = 0; j < TN; j++)
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int64_t m = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        const float v = acc[i][j][r];
-        if (EPI == EPI_BIAS) c[m * g.ldc + n] = ldexpf(v, e) + b;
-        if (EPI == EPI_SLAB) c[m * g.ldc + n] = v;
-        if (EPI == EPI_STORE && m < g.m && n < g.n) c[m * g.ldc + n] = ldexpf(v, e) * sc;
-        if (EPI == EPI_ADD && m < g.m && n < g.n) c[m * g.ldc + n] += ldexpf(v, e) * sc;
-      }
+      for (int r = 0; r < 16; r++)
+        emit<EPI>(g, e, sc, bias[j], m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n0 + wn + j * 32 + (lane & 31),
+                  acc[i][j][r]);
+}
+
+// the parts of the cut tiles added up: 1024 cells of one tile a workgroup, four a thread
+template <int BM, int BN, int EPI>
+__global__ __launch_bounds__(256) void k_split_rest(Gemm g) {
+  constexpr int SLICES = BM * BN / 1024, CELLS = BM * BN + BN;
+  const int t = (int)blockIdx.x / SLICES, slice = (int)blockIdx.x % SLICES, tile = g.full + t;
+  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const float* part = g.parts + (int64_t)t * g.splits * CELLS;
+  const int e = exponent(g);
+  const float sc = g.scale ? g.scale[0] : 1.0f;
+  const int cell = slice * 1024 + (int)threadIdx.x * 4;
+  const float* p = part + cell;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  int z = 0;
+  for (; z + 8 <= g.splits; z += 8) {              // eight loads in flight
+    float4 q[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) q[k] = *reinterpret_cast<const float4*>(p + (int64_t)(z + k) * CELLS);
+#pragma unroll
+    for (int k = 0; k < 8; k++) { v[0] += q[k].x; v[1] += q[k].y; v[2] += q[k].z; v[3] += q[k].w; }
+  }
+  for (; z < g.splits; z++) {
+    const float4 q = *reinterpret_cast<const float4*>(p + (int64_t)z * CELLS);
+    v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+  }
+  const int64_t n = n0 + cell % BN;
+  float bias[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) bias[k] = bias_of<EPI>(g, n + k);
+#pragma unroll
+  for (int k = 0; k < 4; k++) emit<EPI>(g, e, sc, bias[k], m0 + cell / BN, n + k, v[k]);
+  if (g.colsum && tm == 0 && slice == 0 && (int)threadIdx.x < BN) {
+    const float* c = part + BM * BN + threadIdx.x;
+    float s = 0.0f;
+    for (int y = 0; y < g.splits; y++) s += c[(int64_t)y * CELLS];
+    emit_colsum<EPI>(g, sc, n0 + threadIdx.x, s);
   }
 }
 
@@ -236,12 +330,48 @@ int launch(const Gemm& g) {
                                hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     set = true;
   }
-  const int64_t total = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  DF_CHECK_ARG(total > 0 && total < (1 << 28), "split product: %lld tiles", (long long)total);
-  DF_LAUNCH((k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WM * WN * 64), lds,
-            dfhip::stream(), g);
+  const int64_t groups = (int64_t)((g.full + 7) / 8 + ((int64_t)g.rest * g.splits + 7) / 8) * 8;
+  DF_LAUNCH((k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>), dim3((unsigned)groups), dim3(WM * WN * 64), lds, dfhip::stream(), g);
   DF_LAUNCH_CHECK();
+  if (g.rest) {
+    DF_LAUNCH((k_split_rest<BM, BN, EPI>), dim3((unsigned)g.rest * (BM * BN / 1024)), dim3(256), 0, dfhip::stream(), g);
+    DF_LAUNCH_CHECK();
+  }
   return DFHIP_OK;
 }
+
+// How a product of m x n outputs and `steps` steps runs: the tile, and which tiles are cut.  Costs in microseconds, measured on
+// long reductions: a step of a round is 1.25 with 256 x 256 tiles (one workgroup a CU) and 0.8 with 128 x 128 (two); a part costs its
+// share of writing and adding up (0.1 and 0.025), a cut product another launch (5).
+struct Plan { bool big; int tiles_m, tiles_n, full, rest, splits, ksteps_split; double us; };
+inline Plan plan(int64_t m, int64_t n, int steps) {
+  Plan best = {};
+  for (int big = 0; big < 2; big++) {
+    const int64_t t = big ? 256 : 128, slots = (big ? 1 : 2) * (int64_t)dfhip::num_cus();
+    const double step_us = big ? 1.25 : 0.8, part_us = big ? 0.1 : 0.025;
+    const int64_t tm = (m + t - 1) / t, tn = (n + t - 1) / t, tiles = tm * tn;
+    if (tiles > (1 << 28)) continue;
+    for (int cut = 0; cut < 2; cut++) {
+      const int64_t rest = cut ? tiles % slots : 0;
+      if (cut && !rest) continue;
+      Plan p = {big != 0, (int)tm, (int)tn, (int)(tiles - rest), (int)rest, 1, steps, 0.0};
+      p.us = (double)((p.full + slots - 1) / slots) * steps * step_us;
+      if (cut) {
+        double least = 1e30;
+        const int64_t most = std::min<int64_t>(slots / rest, steps / 4);
+        if (most < 2) continue;
+        for (int64_t s = 2; s <= most; s++) {
+          const int64_t ks = (steps + s - 1) / s, real = (steps + ks - 1) / ks;
+          const double us = (double)ks * step_us + (double)(rest * real) * part_us + 5.0;
+          if (us < least) { least = us; p.splits = (int)real; p.ksteps_split = (int)ks; }
+        }
+        p.us += least;
+      }
+      if (best.us == 0.0 || p.us < best.us) best = p;
+    }
+  }
+  return best;
+}
+inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.big ? 256 * 256 + 256 : 128 * 128 + 128); }
 
 }  // namespace dfhip_split

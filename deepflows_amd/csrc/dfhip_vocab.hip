@@ -12,9 +12,9 @@
 // dl where it is formed.  The launches of a call:
 //   k_lce_scan     the largest magnitudes of x and W (finite elements only)
 //   k_lce_split    x, W -> split arrays; the number of counted rows
-//   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> [k_lce_colsum] -> dx
-//                  product -> dW product (both [+ k_lce_slabs where the reduction is cut])
-//   k_lce_finish   loss, db
+//   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> dx product ->
+//                  dW product (db on the side: the column sums of its second operand)
+//   k_lce_loss     loss
 #include <math.h>
 
 #include <algorithm>
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kScan = 512;                                 // workgroups (= partial maxima) a tensor
-constexpr int64_t kPieceBytes = (int64_t)512 << 20;        // the logits of one piece of the rows
+constexpr int64_t kPieceBytes = (int64_t)2 << 30;          // the logits of one piece of the rows
 
 // what the launches of one call hand to each other
 struct Ctl {
@@ -94,13 +94,15 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
   if (threadIdx.x == 0) (second ? ctl->max_w : ctl->max_x)[blk] = m;
 }
 
-// eight columns of one storage row a thread; workgroups [0, bx): x, [bx, bx + bw): W, the last one: the counted rows
+// workgroups [0, bx): x, [bx, bx + bw): W, the last one: the counted rows.  A wave takes 512 consecutive cells of the padded
+// array at a time, eight a lane; where rows do not begin on 16 bytes it reads them lane by lane and turns them in LDS.
 __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict__ x, int64_t rows, int64_t width,
                                                         const float* __restrict__ w, int64_t classes, char* __restrict__ xs,
                                                         char* __restrict__ ws, const float* __restrict__ target, float ignore,
                                                         int mean, int64_t bx, int64_t bw, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
   __shared__ int shi[kThreads / 64];
+  __shared__ __attribute__((aligned(16))) float turn[kThreads / 64][512];
   if (blockIdx.x == bx + bw) {
     int n = 0;
     for (int64_t i = threadIdx.x; i < rows; i += kThreads) n += target[i] != ignore ? 1 : 0;
@@ -119,18 +121,36 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   const float* src = second ? w : x;
   char* dst = second ? ws : xs;
   const int64_t nr = second ? width : rows, nc = second ? classes : width;
-  const int64_t pr = padded(nr), pc = padded(nc), groups = pr * (pc >> 3);
+  const int64_t pr = padded(nr), pc = padded(nc), units = pr * pc / 512;      // (a multiple of 4: the workgroup stays together)
   const int64_t nblk = second ? bw : bx;
   const bool vec = (nc & 3) == 0 && (((uintptr_t)src) & 15) == 0;
-  for (int64_t i = ((int64_t)blockIdx.x - (second ? bx : 0)) * kThreads + threadIdx.x; i < groups; i += nblk * kThreads) {
-    const int64_t r = i / (pc >> 3), c = (i - r * (pc >> 3)) << 3;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int64_t u0 = ((int64_t)blockIdx.x - (second ? bx : 0)) * 4; u0 < units; u0 += nblk * 4) {
+    const int64_t first = (u0 + wave) * 512, r0 = first / pc, c0 = first - r0 * pc;
+    int64_t r = r0, c = c0 + lane * 8;
+    while (c >= pc) { c -= pc; r++; }
     float v[8];
-    if (r < nr && c + 8 <= nc && vec) {
-      const float4 a = *reinterpret_cast<const float4*>(src + r * nc + c), b = *reinterpret_cast<const float4*>(src + r * nc + c + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    if (vec) {
+      if (r < nr && c + 8 <= nc) {
+        const float4 a = *reinterpret_cast<const float4*>(src + r * nc + c), b = *reinterpret_cast<const float4*>(src + r * nc + c + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = (r < nr && c + k < nc) ? src[r * nc + c + k] : 0.0f;
+      }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = (r < nr && c + k < nc) ? src[r * nc + c + k] : 0.0f;
+      for (int k = 0; k < 8; k++) {
+        int64_t rk = r0, ck = c0 + k * 64 + lane;
+        while (ck >= pc) { ck -= pc; rk++; }
+        v[k] = (rk < nr && ck < nc) ? src[rk * nc + ck] : 0.0f;
+      }
+      __syncthreads();                             // (the last trip's values have been read)
+#pragma unroll
+      for (int k = 0; k < 8; k++) turn[wave][k * 64 + lane] = v[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = turn[wave][lane * 8 + k];
     }
     half8 hi, lo;
 #pragma unroll
@@ -281,57 +301,6 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   }
 }
 
-// column sums of a piece's dl: a workgroup takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows
-__global__ __launch_bounds__(kThreads) void k_lce_colsum(const char* __restrict__ dl, int rows, int64_t cells,
-                                                         float* __restrict__ partial) {
-  __shared__ float sh[8][256];
-  const int col = ((int)threadIdx.x & 31) * 8, sub = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 256 + col;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const char* p = dl + (c >> 5) * 128 + (c & 31) * 2;
-  for (int r = (int)blockIdx.y * 8 + sub; r < rows; r += (int)gridDim.y * 8) {
-    const half8 hi = *reinterpret_cast<const half8*>(p + (int64_t)r * cells * 4);
-    const half8 lo = *reinterpret_cast<const half8*>(p + (int64_t)r * cells * 4 + 64);
-#pragma unroll
-    for (int k = 0; k < 8; k++) s[k] += (float)hi[k] + (float)lo[k];
-  }
-#pragma unroll
-  for (int k = 0; k < 8; k++) sh[sub][col + k] = s[k];
-  __syncthreads();
-  float t = 0.0f;
-#pragma unroll
-  for (int g = 0; g < 8; g++) t += sh[g][threadIdx.x];
-  partial[(int64_t)blockIdx.y * cells + (int64_t)blockIdx.x * 256 + threadIdx.x] = t;
-}
-
-// db (+)= 2^-kTop scale * sum of the partial rows
-__global__ __launch_bounds__(kThreads) void k_lce_db(const float* __restrict__ partial, int n, int64_t cells,
-                                                     float* __restrict__ db, int classes, const Ctl* __restrict__ ctl, int add) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= classes) return;
-  float s = 0.0f;
-  for (int i = 0; i < n; i++) s += partial[i * cells + c];
-  s = ldexpf(s, -kTop) * ctl->scale;
-  db[c] = add ? db[c] + s : s;
-}
-
-// out (m, n) (+)= 2^(...) scale * sum over the splits, in their order
-__global__ __launch_bounds__(kThreads) void k_lce_slabs(const float* __restrict__ slabs, int splits, int64_t slab, int64_t lds_,
-                                                        float* __restrict__ out, int64_t m, int64_t n,
-                                                        const int* __restrict__ exp_in, const Ctl* __restrict__ ctl, int add) {
-  const int e = exp_in[0] - kTop;
-  const float sc = ctl->scale;
-  const int64_t total = m * n;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = i / n, c = i - r * n;
-    const float* p = slabs + r * lds_ + c;
-    float s = 0.0f;
-    for (int z = 0; z < splits; z++) s += p[z * slab];
-    s = ldexpf(s, e) * sc;
-    out[i] = add ? out[i] + s : s;
-  }
-}
-
 // loss = sum of the row losses times the scale, in a fixed order
 __global__ __launch_bounds__(1024) void k_lce_loss(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl,
                                                    float* __restrict__ loss, int64_t rows) {
@@ -354,64 +323,27 @@ struct Held {                                      // a pool block for the durat
   int take(int64_t floats) { return p ? DFHIP_OK : dfhip_malloc(floats, &p); }
 };
 
-// tile of a product of m x n outputs and `steps` steps of 32: 256 x 256 (one workgroup a CU) where that gives every CU work,
-// 128 x 128 (two a CU) otherwise; `cut`: the reduction may be cut into splits of at least 8 steps
-struct Plan { bool big; int splits, steps_split; };
-Plan plan(int64_t m, int64_t n, int steps, bool cut) {
-  const int64_t t256 = df_ceil_div(m, 256) * df_ceil_div(n, 256), t128 = df_ceil_div(m, 128) * df_ceil_div(n, 128);
-  Plan p;
-  p.big = cut ? t256 * steps >= (int64_t)num_cus() * 24 : t256 * 4 >= (int64_t)num_cus() * 3;
-  const int64_t tiles = p.big ? t256 : t128, want = p.big ? num_cus() : 2 * num_cus();
-  int64_t s = cut && tiles < want ? want / tiles : 1;
-  s = std::max<int64_t>(1, std::min<int64_t>(s, steps / 8));
-  p.steps_split = (int)df_ceil_div(steps, s);
-  p.splits = (int)df_ceil_div(steps, p.steps_split);
-  return p;
-}
-
+// one product as the plan says; the parts of cut tiles live in `parts`, which grows as needed
 template <bool AX, bool BX, int EPI>
-int product(Gemm& g, const Plan& p, int64_t m, int64_t n) {
-  const int t = p.big ? 256 : 128;
-  g.tiles_m = (int)df_ceil_div(m, t);
-  g.tiles_n = (int)df_ceil_div(n, t);
+int product(Gemm& g, int64_t m, int64_t n, Held& parts, int64_t& held) {
+  const Plan p = plan(m, n, g.ksteps);
+  DF_CHECK_ARG(p.us > 0.0, "linear_ce_forward: too many tiles");
+  g.tiles_m = p.tiles_m;
+  g.full = p.full;
+  g.rest = p.rest;
   g.splits = p.splits;
-  g.ksteps_split = p.steps_split;
-  return p.big ? launch<256, 256, 2, 4, AX, BX, EPI>(g) : launch<128, 128, 2, 2, AX, BX, EPI>(g);
-}
-
-// out (m, n) (+)= 2^(e - kTop) scale * a . b; the reduction may be cut, the cut sums meet in `slabs`
-template <bool AX, bool BX>
-int gradient_product(Gemm g, int64_t m, int64_t n, float* out, bool add, const int* e, const Ctl* ctl, Held& slabs,
-                     int64_t& held) {
-  const Plan p = plan(m, n, g.ksteps, true);
-  g.m = (int)m;
+  g.ksteps_split = p.ksteps_split;
+  g.m = g.c ? (int)m : 0;                         // (db alone: nothing of the product is stored)
   g.n = (int)n;
-  g.exp_a = e;
-  g.exp_b = nullptr;
-  g.exp_c = -kTop;
-  g.scale = &ctl->scale;
-  g.bias = nullptr;
-  if (p.splits == 1) {
-    g.c = out;
-    g.ldc = n;
-    g.slab = 0;
-    return add ? product<AX, BX, EPI_ADD>(g, p, m, n) : product<AX, BX, EPI_STORE>(g, p, m, n);
-  }
-  g.ldc = padded(n);
-  g.slab = padded(m) * g.ldc;
-  if (held < p.splits * g.slab) {
-    if (slabs.p) { (void)dfhip_free(slabs.p); slabs.p = nullptr; }
-    held = p.splits * g.slab;
-    const int st = slabs.take(held);
+  const int64_t need = p.rest ? parts_floats(p) : 0;
+  if (held < need) {
+    if (parts.p) { (void)dfhip_free(parts.p); parts.p = nullptr; }
+    held = need;
+    const int st = parts.take(need);
     if (st != DFHIP_OK) return st;
   }
-  g.c = slabs.p;
-  const int st = product<AX, BX, EPI_SLAB>(g, p, m, n);
-  if (st != DFHIP_OK) return st;
-  DF_LAUNCH(k_lce_slabs, dim3((unsigned)std::min<int64_t>(df_ceil_div(m * n, kThreads), 8192)), dim3(kThreads), 0, stream(),
-            slabs.p, p.splits, g.slab, g.ldc, out, m, n, e, ctl, add ? 1 : 0);
-  DF_LAUNCH_CHECK();
-  return DFHIP_OK;
+  g.parts = parts.p;
+  return p.big ? launch<256, 256, 2, 4, AX, BX, EPI>(g) : launch<128, 128, 2, 2, AX, BX, EPI>(g);
 }
 
 int rows_pass(float* logits, const float* target, int n, int launch_rows, float* rowloss, int classes, int cells, float ignore,
@@ -459,23 +391,22 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   // pieces of about the same length, a multiple of 256 rows
   const int64_t cap = std::max<int64_t>(256, kPieceBytes / (4 * vp) / 256 * 256), pieces = df_ceil_div(rows, cap);
   const int64_t piece = padded(df_ceil_div(rows, pieces));
-  constexpr int kColSlices = 32;
-  Held xs, ws, logits, small, slabs;
+  Held xs, ws, logits, small, parts;
   int64_t held = 0;
-  int st = small.take((int64_t)(sizeof(Ctl) / 4) + rows + (db ? kColSlices * vp : 0));
+  int st = small.take((int64_t)(sizeof(Ctl) / 4) + rows);
   if (st == DFHIP_OK) st = xs.take(np * dp);
   if (st == DFHIP_OK) st = ws.take(dp * vp);
   if (st == DFHIP_OK) st = logits.take(piece * vp);
   if (st != DFHIP_OK) return st;
   Ctl* ctl = reinterpret_cast<Ctl*>(small.p);
-  float *partial = small.p + sizeof(Ctl) / 4, *rowloss = partial + (db ? kColSlices * vp : 0);
+  float* rowloss = small.p + sizeof(Ctl) / 4;
   const float ignore = (float)ignore_index;
   ProfScope prof("linear_ce", (grads ? 6.0 : 2.0) * (double)rows * (double)width * (double)classes,
                  4.0 * (grads ? 2.0 : 1.0) * ((double)rows * width + (double)width * classes));
 
   DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows * width, w, width * classes, ctl);
   DF_LAUNCH_CHECK();
-  const int64_t bx = std::min<int64_t>(df_ceil_div(np * dp / 8, kThreads), 2048), bw = std::min<int64_t>(df_ceil_div(dp * vp / 8, kThreads), 4096);
+  const int64_t bx = std::min<int64_t>(np * dp / 2048, 2048), bw = std::min<int64_t>(dp * vp / 2048, 4096);
   DF_LAUNCH(k_lce_split, dim3((unsigned)(bx + bw + 1)), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p,
             (char*)ws.p, target, ignore, mean, bx, bw, ctl);
   DF_LAUNCH_CHECK();
@@ -490,40 +421,39 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     g.ksteps = (int)df_ceil_div(width, 32);
     g.c = logits.p;
     g.ldc = vp;
-    g.n = (int)classes;
     g.bias = bias;
     g.exp_a = &ctl->ex;
     g.exp_b = &ctl->ew;
-    st = product<false, true, EPI_BIAS>(g, plan(n, classes, g.ksteps, false), n, classes);
+    st = product<false, true, EPI_BIAS>(g, n, classes, parts, held);
     if (st != DFHIP_OK) return st;
     st = rows_pass(logits.p, target + r0, (int)n, (int)(grads ? df_ceil_div(n, 32) * 32 : n), rowloss + r0, (int)classes, (int)vp,
                    ignore, (float)label_smoothing, grads ? 1 : 0);
     if (st != DFHIP_OK) return st;
-    if (db) {
-      const int slices = (int)std::min<int64_t>(kColSlices, df_ceil_div(n, 32));
-      DF_LAUNCH(k_lce_colsum, dim3((unsigned)(vp / 256), (unsigned)slices), dim3(kThreads), 0, stream(), (const char*)logits.p, (int)n,
-                vp, partial);
-      DF_LAUNCH_CHECK();
-      DF_LAUNCH(k_lce_db, dim3((unsigned)df_ceil_div(classes, kThreads)), dim3(kThreads), 0, stream(), partial, slices, vp, db,
-                (int)classes, ctl, r0 ? 1 : 0);
-      DF_LAUNCH_CHECK();
-    }
+    g.bias = nullptr;
+    g.exp_b = nullptr;
+    g.exp_c = -kTop;
+    g.scale = &ctl->scale;
     if (dx) {
       g.a = (const char*)logits.p;
       g.lda = vp * 4;
-      g.b = (const char*)ws.p;
-      g.ldb = vp * 4;
       g.ksteps = (int)df_ceil_div(classes, 32);
-      st = gradient_product<false, false>(g, n, width, dx + r0 * width, false, &ctl->ew, ctl, slabs, held);
+      g.c = dx + r0 * width;
+      g.ldc = width;
+      g.exp_a = &ctl->ew;
+      st = product<false, false, EPI_STORE>(g, n, width, parts, held);
       if (st != DFHIP_OK) return st;
     }
-    if (dw) {
+    if (dw || db) {
       g.a = (const char*)xs.p + r0 * dp * 4;
       g.lda = dp * 4;
       g.b = (const char*)logits.p;
-      g.ldb = vp * 4;
       g.ksteps = (int)df_ceil_div(n, 32);
-      st = gradient_product<true, true>(g, width, classes, dw, r0 > 0, &ctl->ex, ctl, slabs, held);
+      g.c = dw;
+      g.ldc = classes;
+      g.exp_a = &ctl->ex;
+      g.colsum = db;
+      st = r0 ? product<true, true, EPI_ADD>(g, dw ? width : 1, classes, parts, held)
+              : product<true, true, EPI_STORE>(g, dw ? width : 1, classes, parts, held);
       if (st != DFHIP_OK) return st;
     }
   }
