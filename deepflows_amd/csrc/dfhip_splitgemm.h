@@ -11,14 +11,16 @@
 // STORAGE ("split array"): a padded row-major array of 4-byte cells, columns in blocks of 32: 128 bytes that hold the block's 32
 // hi halves, then its 32 lo halves.  A cell takes as much room as the fp32 value it stands for, so an fp32 array can be converted
 // in place block by block, and ONE copy of an array serves as either operand of a product:
-//   the reduction runs along the rows of the storage ("K along"): a tile is 128-byte pieces of BM rows, read as 16-byte fragments;
-//   the reduction runs across them ("K across"): a tile is 32 rows of 4 BM bytes, read with the transposing LDS loads
+//   the reduction runs along the rows of the storage ("K along"): a tile is 128-byte pieces of T rows, read as 16-byte fragments;
+//   the reduction runs across them ("K across"): a tile is 32 rows of 4 T bytes, read with the transposing LDS loads
 //   (ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 halves, each lane receives the 4 rows of its column).
 //
-// KERNEL: workgroup tile BM x BN, K step 32, two LDS buffers filled by 16-byte global-to-LDS copies that are issued a step ahead;
-// one barrier a step.  32 x 32 x 16 MFMA; a wave owns (BM / WM) x (BN / WN).  LDS positions are XOR-permuted at 16-byte
-// granularity by the ROW (the copy's source address is permuted, its LDS side is linear): 16 lanes that read the same piece of 16
-// rows, or 32 lanes that read 4 rows transposed, touch every bank once.
+// KERNEL: workgroup tile T x T, K step 32, LDS buffers filled by 16-byte global-to-LDS copies issued NS - 1 steps ahead; one
+// barrier a step.  32 x 32 x 16 MFMA.  T = 256: 8 waves of 128 x 64, two buffers, one workgroup a CU; T = 128: 4 waves of 64 x 64,
+// two buffers, two workgroups a CU; T = 64: 4 waves of 32 x 32, four buffers (short reductions and few tiles wait for memory, not
+// for the matrix cores).  LDS positions are XOR-permuted at 16-byte granularity by the ROW (the copy's source address is permuted,
+// its LDS side is linear): 16 lanes that read the same piece of 16 rows, or 32 lanes that read 4 rows transposed, touch every bank
+// once (SQ_LDS_BANK_CONFLICT reads 0).
 // LDS reads: three products share two fragments a side, so the LDS moves half the bytes an fp16 GEMM of the same rate would.
 #pragma once
 #include <algorithm>
@@ -70,11 +72,12 @@ template <int EPI>
 __device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
   return EPI == EPI_BIAS && g.bias && n < g.n ? g.bias[n] : 0.0f;
 }
+// one value of row m (c: its place) and column n
 template <int EPI>
-__device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias, int64_t m, int64_t n, float v) {
-  if (EPI == EPI_BIAS) g.c[m * g.ldc + n] = ldexpf(v, e) + bias;
-  if (EPI == EPI_STORE && m < g.m && n < g.n) g.c[m * g.ldc + n] = ldexpf(v, e) * sc;
-  if (EPI == EPI_ADD && m < g.m && n < g.n) g.c[m * g.ldc + n] += ldexpf(v, e) * sc;
+__device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias, int64_t m, int64_t n, float* c, float v) {
+  if (EPI == EPI_BIAS) *c = ldexpf(v, e) + bias;
+  if (EPI == EPI_STORE && m < g.m && n < g.n) *c = ldexpf(v, e) * sc;
+  if (EPI == EPI_ADD && m < g.m && n < g.n) *c += ldexpf(v, e) * sc;
 }
 template <int EPI>
 __device__ __forceinline__ void emit_colsum(const Gemm& g, float sc, int64_t n, float v) {
@@ -135,7 +138,8 @@ struct Reader {
       for (int par = 0; par < 2; par++)
 #pragma unroll
         for (int plane = 0; plane < 2; plane++)
-          off[par * 2 + plane] = k * (BM * 4) + (w0 >> 6) * 256 + (((8 * par + 4 * plane + q) ^ (x << 2)) << 4) + (lane & 1) * 8;
+          off[par * 2 + plane] = k * (BM * 4) + (w0 >> 6) * 256 +
+                                 (((8 * (par ^ ((w0 >> 5) & 1)) + 4 * plane + q) ^ (x << 2)) << 4) + (lane & 1) * 8;
     } else {
       const int x = ((lane & 31) >> 1) & 7;
 #pragma unroll
@@ -145,7 +149,7 @@ struct Reader {
           off[kk * 2 + plane] = (w0 + (lane & 31)) * 128 + (((plane * 4 + kk * 2 + (lane >> 5)) ^ x) << 4);
     }
   }
-  // tile i, counted from w0 (w0 is a multiple of 64 where the reduction runs across)
+  // tile i, counted from w0 (where the reduction runs across, w0 is a multiple of 64 or there is tile 0 alone)
   __device__ __forceinline__ half8 get(const char* lds, int i, int kk, int plane) const {
     if (ACROSS) {
       const char* s = lds + off[(i & 1) * 2 + plane] + (i >> 1) * 256 + kk * 16 * (BM * 4);
@@ -159,16 +163,30 @@ struct Reader {
   }
 };
 
-template <int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
+template <int T> struct Tile;
+template <> struct Tile<256> { static constexpr int WM = 2, WN = 4, NS = 2; };
+template <> struct Tile<128> { static constexpr int WM = 2, WN = 2, NS = 2; };
+template <> struct Tile<64> { static constexpr int WM = 2, WN = 2, NS = 4; };
+template <int T> constexpr int threads() { return Tile<T>::WM * Tile<T>::WN * 64; }
+template <int T> constexpr int lds_bytes() { return Tile<T>::NS * 2 * T * 128; }
+// workgroups of a product
+__host__ __device__ inline int groups(const Gemm& g) { return ((g.full + 7) / 8 + (g.rest * g.splits + 7) / 8) * 8; }
+
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+template <int T, bool AX, bool BX, int EPI>
+__device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* lds) {
+  constexpr int BM = T, BN = T, WM = Tile<T>::WM, WN = Tile<T>::WN, NS = Tile<T>::NS;
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128, COPIES = (BM + BN) / 8 / NW;
+  static_assert((BM / WM) % 64 == 0 || TM == 1, "Reader");
+  static_assert((BN / WN) % 64 == 0 || TN == 1, "Reader");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (rows fastest), so that the
   // tiles that share a column of B meet in one L2
-  const bool whole = (int)blockIdx.x < (g.full + 7) / 8 * 8;
-  const int id = whole ? (int)blockIdx.x : (int)blockIdx.x - (g.full + 7) / 8 * 8;
+  const bool whole = block < (g.full + 7) / 8 * 8;
+  const int id = whole ? block : block - (g.full + 7) / 8 * 8;
   const int total = whole ? g.full : g.rest * g.splits, per = (total + 7) >> 3;
   const int item = (id & 7) * per + (id >> 3);
   if ((id >> 3) >= per || item >= total) return;
@@ -199,18 +217,24 @@ __global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
   ra.init(wm, lane);
   rb.init(wn, lane);
 
-  if (steps > 0) {
-    la.issue(lds, wave);
-    lb.issue(lds + ABYTES, wave);
-  }
+#pragma unroll
+  for (int s = 0; s < NS - 1; s++)
+    if (s < steps) {
+      la.issue(lds + s * STAGE, wave);
+      lb.issue(lds + s * STAGE + ABYTES, wave);
+    }
   for (int s = 0; s < steps; s++) {
-    // this wave's copies of step s have landed and its reads of step s - 1 are back; behind the barrier everybody's are
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // this wave's copies of step s have landed (the later ones may be under way) and its reads of step s - 1 are back; behind the
+    // barrier everybody's are
+    if (NS > 2 && steps - 1 - s >= 2) wait_copies<(NS > 2 ? 2 : 0) * COPIES>();
+    else if (NS > 2 && steps - 1 - s == 1) wait_copies<(NS > 2 ? 1 : 0) * COPIES>();
+    else wait_copies<0>();
+    static_assert(NS == 2 || NS == 4, "the waits above");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const char* cur = lds + (s & 1) * STAGE;
-    char* nxt = lds + ((s + 1) & 1) * STAGE;
-    if (s + 1 < steps) {
+    const char* cur = lds + (s & (NS - 1)) * STAGE;
+    char* nxt = lds + ((s + NS - 1) & (NS - 1)) * STAGE;
+    if (s + NS - 1 < steps) {
       la.issue(nxt, wave);
       lb.issue(nxt + ABYTES, wave);
     }
@@ -259,34 +283,43 @@ __global__ __launch_bounds__(WM * WN * 64) void k_split_gemm(Gemm g) {
       }
     }
   }
+  // (rows outermost: an address a row, the columns of a wave's tiles are constants from it)
   if (!whole) {
-#pragma unroll
-    for (int j = 0; j < TN; j++)
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          part[(wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * BN + wn + j * 32 + (lane & 31)] = acc[i][j][r];
-    return;
-  }
-  float bias[TN];
-#pragma unroll
-  for (int j = 0; j < TN; j++) bias[j] = bias_of<EPI>(g, n0 + wn + j * 32 + (lane & 31));
-#pragma unroll
-  for (int j = 0; j < TN; j++)
+    float* c0 = part + (wm + 4 * (lane >> 5)) * BN + wn + (lane & 31);
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
       for (int r = 0; r < 16; r++)
-        emit<EPI>(g, e, sc, bias[j], m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n0 + wn + j * 32 + (lane & 31),
-                  acc[i][j][r]);
+#pragma unroll
+        for (int j = 0; j < TN; j++) c0[(i * 32 + 8 * (r >> 2) + (r & 3)) * BN + j * 32] = acc[i][j][r];
+    return;
+  }
+  const int64_t n = n0 + wn + (lane & 31);
+  float bias[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) bias[j] = bias_of<EPI>(g, n + j * 32);
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int64_t m = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+      float* c = g.c + m * g.ldc + n;
+#pragma unroll
+      for (int j = 0; j < TN; j++) emit<EPI>(g, e, sc, bias[j], m, n + j * 32, c + j * 32, acc[i][j][r]);
+    }
+}
+
+template <int T, bool AX, bool BX, int EPI>
+__global__ __launch_bounds__(threads<T>()) void k_split_gemm(Gemm g) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  gemm_body<T, AX, BX, EPI>(g, (int)blockIdx.x, lds);
 }
 
 // the parts of the cut tiles added up: 1024 cells of one tile a workgroup, four a thread
-template <int BM, int BN, int EPI>
-__global__ __launch_bounds__(256) void k_split_rest(Gemm g) {
-  constexpr int SLICES = BM * BN / 1024, CELLS = BM * BN + BN;
-  const int t = (int)blockIdx.x / SLICES, slice = (int)blockIdx.x % SLICES, tile = g.full + t;
+template <int T, int EPI>
+__device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
+  constexpr int BM = T, BN = T, SLICES = BM * BN / 1024, CELLS = BM * BN + BN;
+  const int t = block / SLICES, slice = block % SLICES, tile = g.full + t;
   const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const float* part = g.parts + (int64_t)t * g.splits * CELLS;
@@ -312,7 +345,7 @@ __global__ __launch_bounds__(256) void k_split_rest(Gemm g) {
 #pragma unroll
   for (int k = 0; k < 4; k++) bias[k] = bias_of<EPI>(g, n + k);
 #pragma unroll
-  for (int k = 0; k < 4; k++) emit<EPI>(g, e, sc, bias[k], m0 + cell / BN, n + k, v[k]);
+  for (int k = 0; k < 4; k++) emit<EPI>(g, e, sc, bias[k], m0 + cell / BN, n + k, g.c + (m0 + cell / BN) * g.ldc + n + k, v[k]);
   if (g.colsum && tm == 0 && slice == 0 && (int)threadIdx.x < BN) {
     const float* c = part + BM * BN + threadIdx.x;
     float s = 0.0f;
@@ -321,57 +354,56 @@ __global__ __launch_bounds__(256) void k_split_rest(Gemm g) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
-int launch(const Gemm& g) {
-  constexpr int lds = 2 * (BM + BN) * 128;
-  static bool set = false;
-  if (lds > 65536 && !set) {
-    DF_HIP(hipFuncSetAttribute((const void*)k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>,
-                               hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    set = true;
-  }
-  const int64_t groups = (int64_t)((g.full + 7) / 8 + ((int64_t)g.rest * g.splits + 7) / 8) * 8;
-  DF_LAUNCH((k_split_gemm<BM, BN, WM, WN, AX, BX, EPI>), dim3((unsigned)groups), dim3(WM * WN * 64), lds, dfhip::stream(), g);
-  DF_LAUNCH_CHECK();
-  if (g.rest) {
-    DF_LAUNCH((k_split_rest<BM, BN, EPI>), dim3((unsigned)g.rest * (BM * BN / 1024)), dim3(256), 0, dfhip::stream(), g);
-    DF_LAUNCH_CHECK();
-  }
-  return DFHIP_OK;
-}
+template <int T, int EPI>
+__global__ __launch_bounds__(256) void k_split_rest(Gemm g) { rest_body<T, EPI>(g, (int)blockIdx.x); }
 
-// How a product of m x n outputs and `steps` steps runs: the tile, and which tiles are cut.  Costs in microseconds, measured on
-// long reductions: a step of a round is 1.25 with 256 x 256 tiles (one workgroup a CU) and 0.8 with 128 x 128 (two); a part costs its
-// share of writing and adding up (0.1 and 0.025), a cut product another launch (5).
-struct Plan { bool big; int tiles_m, tiles_n, full, rest, splits, ksteps_split; double us; };
-inline Plan plan(int64_t m, int64_t n, int steps) {
+// How a product of m x n outputs and `steps` steps runs with T x T tiles: which tiles are cut.  Costs in microseconds, measured: a
+// step of a full round of tiles, what begins and ends a round, a part's share of being written and added up, another launch (5).
+struct Plan { int tile, tiles_m, tiles_n, full, rest, splits, ksteps_split; double us; };
+inline Plan plan(int tile, int64_t m, int64_t n, int steps) {
+  const int64_t slots = (tile == 256 ? 1 : 2) * (int64_t)dfhip::num_cus();
+  const double step_us = tile == 256 ? 1.25 : tile == 128 ? 0.8 : 0.4, round_us = tile == 256 ? 5.0 : 3.0;
+  const double part_us = tile == 256 ? 0.1 : tile == 128 ? 0.025 : 0.006;
+  const int64_t tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, tiles = tm * tn;
   Plan best = {};
-  for (int big = 0; big < 2; big++) {
-    const int64_t t = big ? 256 : 128, slots = (big ? 1 : 2) * (int64_t)dfhip::num_cus();
-    const double step_us = big ? 1.25 : 0.8, part_us = big ? 0.1 : 0.025;
-    const int64_t tm = (m + t - 1) / t, tn = (n + t - 1) / t, tiles = tm * tn;
-    if (tiles > (1 << 28)) continue;
-    for (int cut = 0; cut < 2; cut++) {
-      const int64_t rest = cut ? tiles % slots : 0;
-      if (cut && !rest) continue;
-      Plan p = {big != 0, (int)tm, (int)tn, (int)(tiles - rest), (int)rest, 1, steps, 0.0};
-      p.us = (double)((p.full + slots - 1) / slots) * steps * step_us;
-      if (cut) {
-        double least = 1e30;
-        const int64_t most = std::min<int64_t>(slots / rest, steps / 4);
-        if (most < 2) continue;
-        for (int64_t s = 2; s <= most; s++) {
-          const int64_t ks = (steps + s - 1) / s, real = (steps + ks - 1) / ks;
-          const double us = (double)ks * step_us + (double)(rest * real) * part_us + 5.0;
-          if (us < least) { least = us; p.splits = (int)real; p.ksteps_split = (int)ks; }
-        }
-        p.us += least;
+  best.us = 1e30;
+  if (tiles > (1 << 28)) return best;
+  for (int cut = 0; cut < 2; cut++) {
+    const int64_t rest = cut ? tiles % slots : 0;
+    if (cut && !rest) continue;
+    Plan p = {tile, (int)tm, (int)tn, (int)(tiles - rest), (int)rest, 1, steps, 0.0};
+    p.us = (double)((p.full + slots - 1) / slots) * (steps * step_us + round_us);
+    if (cut) {
+      double least = 1e30;
+      for (int64_t s = 2; s <= std::min<int64_t>(slots / rest, steps / 4); s++) {
+        const int64_t ks = (steps + s - 1) / s, real = (steps + ks - 1) / ks;
+        const double us = (double)ks * step_us + round_us + (double)(rest * real) * part_us + 5.0;
+        if (us < least) { least = us; p.splits = (int)real; p.ksteps_split = (int)ks; }
       }
-      if (best.us == 0.0 || p.us < best.us) best = p;
+      p.us += least;
     }
+    if (p.us < best.us) best = p;
   }
   return best;
 }
-inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.big ? 256 * 256 + 256 : 128 * 128 + 128); }
+inline void apply(Gemm& g, const Plan& p, int64_t m, int64_t n) {
+  g.tiles_m = p.tiles_m;
+  g.full = p.full;
+  g.rest = p.rest;
+  g.splits = p.splits;
+  g.ksteps_split = p.ksteps_split;
+  g.m = g.c ? (int)m : 0;                          // (column sums alone: nothing of the product is stored)
+  g.n = (int)n;
+}
+inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.tile * p.tile + p.tile); }
+
+// a kernel's LDS beyond 64 KB has to be asked for once
+inline int allow_lds(const void* kernel, int bytes, bool& done) {
+  if (bytes > 65536 && !done) {
+    DF_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done = true;
+  }
+  return DFHIP_OK;
+}
 
 }  // namespace dfhip_split

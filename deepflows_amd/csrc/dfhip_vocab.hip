@@ -12,9 +12,9 @@
 // dl where it is formed.  The launches of a call:
 //   k_lce_scan     the largest magnitudes of x and W (finite elements only)
 //   k_lce_split    x, W -> split arrays; the number of counted rows
-//   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> dx product ->
-//                  dW product (db on the side: the column sums of its second operand)
-//   k_lce_loss     loss
+//   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> k_lce_pair: the dx
+//                  product and the dW product (db on the side: the column sums of its second operand); with the last piece, the loss
+//   (k_lce_loss    the loss, where there are no gradients)
 #include <math.h>
 
 #include <algorithm>
@@ -301,14 +301,45 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   }
 }
 
-// loss = sum of the row losses times the scale, in a fixed order
+// loss = sum of the row losses times the scale, in a fixed order; one workgroup of T threads
+template <int T>
+__device__ __forceinline__ void loss_body(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl, float* __restrict__ loss,
+                                          int64_t rows, float* sh) {
+  float s = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows; i += T) s += rowloss[i];
+  s = block_reduce<T>(s, sh, Add());
+  if (threadIdx.x == 0) loss[0] = s * ctl->scale;
+}
 __global__ __launch_bounds__(1024) void k_lce_loss(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl,
                                                    float* __restrict__ loss, int64_t rows) {
   __shared__ float sh[1024 / 64];
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += rowloss[i];
-  s = block_reduce<1024>(s, sh, Add());
-  if (threadIdx.x == 0) loss[0] = s * ctl->scale;
+  loss_body<1024>(rowloss, ctl, loss, rows, sh);
+}
+
+// The two gradient products of a piece as one launch (they read the same dl; together they leave fewer idle CUs at the end, and a
+// small call is one launch shorter): workgroups [0, na): dx, [na, na + nb): dW, and one more for the loss behind the last piece.
+struct Pair {
+  Gemm a, b;
+  int na, nb;
+  const float* rowloss;
+  const Ctl* ctl;
+  float* loss;
+  int64_t rows;
+};
+template <int T, int EPI>
+__global__ __launch_bounds__(threads<T>()) void k_lce_pair(Pair p) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int block = (int)blockIdx.x;
+  if (block < p.na) gemm_body<T, false, false, EPI_STORE>(p.a, block, lds);
+  else if (block < p.na + p.nb) gemm_body<T, true, true, EPI>(p.b, block - p.na, lds);
+  else loss_body<threads<T>()>(p.rowloss, p.ctl, p.loss, p.rows, reinterpret_cast<float*>(lds));
+}
+template <int T, int EPI>
+__global__ __launch_bounds__(256) void k_lce_pair_rest(Pair p) {
+  constexpr int SLICES = T * T / 1024;
+  const int block = (int)blockIdx.x;
+  if (block < p.a.rest * SLICES) rest_body<T, EPI_STORE>(p.a, block);
+  else rest_body<T, EPI>(p.b, block - p.a.rest * SLICES);
 }
 
 __global__ __launch_bounds__(kThreads) void k_lce_scale(const float* __restrict__ src, const float* __restrict__ scalar,
@@ -323,28 +354,42 @@ struct Held {                                      // a pool block for the durat
   int take(int64_t floats) { return p ? DFHIP_OK : dfhip_malloc(floats, &p); }
 };
 
-// one product as the plan says; the parts of cut tiles live in `parts`, which grows as needed
-template <bool AX, bool BX, int EPI>
-int product(Gemm& g, int64_t m, int64_t n, Held& parts, int64_t& held) {
-  const Plan p = plan(m, n, g.ksteps);
-  DF_CHECK_ARG(p.us > 0.0, "linear_ce_forward: too many tiles");
-  g.tiles_m = p.tiles_m;
-  g.full = p.full;
-  g.rest = p.rest;
-  g.splits = p.splits;
-  g.ksteps_split = p.ksteps_split;
-  g.m = g.c ? (int)m : 0;                         // (db alone: nothing of the product is stored)
-  g.n = (int)n;
-  const int64_t need = p.rest ? parts_floats(p) : 0;
-  if (held < need) {
-    if (parts.p) { (void)dfhip_free(parts.p); parts.p = nullptr; }
-    held = need;
-    const int st = parts.take(need);
-    if (st != DFHIP_OK) return st;
-  }
-  g.parts = parts.p;
-  return p.big ? launch<256, 256, 2, 4, AX, BX, EPI>(g) : launch<128, 128, 2, 2, AX, BX, EPI>(g);
+int room(Held& h, int64_t& held, int64_t need) {   // scratch that grows as needed
+  if (held >= need) return DFHIP_OK;
+  if (h.p) { (void)dfhip_free(h.p); h.p = nullptr; }
+  held = need;
+  return h.take(need);
 }
+
+template <int T>
+int launch_logits(const Gemm& g) {
+  static bool done = false;
+  const int st = allow_lds((const void*)k_split_gemm<T, false, true, EPI_BIAS>, lds_bytes<T>(), done);
+  if (st != DFHIP_OK) return st;
+  DF_LAUNCH((k_split_gemm<T, false, true, EPI_BIAS>), dim3((unsigned)groups(g)), dim3(threads<T>()), lds_bytes<T>(), stream(), g);
+  DF_LAUNCH_CHECK();
+  if (g.rest) {
+    DF_LAUNCH((k_split_rest<T, EPI_BIAS>), dim3((unsigned)g.rest * (T * T / 1024)), dim3(256), 0, stream(), g);
+    DF_LAUNCH_CHECK();
+  }
+  return DFHIP_OK;
+}
+
+template <int T, int EPI>
+int launch_pair(const Pair& p) {
+  static bool done = false;
+  const int st = allow_lds((const void*)k_lce_pair<T, EPI>, lds_bytes<T>(), done);
+  if (st != DFHIP_OK) return st;
+  DF_LAUNCH((k_lce_pair<T, EPI>), dim3((unsigned)(p.na + p.nb + (p.loss ? 1 : 0))), dim3(threads<T>()), lds_bytes<T>(), stream(), p);
+  DF_LAUNCH_CHECK();
+  if (p.a.rest + p.b.rest) {
+    DF_LAUNCH((k_lce_pair_rest<T, EPI>), dim3((unsigned)(p.a.rest + p.b.rest) * (T * T / 1024)), dim3(256), 0, stream(), p);
+    DF_LAUNCH_CHECK();
+  }
+  return DFHIP_OK;
+}
+
+constexpr int kTiles[3] = {256, 128, 64};
 
 int rows_pass(float* logits, const float* target, int n, int launch_rows, float* rowloss, int classes, int cells, float ignore,
               float smooth, int grads) {
@@ -424,39 +469,81 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     g.bias = bias;
     g.exp_a = &ctl->ex;
     g.exp_b = &ctl->ew;
-    st = product<false, true, EPI_BIAS>(g, n, classes, parts, held);
-    if (st != DFHIP_OK) return st;
+    {
+      Plan best = plan(kTiles[0], n, classes, g.ksteps);
+      for (int t : {kTiles[1], kTiles[2]}) {
+        const Plan q = plan(t, n, classes, g.ksteps);
+        if (q.us < best.us) best = q;
+      }
+      DF_CHECK_ARG(best.tile, "linear_ce_forward: too many tiles");
+      apply(g, best, n, classes);
+      st = room(parts, held, parts_floats(best));
+      if (st != DFHIP_OK) return st;
+      g.parts = parts.p;
+      st = best.tile == 256 ? launch_logits<256>(g) : best.tile == 128 ? launch_logits<128>(g) : launch_logits<64>(g);
+      if (st != DFHIP_OK) return st;
+    }
     st = rows_pass(logits.p, target + r0, (int)n, (int)(grads ? df_ceil_div(n, 32) * 32 : n), rowloss + r0, (int)classes, (int)vp,
                    ignore, (float)label_smoothing, grads ? 1 : 0);
     if (st != DFHIP_OK) return st;
-    g.bias = nullptr;
-    g.exp_b = nullptr;
-    g.exp_c = -kTop;
-    g.scale = &ctl->scale;
+    if (!grads) continue;
+    Pair p = {};
+    Plan pa = {}, pb = {};
+    double least = 1e31;
+    const int steps_a = (int)df_ceil_div(classes, 32), steps_b = (int)df_ceil_div(n, 32);
+    const int64_t mb = dw ? width : 1;             // (db alone: one tile high, nothing of the product stored)
+    for (int t : kTiles) {
+      Plan qa = {}, qb = {};
+      qa.tile = qb.tile = t;
+      if (dx) qa = plan(t, n, width, steps_a);
+      if (dw || db) qb = plan(t, mb, classes, steps_b);
+      if (qa.us + qb.us < least) { least = qa.us + qb.us; pa = qa; pb = qb; }
+    }
+    DF_CHECK_ARG(pa.tile && pb.tile, "linear_ce_forward: too many tiles");
+    st = room(parts, held, parts_floats(pa) + parts_floats(pb));
+    if (st != DFHIP_OK) return st;
+    p.a.exp_c = p.b.exp_c = -kTop;
+    p.a.scale = p.b.scale = &ctl->scale;
     if (dx) {
-      g.a = (const char*)logits.p;
-      g.lda = vp * 4;
-      g.ksteps = (int)df_ceil_div(classes, 32);
-      g.c = dx + r0 * width;
-      g.ldc = width;
-      g.exp_a = &ctl->ew;
-      st = product<false, false, EPI_STORE>(g, n, width, parts, held);
-      if (st != DFHIP_OK) return st;
+      p.a.a = (const char*)logits.p;
+      p.a.lda = vp * 4;
+      p.a.b = (const char*)ws.p;
+      p.a.ldb = vp * 4;
+      p.a.ksteps = steps_a;
+      p.a.c = dx + r0 * width;
+      p.a.ldc = width;
+      p.a.exp_a = &ctl->ew;
+      p.a.parts = parts.p;
+      apply(p.a, pa, n, width);
+      p.na = groups(p.a);
     }
     if (dw || db) {
-      g.a = (const char*)xs.p + r0 * dp * 4;
-      g.lda = dp * 4;
-      g.b = (const char*)logits.p;
-      g.ksteps = (int)df_ceil_div(n, 32);
-      g.c = dw;
-      g.ldc = classes;
-      g.exp_a = &ctl->ex;
-      g.colsum = db;
-      st = r0 ? product<true, true, EPI_ADD>(g, dw ? width : 1, classes, parts, held)
-              : product<true, true, EPI_STORE>(g, dw ? width : 1, classes, parts, held);
-      if (st != DFHIP_OK) return st;
+      p.b.a = (const char*)xs.p + r0 * dp * 4;
+      p.b.lda = dp * 4;
+      p.b.b = (const char*)logits.p;
+      p.b.ldb = vp * 4;
+      p.b.ksteps = steps_b;
+      p.b.c = dw;
+      p.b.ldc = classes;
+      p.b.exp_a = &ctl->ex;
+      p.b.colsum = db;
+      p.b.parts = parts.p + parts_floats(pa);
+      apply(p.b, pb, mb, classes);
+      p.nb = groups(p.b);
     }
+    if (r0 + n == rows) {
+      p.rowloss = rowloss;
+      p.ctl = ctl;
+      p.loss = loss;
+      p.rows = rows;
+    }
+    if (r0 == 0)
+      st = pa.tile == 256 ? launch_pair<256, EPI_STORE>(p) : pa.tile == 128 ? launch_pair<128, EPI_STORE>(p) : launch_pair<64, EPI_STORE>(p);
+    else
+      st = pa.tile == 256 ? launch_pair<256, EPI_ADD>(p) : pa.tile == 128 ? launch_pair<128, EPI_ADD>(p) : launch_pair<64, EPI_ADD>(p);
+    if (st != DFHIP_OK) return st;
   }
+  if (grads) return DFHIP_OK;
   DF_LAUNCH(k_lce_loss, dim3(1), dim3(1024), 0, stream(), rowloss, ctl, loss, rows);
   DF_LAUNCH_CHECK();
   return DFHIP_OK;
