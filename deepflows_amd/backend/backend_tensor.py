@@ -10,7 +10,7 @@ and the CPU-baseline leg of bench.py register the NumPy oracle device explicitly
 `register_device` — nothing falls back to it.
 """
 import math
-from functools import reduce as _reduce
+from functools import lru_cache, reduce as _reduce
 
 import numpy as np
 
@@ -140,6 +140,16 @@ def default_device():
     return Device(_default_name if _default_name is not None else "hip")
 
 
+@lru_cache(maxsize=4096)
+def _layout(shape):
+    """(row-major strides, number of elements) of a shape; a training loop asks for the same few shapes every step"""
+    strides, acc = [], 1
+    for extent in reversed(shape):
+        strides.append(acc)
+        acc *= extent
+    return tuple(reversed(strides)), acc
+
+
 # ---- the strided array -----------------------------------------------------------------------
 class BackendTensor:
     def __init__(self, other, device=None):
@@ -162,20 +172,16 @@ class BackendTensor:
 
     @staticmethod
     def compact_strides(shape):
-        strides, acc = [], 1
-        for extent in reversed(tuple(shape)):
-            strides.append(acc)
-            acc *= extent
-        return tuple(reversed(strides))
+        return _layout(tuple(shape))[0]
 
     @staticmethod
     def make(shape, strides=None, device=None, handle=None, offset=0):
         t = BackendTensor.__new__(BackendTensor)
-        t._shape = tuple(shape)
-        t._strides = BackendTensor.compact_strides(shape) if strides is None else strides
+        t._shape = shape = tuple(shape)
+        t._strides = _layout(shape)[0] if strides is None else strides
         t._offset = offset
-        t._device = device if device is not None else default_device()
-        t._handle = t._device.Array(prod(shape)) if handle is None else handle
+        t._device = device = device if device is not None else default_device()
+        t._handle = device.mod.Array(_layout(shape)[1]) if handle is None else handle
         return t
 
     shape = property(lambda self: self._shape)
@@ -204,8 +210,8 @@ class BackendTensor:
         return self.device.to_numpy(self._handle, self.shape, self.strides, self._offset)
 
     def is_compact(self):
-        return (tuple(self._strides) == self.compact_strides(self._shape)
-                and prod(self._shape) == self._handle.size)
+        strides, size = _layout(self._shape)
+        return tuple(self._strides) == strides and size == self._handle.size
 
     def compact(self):
         if self.is_compact():

@@ -458,21 +458,20 @@ class _RMSNormFused(_FusedNode):
 
     fuses_accumulation = True
 
-    def __init__(self, x, weight, yd, rstd):
+    def __init__(self, x, weight, yd, rstd, xd, wd):
         self.x, self.weight = x, weight
-        self._saved = (x.data.compact(), weight.data.compact() if weight is not None else None, rstd)
+        self._saved = (xd, wd, rstd)
         self._dw = None                          # (upstream gradient, weight gradient) left behind by the input's turn
         super().__init__(yd, [x, weight])
 
     def _launch(self, grad, want_dx, held):
         xd, wd, rstd = self._saved
-        dev = grad.device
-        dx = _new(xd.shape, dev) if want_dx else None
-        dw = _grad_out(self.weight, self.weight.shape, dev) if self.weight is not None and self.weight.requires_grad else None
+        dev = xd._device
+        dx = BackendTensor.make(xd._shape, device=dev) if want_dx else None
+        dw = _grad_out(self.weight, wd._shape, dev) if wd is not None and self.weight.requires_grad else None
         h = lambda t: t._handle if t is not None else None
-        width = int(xd.shape[-1])
         dev.mod.rms_norm_backward(grad.compact()._handle, xd._handle, rstd._handle, h(wd), h(held), h(dx), h(dw),
-                                  xd.size // width, width)
+                                  rstd._handle.size, int(xd._shape[-1]))
         return dx, dw
 
     def grad_fn(self, node, grad, held=None):
@@ -493,36 +492,40 @@ def rms_norm(input: Tensor, weight=None, eps: float = 1e-6, residual=None):
     next residual sum starts from.  weight: None or a tensor with as many elements as the last axis.  Zero rows are allowed."""
     input = realize(input)
     residual = realize(residual) if residual is not None else None
-    if input.ndim < 1 or int(input.shape[-1]) < 1:
-        raise ValueError(f"rms_norm: the last axis must have at least one element, got shape {tuple(input.shape)}")
+    x, device = input.data, input.data._device
+    shape = tuple(x.shape)
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"rms_norm: the last axis must have at least one element, got shape {shape}")
     if not eps >= 0:
         raise ValueError(f"rms_norm: eps must be >= 0, got {eps}")
-    shape = tuple(int(v) for v in input.shape)
-    width = shape[-1]
-    if weight is not None and (int(weight.size) != width or int(weight.shape[-1]) != width):
-        raise ValueError(f"rms_norm: weight of shape {tuple(weight.shape)} for a last axis of {width}")
-    if weight is input:
-        raise ValueError("rms_norm: weight and input are one tensor")
-    if residual is not None and tuple(int(v) for v in residual.shape) != shape:
+    width = int(shape[-1])
+    if weight is not None:
+        if weight is input:
+            raise ValueError("rms_norm: weight and input are one tensor")
+        if weight.size != width or weight.shape[-1] != width:
+            raise ValueError(f"rms_norm: weight of shape {tuple(weight.shape)} for a last axis of {width}")
+    if residual is not None and tuple(residual.shape) != shape:
         raise ValueError(f"rms_norm: residual of shape {tuple(residual.shape)} for an input of shape {shape}")
     for other in (weight, residual):
-        if other is not None and other.device != input.device:
+        if other is not None and other.device is not device and other.device != device:
             raise ValueError("rms_norm: all tensors must be on one device")
-    mod = input.device.mod
-    if _fused(input) and hasattr(mod, "rms_norm_forward"):
-        dev = input.device
-        xd = input.data.compact()
-        y = _new(shape, dev)
-        grad = is_grad_enable() and any(t is not None and t.requires_grad for t in (input, weight, residual))
-        rows = y.size // width
-        rstd = _new((rows,), dev) if grad else None
+    mod = device.mod
+    if getattr(mod, "fused", False) and hasattr(mod, "rms_norm_forward"):
+        grad = is_grad_enable() and (input.requires_grad or (weight is not None and weight.requires_grad)
+                                     or (residual is not None and residual.requires_grad))
+        xd = x.compact()
+        y = BackendTensor.make(shape, device=device)
+        rows = y._handle.size // width
+        rstd = BackendTensor.make((rows,), device=device) if grad else None
+        hd = rd = wd = None
+        if residual is not None:
+            rd, hd = residual.data.compact(), BackendTensor.make(shape, device=device)
+        if weight is not None:
+            wd = weight.data.compact()
         h = lambda t: t._handle if t is not None else None
-        hd = _new(shape, dev) if residual is not None else None
-        wd = weight.data.compact() if weight is not None else None
-        rd = residual.data.compact() if residual is not None else None
         mod.rms_norm_forward(xd._handle, h(rd), h(wd), y._handle, h(hd), h(rstd), rows, width, eps)
         summed = _ResidualSum(input, residual, hd) if residual is not None else input
-        out = _RMSNormFused(summed, weight, y, rstd)
+        out = _RMSNormFused(summed, weight, y, rstd, hd if residual is not None else xd, wd)
     else:
         summed = input + residual if residual is not None else input
         axis = len(shape) - 1
@@ -611,15 +614,15 @@ class _LinearCrossEntropyFused(_FusedNode):
     def __init__(self, x, weight, bias, target, mean, ignore_index, label_smoothing):
         self.x, self.w, self.b = x, weight, bias
         dev = x.device
-        rows, width = (int(v) for v in x.shape)
-        grads = [_new(p.shape, dev) if p is not None and is_grad_enable() and p.requires_grad else None
-                 for p in (x, weight, bias)]
-        h = lambda t: t._handle if t is not None else None
-        out = _new((1,), dev)
         xd, wd, td = x.data.compact(), weight.data.compact(), target.data.compact()
         bd = bias.data.compact() if bias is not None else None
-        dev.mod.linear_ce_forward(xd._handle, wd._handle, h(bd), td._handle, out._handle, *[h(g) for g in grads], rows, width,
-                                  int(weight.shape[1]), ignore_index, label_smoothing, mean)
+        on = is_grad_enable()
+        grads = [BackendTensor.make(d._shape, device=dev) if d is not None and on and p.requires_grad else None
+                 for p, d in ((x, xd), (weight, wd), (bias, bd))]
+        h = lambda t: t._handle if t is not None else None
+        out = BackendTensor.make((1,), device=dev)
+        dev.mod.linear_ce_forward(xd._handle, wd._handle, h(bd), td._handle, out._handle, *[h(g) for g in grads],
+                                  int(xd._shape[0]), int(xd._shape[1]), int(wd._shape[1]), ignore_index, label_smoothing, mean)
         self._unit = grads
         super().__init__(out, [x, weight, bias])
 
@@ -642,14 +645,15 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     (1 - e) onehot + e / V.  On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it
     in time to raise would stall the device); elsewhere it raises ValueError."""
     input = realize(input)
-    if input.ndim != 2 or weight.ndim != 2 or int(input.shape[1]) != int(weight.shape[0]):
-        raise ValueError(f"linear_cross_entropy: input {tuple(input.shape)} and weight {tuple(weight.shape)} do not match")
-    rows, classes = int(input.shape[0]), int(weight.shape[1])
-    if classes < 1 or int(input.shape[1]) < 1:
+    xs, ws, device = tuple(input.shape), tuple(weight.shape), input.device
+    if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[0]:
+        raise ValueError(f"linear_cross_entropy: input {xs} and weight {ws} do not match")
+    rows, classes = int(xs[0]), int(ws[1])
+    if classes < 1 or xs[1] < 1:
         raise ValueError("linear_cross_entropy: at least one class and one input feature are needed")
-    if bias is not None and (int(bias.size) != classes or int(bias.shape[-1]) != classes):
+    if bias is not None and (bias.size != classes or bias.shape[-1] != classes):
         raise ValueError(f"linear_cross_entropy: bias of shape {tuple(bias.shape)} for {classes} classes")
-    if tuple(int(v) for v in target.shape) != (rows,):
+    if tuple(target.shape) != (rows,):
         raise ValueError(f"linear_cross_entropy: target of shape {tuple(target.shape)} for {rows} rows (class indices, one a row)")
     if target.requires_grad:
         raise ValueError("linear_cross_entropy: the class indices cannot require a gradient")
@@ -662,10 +666,11 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     if input is weight or (bias is not None and (bias is input or bias is weight)):
         raise ValueError("linear_cross_entropy: input, weight and bias must be different tensors")
     for other in (weight, bias, target):
-        if other is not None and other.device != input.device:
+        if other is not None and other.device is not device and other.device != device:
             raise ValueError("linear_cross_entropy: all tensors must be on one device")
     mean = reduction == 'mean'
-    if _fused(input) and hasattr(input.device.mod, "linear_ce_forward"):
+    mod = device.mod
+    if getattr(mod, "fused", False) and hasattr(mod, "linear_ce_forward"):
         return _LinearCrossEntropyFused(input, weight, bias, target, mean, int(ignore_index), float(label_smoothing))
     t = target.numpy()
     counted = t != ignore_index
