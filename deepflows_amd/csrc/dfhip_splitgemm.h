@@ -92,36 +92,42 @@ __device__ __forceinline__ int exponent(const Gemm& g) {
 template <int BM, int NW, bool ACROSS>
 struct Loader {
   static constexpr int J = BM / 8 / NW;  // 1024-byte copies a wave and step
-  const char* p[J];
-  int64_t step;
-  __device__ __forceinline__ void init(const char* base, int64_t ld, int64_t r0, int kstep0, int wave, int lane) {
-#pragma unroll
-    for (int i = 0; i < J; i++) {
-      const int j = wave * J + i;
-      if (ACROSS) {
-        const int o = j * 1024 + lane * 16;
-        const int k = o / (BM * 4);
-        const int c = ((o % (BM * 4)) >> 4) ^ ((k & 3) << 2);
-        p[i] = base + ((int64_t)kstep0 * 32 + k) * ld + r0 * 4 + c * 16;
-      } else {
-        const int row = 8 * j + (lane >> 3);
-        const int c = (lane & 7) ^ ((row >> 1) & 7);
-        p[i] = base + (r0 + row) * ld + (int64_t)kstep0 * 128 + c * 16;
-      }
+  static constexpr int ROWS = ACROSS ? 1024 / (BM * 4) : 8;      // storage rows one of them covers
+  const char* base;                      // uniform: the wave's first storage row of the next step's tile
+  int64_t ld, step;
+  unsigned off;                          // this lane's place in the first copy (K across: without its permutation)
+  int across;                            // K across: row of the tile this lane copies from, mod 4
+  __device__ __forceinline__ void init(const char* p, int64_t ld_, int64_t r0, int kstep0, int wave, int lane) {
+    ld = ld_;
+    if (ACROSS) {
+      const int k = lane * 16 / (BM * 4);          // (0 for BM = 256)
+      base = p + ((int64_t)kstep0 * 32 + wave * J * ROWS) * ld + r0 * 4;
+      off = (unsigned)(k * ld) + (unsigned)(lane * 16 % (BM * 4));
+      across = (wave * J * ROWS + k) & 3;
+      step = 32 * ld;
+    } else {
+      base = p + (r0 + wave * J * ROWS) * ld + (int64_t)kstep0 * 128;
+      // (row >> 1) & 7 with row = 8 (wave J + i) + (lane >> 3); J is even, so only i's parity moves it, by 4
+      off = (unsigned)((lane >> 3) * ld) + (unsigned)(((lane & 7) ^ ((lane >> 4) & 7)) * 16);
+      across = 0;
+      step = 128;
     }
-    step = ACROSS ? 32 * ld : 128;
   }
   __device__ __forceinline__ void issue(char* lds, int wave) {
+    static_assert(ACROSS || J % 2 == 0, "the permutation of the first copy");
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
+                                                       (unsigned)(wave * J) * 1024u);
 #pragma unroll
     for (int i = 0; i < J; i++) {
-      // (written out because the compiler, which cannot tell the two buffers apart, waits for the builtin's copies in front of
-      // the next LDS read; there is no output register, nothing else here uses m0, and the kernel's own wait and barrier order
-      // the copies)
-      const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
-                                                         (unsigned)(wave * J + i) * 1024u);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p[i]) : "memory");
-      p[i] += step;
+      const unsigned o = ACROSS ? off ^ (unsigned)(((across + i * ROWS) & 3) << 6) : (i & 1 ? off ^ 64u : off);
+      // (written out because the compiler, which cannot tell the buffers apart, waits for the builtin's copies in front of the
+      // next LDS read; there is no output register, nothing else here uses m0, and the kernel's own waits and barriers order the
+      // copies)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at + i * 1024u), "v"(o),
+                   "s"(base + (int64_t)i * ROWS * ld)
+                   : "memory");
     }
+    base += step;
   }
 };
 
@@ -175,6 +181,16 @@ __host__ __device__ inline int groups(const Gemm& g) { return ((g.full + 7) / 8 
 template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
+// the order of a half step for the scheduler: its LDS reads (of the next half) spread evenly over its products
+template <int K, int READS, int MULS>
+__device__ __forceinline__ void spread() {
+  if constexpr (K < READS) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, (K + 1) * MULS / READS - K * MULS / READS, 0);
+    spread<K + 1, READS, MULS>();
+  }
+}
+
 template <int T, bool AX, bool BX, int EPI>
 __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* lds) {
   constexpr int BM = T, BN = T, WM = Tile<T>::WM, WN = Tile<T>::WN, NS = Tile<T>::NS;
@@ -217,58 +233,89 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
   ra.init(wm, lane);
   rb.init(wn, lane);
 
+  struct Frag { half8 ah[TM], al[TM], bh[TN], bl[TN]; };
+  auto read = [&](Frag& f, int stage, int kk) {
+    const char* cur = lds + stage * STAGE;
 #pragma unroll
-  for (int s = 0; s < NS - 1; s++)
+    for (int j = 0; j < TN; j++) f.bh[j] = rb.get(cur + ABYTES, j, kk, 0);
+#pragma unroll
+    for (int i = 0; i < TM; i++) f.al[i] = ra.get(cur, i, kk, 1);
+#pragma unroll
+    for (int j = 0; j < TN; j++) f.bl[j] = rb.get(cur + ABYTES, j, kk, 1);
+#pragma unroll
+    for (int i = 0; i < TM; i++) f.ah[i] = ra.get(cur, i, kk, 0);
+  };
+  auto multiply = [&](const Frag& f) {
+    // (the same accumulator comes up again after TM * TN products)
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+  };
+  auto add_columns = [&](const Frag& f) {          // (a lane holds eight rows of one column)
+    if (BX && sums) {
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) t += (float)f.bh[j][k] + (float)f.bl[j][k];
+        col[j] += t;
+      }
+    }
+  };
+
+  // A step is two halves of 16.  While one half is multiplied the next one's fragments are read, across the step's end too: the
+  // barrier stands in the MIDDLE of a step, where every wave holds the second half in registers.  Behind it the step's buffer is
+  // free for the copies of step s + NS, and the first half of step s + 1, whose copies have landed, can be read.
+#pragma unroll
+  for (int s = 0; s < NS; s++)
     if (s < steps) {
       la.issue(lds + s * STAGE, wave);
       lb.issue(lds + s * STAGE + ABYTES, wave);
     }
-  for (int s = 0; s < steps; s++) {
-    // this wave's copies of step s have landed (the later ones may be under way) and its reads of step s - 1 are back; behind the
-    // barrier everybody's are
-    if (NS > 2 && steps - 1 - s >= 2) wait_copies<(NS > 2 ? 2 : 0) * COPIES>();
-    else if (NS > 2 && steps - 1 - s == 1) wait_copies<(NS > 2 ? 1 : 0) * COPIES>();
+  if (NS == 4 && steps >= 4) wait_copies<(NS == 4 ? 3 : 0) * COPIES>();
+  else if (NS == 4 && steps == 3) wait_copies<(NS == 4 ? 2 : 0) * COPIES>();
+  else if (steps >= 2) wait_copies<COPIES>();
+  else wait_copies<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  Frag f0, f1;
+  read(f0, 0, 0);
+  constexpr int READS = TM * 2 * (AX ? 2 : 1) + TN * 2 * (BX ? 2 : 1), MULS = 3 * TM * TN;
+  for (int s = 0; s < steps - 1; s++) {
+    read(f1, s & (NS - 1), 1);
+    multiply(f0);
+    spread<0, READS, MULS>();
+    add_columns(f0);
+    // this wave's copies of step s + 1 have landed (later ones may be under way) and its reads of step s are back
+    if (NS == 4 && steps - 2 - s >= 2) wait_copies<(NS == 4 ? 2 : 0) * COPIES>();
+    else if (NS == 4 && steps - 2 - s == 1) wait_copies<(NS == 4 ? 1 : 0) * COPIES>();
     else wait_copies<0>();
-    static_assert(NS == 2 || NS == 4, "the waits above");
+    static_assert(NS == 2 || NS == 4, "the waits");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const char* cur = lds + (s & (NS - 1)) * STAGE;
-    char* nxt = lds + ((s + NS - 1) & (NS - 1)) * STAGE;
-    if (s + NS - 1 < steps) {
-      la.issue(nxt, wave);
-      lb.issue(nxt + ABYTES, wave);
+    if (s + NS < steps) {
+      la.issue(lds + (s & (NS - 1)) * STAGE, wave);
+      lb.issue(lds + (s & (NS - 1)) * STAGE + ABYTES, wave);
     }
-#pragma unroll
-    for (int kk = 0; kk < 2; kk++) {
-      half8 ah[TM], al[TM], bh[TN], bl[TN];
-#pragma unroll
-      for (int i = 0; i < TM; i++) { ah[i] = ra.get(cur, i, kk, 0); al[i] = ra.get(cur, i, kk, 1); }
-#pragma unroll
-      for (int j = 0; j < TN; j++) { bh[j] = rb.get(cur + ABYTES, j, kk, 0); bl[j] = rb.get(cur + ABYTES, j, kk, 1); }
-      // (the same accumulator comes up again after TM * TN products)
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-      if (BX && sums) {                            // (a lane holds eight rows of one column)
-#pragma unroll
-        for (int j = 0; j < TN; j++) {
-          float t = 0.0f;
-#pragma unroll
-          for (int k = 0; k < 8; k++) t += (float)bh[j][k] + (float)bl[j][k];
-          col[j] += t;
-        }
-      }
-    }
+    read(f0, (s + 1) & (NS - 1), 0);
+    multiply(f1);
+    spread<0, READS, MULS>();
+    add_columns(f1);
   }
+  read(f1, (steps - 1) & (NS - 1), 1);
+  multiply(f0);
+  add_columns(f0);
+  multiply(f1);
+  add_columns(f1);
 
   const int e = exponent(g);
   const float sc = g.scale ? g.scale[0] : 1.0f;
