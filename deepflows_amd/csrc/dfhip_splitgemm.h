@@ -404,40 +404,91 @@ __device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
 template <int T, int EPI>
 __global__ __launch_bounds__(256) void k_split_rest(Gemm g) { rest_body<T, EPI>(g, (int)blockIdx.x); }
 
-// How a product of m x n outputs and `steps` steps runs with T x T tiles: which tiles are cut.  Costs in microseconds, measured: a
-// step of a full round of tiles, what begins and ends a round, a part's share of being written and added up, another launch (5).
-struct Plan { int tile, tiles_m, tiles_n, full, rest, splits, ksteps_split; double us; };
-inline Plan plan(int tile, int64_t m, int64_t n, int steps) {
-  const int64_t slots = (tile == 256 ? 1 : 2) * (int64_t)dfhip::num_cus();
-  const double step_us = tile == 256 ? 1.25 : tile == 128 ? 0.8 : 0.4, round_us = tile == 256 ? 5.0 : 3.0;
-  const double part_us = tile == 256 ? 0.1 : tile == 128 ? 0.025 : 0.006;
-  const int64_t tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, tiles = tm * tn;
-  Plan best = {};
-  best.us = 1e30;
-  if (tiles > (1 << 28)) return best;
-  for (int cut = 0; cut < 2; cut++) {
-    const int64_t rest = cut ? tiles % slots : 0;
-    if (cut && !rest) continue;
-    Plan p = {tile, (int)tm, (int)tn, (int)(tiles - rest), (int)rest, 1, steps, 0.0};
-    p.us = (double)((p.full + slots - 1) / slots) * (steps * step_us + round_us);
-    if (cut) {
-      double least = 1e30;
-      for (int64_t s = 2; s <= std::min<int64_t>(slots / rest, steps / 4); s++) {
-        const int64_t ks = (steps + s - 1) / s, real = (steps + ks - 1) / ks;
-        const double us = (double)ks * step_us + round_us + (double)(rest * real) * part_us + 5.0;
-        if (us < least) { least = us; p.splits = (int)real; p.ksteps_split = (int)ks; }
-      }
-      p.us += least;
-    }
-    if (p.us < best.us) best = p;
-  }
-  return best;
+// How a product of m x n outputs runs with T x T tiles: which tiles are cut, and into how many parts.
+struct Plan { int tile, tiles_m, tiles_n, full, rest, splits, ksteps, ksteps_split; };
+
+// Microseconds of `items` resident workgroups of one step each, measured (a step: 32 along the reduction): a chip full of 256 x 256
+// tiles (256 workgroups) 2.5, of 128 x 128 (512) 1.42, of 64 x 64 (512) 0.49; few workgroups 1.85, 0.66 and 0.31.
+inline double step_us(int tile, double items) {
+  if (tile == 256) return items <= 64 ? 1.85 : 1.85 + 0.65 * (items - 64) / 192;
+  const double half = items <= 256 ? items / 256 : 1.0, over = items <= 256 ? 0.0 : (items - 256) / 256;
+  return tile == 128 ? 0.66 + 0.15 * half + 0.61 * over : 0.31 + 0.03 * half + 0.15 * over;
 }
+inline int64_t slots(int tile) { return (tile == 256 ? 1 : 2) * (int64_t)dfhip::num_cus(); }
+// one launch of up to two products: their items are handed out in order, each to the workgroup slot that is free first; what is cut
+// costs its share of being written and added up, and another launch
+inline double cost_us(const Plan* p, int n) {
+  const int tile = p[0].tile;
+  const int64_t s = slots(tile);
+  const double begin = tile == 256 ? 8.0 : tile == 128 ? 4.5 : 3.5;
+  int64_t items = 0, parts = 0;
+  for (int i = 0; i < n; i++) {
+    parts += (int64_t)p[i].rest * p[i].splits;
+    items += p[i].full;
+  }
+  items += parts;
+  const double step = step_us(tile, (double)std::min(items, s));
+  struct { double t; int64_t k; } free_at[32] = {{0.0, s}};        // k slots are free at t, the earliest first
+  int groups = 1;
+  double end = 0.0;
+  for (int i = 0; i < 2 * n; i++) {
+    const Plan& q = p[i / 2];
+    int64_t c = i % 2 ? (int64_t)q.rest * q.splits : q.full;
+    const double d = (i % 2 ? q.ksteps_split : q.ksteps) * step + begin;
+    if (c >= 2 * s) {                              // whole rounds at once
+      for (int k = 0; k < groups; k++) free_at[k].t += (double)(c / s - 1) * d;
+      c -= (c / s - 1) * s;
+    }
+    while (c > 0) {
+      const int64_t k = std::min(c, free_at[0].k);
+      const double t = free_at[0].t + d;
+      free_at[0].k -= k;
+      if (free_at[0].k == 0) {
+        for (int m = 1; m < groups; m++) free_at[m - 1] = free_at[m];
+        groups--;
+      }
+      int at = groups;
+      while (at > 0 && free_at[at - 1].t > t) at--;
+      if (at > 0 && free_at[at - 1].t == t) free_at[at - 1].k += k;
+      else if (groups == 32) free_at[31].k += k;   // (never that many: at most a few classes of items)
+      else {
+        for (int m = groups; m > at; m--) free_at[m] = free_at[m - 1];
+        free_at[at] = {t, k};
+        groups++;
+      }
+      end = std::max(end, t);
+      c -= k;
+    }
+    for (int k = 0; k < groups; k++) end = std::max(end, free_at[k].t);
+  }
+  return end + (parts ? 5.0 + (double)parts * (tile == 256 ? 0.1 : tile == 128 ? 0.025 : 0.00625) : 0.0);
+}
+// the ways a product may be cut: not at all; what is left over from whole rounds; every tile
+inline int ways(int tile, int64_t m, int64_t n, int steps, Plan* out) {
+  const int64_t tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, tiles = tm * tn, s = slots(tile);
+  if (tiles > (1 << 24)) return 0;
+  int count = 0;
+  out[count++] = Plan{tile, (int)tm, (int)tn, (int)tiles, 0, 1, steps, steps};
+  const int cuts[] = {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  for (int all = 0; all < 2; all++) {
+    const int64_t rest = all ? tiles : tiles % s;
+    if (rest == 0 || (all && (tiles > s || rest == tiles % s))) continue;
+    for (int c : cuts) {
+      if (steps / c < 4 || rest * c > 2 * s) break;
+      const int ks = (steps + c - 1) / c, real = (steps + ks - 1) / ks;
+      out[count++] = Plan{tile, (int)tm, (int)tn, (int)(tiles - rest), (int)rest, real, steps, ks};
+    }
+  }
+  return count;
+}
+constexpr int kWays = 24;
+
 inline void apply(Gemm& g, const Plan& p, int64_t m, int64_t n) {
   g.tiles_m = p.tiles_m;
   g.full = p.full;
   g.rest = p.rest;
   g.splits = p.splits;
+  g.ksteps = p.ksteps;
   g.ksteps_split = p.ksteps_split;
   g.m = g.c ? (int)m : 0;                          // (column sums alone: nothing of the product is stored)
   g.n = (int)n;

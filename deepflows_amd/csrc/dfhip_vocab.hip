@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "dfhip_splitgemm.h"
 
@@ -389,7 +390,56 @@ int launch_pair(const Pair& p) {
   return DFHIP_OK;
 }
 
-constexpr int kTiles[3] = {256, 128, 64};
+template <class F>
+int with_tile(const Plan& p, F f) {
+  if (p.tile == 256) return f(std::integral_constant<int, 256>());
+  if (p.tile == 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 64>());
+}
+
+// The cheapest way through a call's products.  A training loop asks for the same few again and again: the last answers are kept,
+// by the sizes alone.
+// `dw_rows`: rows of the weight product that are wanted -- width, 1 for the bias gradient alone (a product one tile high of which
+// nothing is stored), 0 for neither.
+struct Choice {
+  int64_t rows, width, classes;
+  bool dx;
+  int64_t dw_rows;
+  Plan logits, a, b;
+};
+const Choice* choose(int64_t rows, int64_t width, int64_t classes, bool dx, int64_t dw_rows) {
+  static thread_local Choice kept[8] = {};
+  static thread_local int turn = 0;
+  for (const Choice& c : kept)
+    if (c.rows == rows && c.width == width && c.classes == classes && c.dx == dx && c.dw_rows == dw_rows && c.logits.tile)
+      return &c;
+  Choice c = {};
+  c.rows = rows; c.width = width; c.classes = classes; c.dx = dx; c.dw_rows = dw_rows;
+  double least = 1e300, least_pair = 1e300;
+  for (int tile : {256, 128, 64}) {
+    Plan l[kWays], a[kWays] = {}, b[kWays] = {};
+    const int nl = ways(tile, rows, classes, (int)df_ceil_div(width, 32), l);
+    for (int i = 0; i < nl; i++) {
+      const double us = cost_us(&l[i], 1);
+      if (us < least) { least = us; c.logits = l[i]; }
+    }
+    if (!dx && !dw_rows) continue;
+    a[0].tile = b[0].tile = tile;                  // (no product)
+    const int na = dx ? ways(tile, rows, width, (int)df_ceil_div(classes, 32), a) : 1;
+    const int nb = dw_rows ? ways(tile, dw_rows, classes, (int)df_ceil_div(rows, 32), b) : 1;
+    for (int i = 0; i < na; i++)
+      for (int j = 0; j < nb; j++) {
+        Plan both[2] = {a[i], b[j]};
+        const double us = dx && dw_rows ? cost_us(both, 2) : cost_us(dx ? &a[i] : &b[j], 1);
+        if (us < least_pair) { least_pair = us; c.a = a[i]; c.b = b[j]; }
+      }
+  }
+  if (!c.logits.tile || ((dx || dw_rows) && !c.a.tile)) return nullptr;
+  kept[turn] = c;
+  const Choice* at = &kept[turn];
+  turn = (turn + 1) & 7;
+  return at;
+}
 
 int rows_pass(float* logits, const float* target, int n, int launch_rows, float* rowloss, int classes, int cells, float ignore,
               float smooth, int grads) {
@@ -463,45 +513,24 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     g.lda = dp * 4;
     g.b = (const char*)ws.p;
     g.ldb = vp * 4;
-    g.ksteps = (int)df_ceil_div(width, 32);
     g.c = logits.p;
     g.ldc = vp;
     g.bias = bias;
     g.exp_a = &ctl->ex;
     g.exp_b = &ctl->ew;
-    {
-      Plan best = plan(kTiles[0], n, classes, g.ksteps);
-      for (int t : {kTiles[1], kTiles[2]}) {
-        const Plan q = plan(t, n, classes, g.ksteps);
-        if (q.us < best.us) best = q;
-      }
-      DF_CHECK_ARG(best.tile, "linear_ce_forward: too many tiles");
-      apply(g, best, n, classes);
-      st = room(parts, held, parts_floats(best));
-      if (st != DFHIP_OK) return st;
-      g.parts = parts.p;
-      st = best.tile == 256 ? launch_logits<256>(g) : best.tile == 128 ? launch_logits<128>(g) : launch_logits<64>(g);
-      if (st != DFHIP_OK) return st;
-    }
+    const Choice* how = choose(n, width, classes, dx != nullptr, dw ? width : db ? 1 : 0);
+    DF_CHECK_ARG(how, "linear_ce_forward: too many tiles");
+    apply(g, how->logits, n, classes);
+    st = room(parts, held, std::max(parts_floats(how->logits), parts_floats(how->a) + parts_floats(how->b)));
+    if (st != DFHIP_OK) return st;
+    g.parts = parts.p;
+    st = with_tile(how->logits, [&](auto t) { return launch_logits<decltype(t)::value>(g); });
+    if (st != DFHIP_OK) return st;
     st = rows_pass(logits.p, target + r0, (int)n, (int)(grads ? df_ceil_div(n, 32) * 32 : n), rowloss + r0, (int)classes, (int)vp,
                    ignore, (float)label_smoothing, grads ? 1 : 0);
     if (st != DFHIP_OK) return st;
     if (!grads) continue;
     Pair p = {};
-    Plan pa = {}, pb = {};
-    double least = 1e31;
-    const int steps_a = (int)df_ceil_div(classes, 32), steps_b = (int)df_ceil_div(n, 32);
-    const int64_t mb = dw ? width : 1;             // (db alone: one tile high, nothing of the product stored)
-    for (int t : kTiles) {
-      Plan qa = {}, qb = {};
-      qa.tile = qb.tile = t;
-      if (dx) qa = plan(t, n, width, steps_a);
-      if (dw || db) qb = plan(t, mb, classes, steps_b);
-      if (qa.us + qb.us < least) { least = qa.us + qb.us; pa = qa; pb = qb; }
-    }
-    DF_CHECK_ARG(pa.tile && pb.tile, "linear_ce_forward: too many tiles");
-    st = room(parts, held, parts_floats(pa) + parts_floats(pb));
-    if (st != DFHIP_OK) return st;
     p.a.exp_c = p.b.exp_c = -kTop;
     p.a.scale = p.b.scale = &ctl->scale;
     if (dx) {
@@ -509,12 +538,11 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
       p.a.lda = vp * 4;
       p.a.b = (const char*)ws.p;
       p.a.ldb = vp * 4;
-      p.a.ksteps = steps_a;
       p.a.c = dx + r0 * width;
       p.a.ldc = width;
       p.a.exp_a = &ctl->ew;
       p.a.parts = parts.p;
-      apply(p.a, pa, n, width);
+      apply(p.a, how->a, n, width);
       p.na = groups(p.a);
     }
     if (dw || db) {
@@ -522,13 +550,12 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
       p.b.lda = dp * 4;
       p.b.b = (const char*)logits.p;
       p.b.ldb = vp * 4;
-      p.b.ksteps = steps_b;
       p.b.c = dw;
       p.b.ldc = classes;
       p.b.exp_a = &ctl->ex;
       p.b.colsum = db;
-      p.b.parts = parts.p + parts_floats(pa);
-      apply(p.b, pb, mb, classes);
+      p.b.parts = parts.p + parts_floats(how->a);
+      apply(p.b, how->b, width, classes);
       p.nb = groups(p.b);
     }
     if (r0 + n == rows) {
@@ -537,10 +564,10 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
       p.loss = loss;
       p.rows = rows;
     }
-    if (r0 == 0)
-      st = pa.tile == 256 ? launch_pair<256, EPI_STORE>(p) : pa.tile == 128 ? launch_pair<128, EPI_STORE>(p) : launch_pair<64, EPI_STORE>(p);
-    else
-      st = pa.tile == 256 ? launch_pair<256, EPI_ADD>(p) : pa.tile == 128 ? launch_pair<128, EPI_ADD>(p) : launch_pair<64, EPI_ADD>(p);
+    st = with_tile(how->a, [&](auto t) {
+      constexpr int T = decltype(t)::value;
+      return r0 == 0 ? launch_pair<T, EPI_STORE>(p) : launch_pair<T, EPI_ADD>(p);
+    });
     if (st != DFHIP_OK) return st;
   }
   if (grads) return DFHIP_OK;
