@@ -72,12 +72,15 @@ template <int EPI>
 __device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
   return EPI == EPI_BIAS && g.bias && n < g.n ? g.bias[n] : 0.0f;
 }
-// one value of row m (c: its place) and column n
-template <int EPI>
+// One value of row m (c: its place) and column n.  STREAM: past the caches, where a wave's stores fill whole lines -- a round of
+// 256 x 256 tiles writes 64 MB that nothing reads soon, and the operands' lines stay (eval 1500 x 1024 x 30011: 373 -> 355 us).
+template <int EPI, bool STREAM>
 __device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias, int64_t m, int64_t n, float* c, float v) {
-  if (EPI == EPI_BIAS) *c = ldexpf(v, e) + bias;
-  if (EPI == EPI_STORE && m < g.m && n < g.n) *c = ldexpf(v, e) * sc;
-  if (EPI == EPI_ADD && m < g.m && n < g.n) *c += ldexpf(v, e) * sc;
+  if (EPI != EPI_BIAS && (m >= g.m || n >= g.n)) return;
+  v = EPI == EPI_BIAS ? ldexpf(v, e) + bias : ldexpf(v, e) * sc;
+  if (EPI == EPI_ADD) *c += v;
+  else if (STREAM) __builtin_nontemporal_store(v, c);
+  else *c = v;
 }
 template <int EPI>
 __device__ __forceinline__ void emit_colsum(const Gemm& g, float sc, int64_t n, float v) {
@@ -352,7 +355,7 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
       const int64_t m = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
       float* c = g.c + m * g.ldc + n;
 #pragma unroll
-      for (int j = 0; j < TN; j++) emit<EPI>(g, e, sc, bias[j], m, n + j * 32, c + j * 32, acc[i][j][r]);
+      for (int j = 0; j < TN; j++) emit<EPI, true>(g, e, sc, bias[j], m, n + j * 32, c + j * 32, acc[i][j][r]);
     }
 }
 
@@ -392,7 +395,7 @@ __device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
 #pragma unroll
   for (int k = 0; k < 4; k++) bias[k] = bias_of<EPI>(g, n + k);
 #pragma unroll
-  for (int k = 0; k < 4; k++) emit<EPI>(g, e, sc, bias[k], m0 + cell / BN, n + k, g.c + (m0 + cell / BN) * g.ldc + n + k, v[k]);
+  for (int k = 0; k < 4; k++) emit<EPI, false>(g, e, sc, bias[k], m0 + cell / BN, n + k, g.c + (m0 + cell / BN) * g.ldc + n + k, v[k]);
   if (g.colsum && tm == 0 && slice == 0 && (int)threadIdx.x < BN) {
     const float* c = part + BM * BN + threadIdx.x;
     float s = 0.0f;
