@@ -54,7 +54,7 @@ enum { EPI_BIAS = 0, EPI_STORE = 1, EPI_ADD = 2 };
 struct Gemm {
   const char *a, *b;                     // split arrays
   int64_t lda, ldb;                      // bytes a storage row
-  int tiles_m, full, rest, splits;
+  int tiles_m, tiles_n, full, rest, splits;
   int ksteps, ksteps_split;              // steps of 32 along the reduction, in all and for a part
   float* c;
   int64_t ldc;
@@ -67,6 +67,13 @@ struct Gemm {
   float* colsum;                         // or NULL: column sums of b (n), scaled by 2^exp_c * scale; added where EPI_ADD (b across)
   float* parts;                          // (rest * splits) x (BM * BN + BN)
 };
+
+// place of a tile: bands of eight tile rows, down the band first
+__device__ __forceinline__ void place(const Gemm& g, int tile, int& tm, int& tn) {
+  const int band = tile / (8 * g.tiles_n), in = tile - band * 8 * g.tiles_n, high = min(8, g.tiles_m - band * 8);
+  tn = in / high;
+  tm = band * 8 + in - tn * high;
+}
 
 template <int EPI>
 __device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
@@ -202,15 +209,16 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
   static_assert((BM / WM) % 64 == 0 || TM == 1, "Reader");
   static_assert((BN / WN) % 64 == 0 || TN == 1, "Reader");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (rows fastest), so that the
-  // tiles that share a column of B meet in one L2
+  // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles, and the 32 that it works on at a
+  // time are 8 x 4 neighbours, which go along the reduction together and share 12 operand tiles in its L2 (a column of 32: 33)
   const bool whole = block < (g.full + 7) / 8 * 8;
   const int id = whole ? block : block - (g.full + 7) / 8 * 8;
   const int total = whole ? g.full : g.rest * g.splits, per = (total + 7) >> 3;
   const int item = (id & 7) * per + (id >> 3);
   if ((id >> 3) >= per || item >= total) return;
   const int z = whole ? 0 : item / g.rest, tile = whole ? item : g.full + item % g.rest;
-  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
+  int tm, tn;
+  place(g, tile, tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const int k0 = whole ? 0 : z * g.ksteps_split, steps = whole ? g.ksteps : min(g.ksteps - k0, g.ksteps_split);
   const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
@@ -370,7 +378,8 @@ template <int T, int EPI>
 __device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
   constexpr int BM = T, BN = T, SLICES = BM * BN / 1024, CELLS = BM * BN + BN;
   const int t = block / SLICES, slice = block % SLICES, tile = g.full + t;
-  const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
+  int tm, tn;
+  place(g, tile, tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const float* part = g.parts + (int64_t)t * g.splits * CELLS;
   const int e = exponent(g);
@@ -488,6 +497,7 @@ constexpr int kWays = 24;
 
 inline void apply(Gemm& g, const Plan& p, int64_t m, int64_t n) {
   g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
   g.full = p.full;
   g.rest = p.rest;
   g.splits = p.splits;
