@@ -6,9 +6,12 @@
 // Bound: HBM.  Forward 16 bytes an element (x, residual in; y, h out), backward 16 (dy, h, the other gradient in; dx out): a
 // row is held in registers between the reduction and its use, so every array is touched once.
 //
-// Layout: a row belongs to a TEAM of threads, a quarter of a wave up to four waves, V consecutive elements a thread and trip:
-//   width <= 128: 16 lanes a row, <= 512: 32 lanes, <= 1024: one wave, <= 16384: four waves; wider rows: four waves that read
-//   the row twice (the second time out of L2).
+// Layout: a row belongs to a TEAM of threads, four consecutive elements a thread and trip:
+//   width <= 128: 16 lanes a row, <= 512: 32 lanes, <= 1024: one wave, <= 4096: four waves, <= 16384 (forward: 32768): sixteen;
+//   wider rows: sixteen waves that read the row twice (the second time out of L2).
+// Loads and stores are 16 bytes wherever the row begins (the hardware asks for 4-byte alignment only): 4-byte accesses for rows of
+// a width that is no multiple of 4 cost 20 % at 1860 x 3578 and 58 % at 315 x 12242 (31 -> 13 us).
+// Measured, with residual: 16384 x 4096 both ways 390 us = 5.5 TB/s, 3890 x 3056 forward 29 us = 6.5 TB/s (a large copy: 5.1).
 // A thread keeps the same columns for every row its team works on, so the sum over rows of dy n stays in registers until the
 // end; the teams of a workgroup meet in LDS, the workgroups' partial rows are added by a second launch in a fixed order.
 #include <math.h>
@@ -22,23 +25,34 @@ using namespace dfhip;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWide = 1024;
+template <int T> constexpr int threads() { return T > kThreads ? T : kThreads; }
 
-template <int V> struct Vec;
-template <> struct Vec<4> { typedef float4 type; };
-template <> struct Vec<1> { typedef float type; };
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
-template <int V>
-__device__ __forceinline__ void vload(float* v, const float* p) {
-  if (V == 4) { const float4 t = *reinterpret_cast<const float4*>(p); v[0] = t.x; v[1 % V] = t.y; v[2 % V] = t.z; v[3 % V] = t.w; }
-  else v[0] = p[0];
+// four elements of which `left` exist; what does not reads as zero and is not written
+__device__ __forceinline__ void load4(float* v, const float* p, int64_t left) {
+  if (left >= 4) {
+    const float4u t = *reinterpret_cast<const float4u*>(p);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = e < left ? p[e] : 0.0f;
+  }
 }
-template <int V>
-__device__ __forceinline__ void vstore(float* p, const float* v) {
-  if (V == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
-  else p[0] = v[0];
+__device__ __forceinline__ void store4(float* p, const float* v, int64_t left) {
+  if (left >= 4) {
+    float4u t;
+    t.x = v[0]; t.y = v[1]; t.z = v[2]; t.w = v[3];
+    *reinterpret_cast<float4u*>(p) = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (e < left) p[e] = v[e];
+  }
 }
 
-// the sum over the T threads of a team, in every one of them (T <= 64: lanes of one wave; T == kThreads: the workgroup)
+// the sum over the T threads of a team, in every one of them (T <= 64: lanes of one wave; more: the workgroup)
 template <int T, class X>
 __device__ __forceinline__ X team_sum(X v, X* sh) {
 #pragma unroll
@@ -49,148 +63,135 @@ __device__ __forceinline__ X team_sum(X v, X* sh) {
     __syncthreads();
     v = sh[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; w++) v += sh[w];
+    for (int w = 1; w < T / 64; w++) v += sh[w];
   }
   return v;
 }
 
-// U trips of V elements a thread cover the row: T * U * V >= width
-template <int T, int U, int V, bool RES>
-__global__ __launch_bounds__(kThreads) void k_rms_fwd(const float* __restrict__ x, const float* res,
-                                                      const float* __restrict__ w, float* __restrict__ y, float* h,
-                                                      float* __restrict__ rstd, int64_t rows, int width, float eps) {
-  __shared__ double sh[kThreads / 64];
+// U trips of four elements a thread cover the row: T * U * 4 >= width
+template <int T, int U, bool RES>
+__global__ __launch_bounds__(threads<T>()) void k_rms_fwd(const float* __restrict__ x, const float* res,
+                                                          const float* __restrict__ w, float* __restrict__ y, float* h,
+                                                          float* __restrict__ rstd, int64_t rows, int width, double inv, float eps) {
+  __shared__ double sh[threads<T>() / 64];
   const int team = threadIdx.x / T, lane = threadIdx.x % T;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / T) + team;
+  const int64_t row = (int64_t)blockIdx.x * (threads<T>() / T) + team;
   const bool live = row < rows;                    // (a team whose row does not exist keeps the others company at barriers)
   const int64_t base = (live ? row : 0) * width;
-  float v[U][V];
+  float v[U][4];
   double ss = 0.0;
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const int c = (u * T + lane) * V;
-    if (c < width) vload<V>(v[u], x + base + c);
-    else
-#pragma unroll
-      for (int e = 0; e < V; e++) v[u][e] = 0.0f;
+    const int c = (u * T + lane) * 4;
+    load4(v[u], x + base + c, width - c);
   }
   if (RES) {
+    float r[U][4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int c = (u * T + lane) * V;
-      if (c < width) {
-        float r[V];
-        vload<V>(r, res + base + c);
+      const int c = (u * T + lane) * 4;
+      load4(r[u], res + base + c, width - c);
+    }
 #pragma unroll
-        for (int e = 0; e < V; e++) v[u][e] += r[e];
-        if (live) vstore<V>(h + base + c, v[u]);
-      }
+    for (int u = 0; u < U; u++) {
+      const int c = (u * T + lane) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[u][e] += r[u][e];
+      if (live) store4(h + base + c, v[u], width - c);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int e = 0; e < V; e++) ss = fma((double)v[u][e], (double)v[u][e], ss);
+    for (int e = 0; e < 4; e++) ss = fma((double)v[u][e], (double)v[u][e], ss);
   ss = team_sum<T>(ss, sh);
-  const float r = (float)(1.0 / sqrt(ss / (double)width + (double)eps));
+  const float r = (float)(1.0 / sqrt(fma(ss, inv, (double)eps)));
   if (!live) return;
   if (rstd && lane == 0) rstd[row] = r;
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const int c = (u * T + lane) * V;
-    if (c < width) {
-      float o[V], wv[V];
-      if (w) vload<V>(wv, w + c);
+    const int c = (u * T + lane) * 4;
+    float o[4], wv[4];
+    if (w) load4(wv, w + c, width - c);
 #pragma unroll
-      for (int e = 0; e < V; e++) o[e] = w ? v[u][e] * r * wv[e] : v[u][e] * r;
-      vstore<V>(y + base + c, o);
-    }
+    for (int e = 0; e < 4; e++) o[e] = w ? v[u][e] * r * wv[e] : v[u][e] * r;
+    store4(y + base + c, o, width - c);
   }
 }
 
 // rows wider than the registers hold: the row twice
-template <int V, bool RES>
-__global__ __launch_bounds__(kThreads) void k_rms_fwd_wide(const float* x, const float* res, const float* __restrict__ w,
-                                                           float* __restrict__ y, float* h, float* __restrict__ rstd,
-                                                           int64_t width, float eps) {
-  __shared__ double sh[kThreads / 64];
+template <bool RES>
+__global__ __launch_bounds__(kWide) void k_rms_fwd_wide(const float* x, const float* res, const float* __restrict__ w,
+                                                        float* __restrict__ y, float* h, float* __restrict__ rstd, int64_t width,
+                                                        double inv, float eps) {
+  __shared__ double sh[kWide / 64];
   const int64_t base = (int64_t)blockIdx.x * width;
   double ss = 0.0;
-  for (int64_t c = (int64_t)threadIdx.x * V; c < width; c += kThreads * V) {
-    float v[V];
-    vload<V>(v, x + base + c);
+  for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += kWide * 4) {
+    float v[4];
+    load4(v, x + base + c, width - c);
     if (RES) {
-      float r[V];
-      vload<V>(r, res + base + c);
+      float r[4];
+      load4(r, res + base + c, width - c);
 #pragma unroll
-      for (int e = 0; e < V; e++) v[e] += r[e];
-      vstore<V>(h + base + c, v);
+      for (int e = 0; e < 4; e++) v[e] += r[e];
+      store4(h + base + c, v, width - c);
     }
 #pragma unroll
-    for (int e = 0; e < V; e++) ss = fma((double)v[e], (double)v[e], ss);
+    for (int e = 0; e < 4; e++) ss = fma((double)v[e], (double)v[e], ss);
   }
-  ss = team_sum<kThreads>(ss, sh);
-  const float r = (float)(1.0 / sqrt(ss / (double)width + (double)eps));
+  ss = team_sum<kWide>(ss, sh);
+  const float r = (float)(1.0 / sqrt(fma(ss, inv, (double)eps)));
   if (rstd && threadIdx.x == 0) rstd[blockIdx.x] = r;
   const float* s = RES ? h : x;                    // (each thread reads back what it wrote itself)
-  for (int64_t c = (int64_t)threadIdx.x * V; c < width; c += kThreads * V) {
-    float v[V], wv[V];
-    vload<V>(v, s + base + c);
-    if (w) vload<V>(wv, w + c);
+  for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += kWide * 4) {
+    float v[4], wv[4];
+    load4(v, s + base + c, width - c);
+    if (w) load4(wv, w + c, width - c);
 #pragma unroll
-    for (int e = 0; e < V; e++) v[e] = w ? v[e] * r * wv[e] : v[e] * r;
-    vstore<V>(y + base + c, v);
+    for (int e = 0; e < 4; e++) v[e] = w ? v[e] * r * wv[e] : v[e] * r;
+    store4(y + base + c, v, width - c);
   }
 }
 
 // partial: gridDim.x rows of `width` sums of dy n, or NULL
-template <int T, int U, int V>
-__global__ __launch_bounds__(kThreads) void k_rms_bwd(const float* __restrict__ dy, const float* __restrict__ h,
-                                                      const float* __restrict__ rstd, const float* __restrict__ w,
-                                                      const float* add, float* dx, float* __restrict__ partial, int64_t rows,
-                                                      int width) {
-  __shared__ float sh[kThreads / 64];
-  constexpr int TEAMS = kThreads / T;
-  __shared__ float meet[TEAMS > 1 ? T * U * V * TEAMS : 1];
+template <int T, int U>
+__global__ __launch_bounds__(threads<T>()) void k_rms_bwd(const float* __restrict__ dy, const float* __restrict__ h,
+                                                          const float* __restrict__ rstd, const float* __restrict__ w,
+                                                          const float* add, float* dx, float* __restrict__ partial, int64_t rows,
+                                                          int width) {
+  __shared__ float sh[threads<T>() / 64];
+  constexpr int TEAMS = threads<T>() / T;
+  __shared__ float meet[TEAMS > 1 ? T * U * 4 * TEAMS : 1];
   const int team = threadIdx.x / T, lane = threadIdx.x % T;
-  float sum[U][V];
-#pragma unroll
-  for (int u = 0; u < U; u++)
-#pragma unroll
-    for (int e = 0; e < V; e++) sum[u][e] = 0.0f;
-  float wv[U][V];
+  float sum[U][4], wv[U][4];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const int c = (u * T + lane) * V;
+    const int c = (u * T + lane) * 4;
 #pragma unroll
-    for (int e = 0; e < V; e++) wv[u][e] = 1.0f;
-    if (w && c < width) vload<V>(wv[u], w + c);
+    for (int e = 0; e < 4; e++) { sum[u][e] = 0.0f; wv[u][e] = 1.0f; }
+    if (w) load4(wv[u], w + c, width - c);
   }
   const float inv = 1.0f / (float)width;
   const int64_t step = (int64_t)gridDim.x * TEAMS;
-  // (the trip count is the workgroup's, so that every thread reaches the barriers of a four-wave team)
+  // (the trip count is the workgroup's, so that every thread reaches the barriers of a team of several waves)
   for (int64_t row0 = (int64_t)blockIdx.x * TEAMS; row0 < rows; row0 += step) {
     const bool live = row0 + team < rows;
     const int64_t row = live ? row0 + team : row0;
     const int64_t base = row * width;
     const float r = rstd[row];
-    float g[U][V], n[U][V];
+    float g[U][4], n[U][4];
     float dot = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int c = (u * T + lane) * V;
-      if (c < width) {
-        vload<V>(g[u], dy + base + c);
-        vload<V>(n[u], h + base + c);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; e++) g[u][e] = n[u][e] = 0.0f;
-      }
+      const int c = (u * T + lane) * 4;
+      load4(g[u], dy + base + c, width - c);
+      load4(n[u], h + base + c, width - c);
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int e = 0; e < V; e++) {
+      for (int e = 0; e < 4; e++) {
         n[u][e] *= r;
         if (live) sum[u][e] = fmaf(g[u][e], n[u][e], sum[u][e]);
         g[u][e] *= wv[u][e];
@@ -201,19 +202,17 @@ __global__ __launch_bounds__(kThreads) void k_rms_bwd(const float* __restrict__ 
     if (live)
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int c = (u * T + lane) * V;
-        if (c < width) {
-          float o[V];
+        const int c = (u * T + lane) * 4;
+        float o[4];
 #pragma unroll
-          for (int e = 0; e < V; e++) o[e] = r * (g[u][e] - n[u][e] * c1);
-          if (add) {
-            float a[V];
-            vload<V>(a, add + base + c);
+        for (int e = 0; e < 4; e++) o[e] = r * (g[u][e] - n[u][e] * c1);
+        if (add) {
+          float a[4];
+          load4(a, add + base + c, width - c);
 #pragma unroll
-            for (int e = 0; e < V; e++) o[e] += a[e];
-          }
-          vstore<V>(dx + base + c, o);
+          for (int e = 0; e < 4; e++) o[e] += a[e];
         }
+        store4(dx + base + c, o, width - c);
       }
   }
   if (!partial) return;
@@ -221,57 +220,54 @@ __global__ __launch_bounds__(kThreads) void k_rms_bwd(const float* __restrict__ 
   if (TEAMS == 1) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int c = (u * T + lane) * V;
-      if (c < width)
-#pragma unroll
-        for (int e = 0; e < V; e++) prow[c + e] = sum[u][e];
+      const int c = (u * T + lane) * 4;
+      store4(prow + c, sum[u], width - c);
     }
     return;
   }
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int e = 0; e < V; e++) meet[team * (T * U * V) + (u * T + lane) * V + e] = sum[u][e];
+    for (int e = 0; e < 4; e++) meet[team * (T * U * 4) + (u * T + lane) * 4 + e] = sum[u][e];
   __syncthreads();
-  for (int c = threadIdx.x; c < width; c += kThreads) {
+  for (int c = threadIdx.x; c < width; c += threads<T>()) {
     float s = 0.0f;
 #pragma unroll
-    for (int t = 0; t < TEAMS; t++) s += meet[t * (T * U * V) + c];
+    for (int t = 0; t < TEAMS; t++) s += meet[t * (T * U * 4) + c];
     prow[c] = s;
   }
 }
 
 // rows wider than the registers hold: dx alone, a workgroup a row
-template <int V>
-__global__ __launch_bounds__(kThreads) void k_rms_bwd_wide(const float* __restrict__ dy, const float* __restrict__ h,
-                                                           const float* __restrict__ rstd, const float* __restrict__ w,
-                                                           const float* add, float* dx, int64_t width) {
-  __shared__ float sh[kThreads / 64];
+__global__ __launch_bounds__(kWide) void k_rms_bwd_wide(const float* __restrict__ dy, const float* __restrict__ h,
+                                                        const float* __restrict__ rstd, const float* __restrict__ w,
+                                                        const float* add, float* dx, int64_t width) {
+  __shared__ float sh[kWide / 64];
   const int64_t base = (int64_t)blockIdx.x * width;
   const float r = rstd[blockIdx.x];
   float dot = 0.0f;
-  for (int64_t c = (int64_t)threadIdx.x * V; c < width; c += kThreads * V) {
-    float g[V], n[V], wv[V];
-    vload<V>(g, dy + base + c);
-    vload<V>(n, h + base + c);
-    if (w) vload<V>(wv, w + c);
+  for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += kWide * 4) {
+    float g[4], n[4], wv[4];
+    load4(g, dy + base + c, width - c);
+    load4(n, h + base + c, width - c);
+    if (w) load4(wv, w + c, width - c);
 #pragma unroll
-    for (int e = 0; e < V; e++) dot = fmaf(w ? g[e] * wv[e] : g[e], n[e] * r, dot);
+    for (int e = 0; e < 4; e++) dot = fmaf(w ? g[e] * wv[e] : g[e], n[e] * r, dot);
   }
-  const float c1 = team_sum<kThreads>(dot, sh) * (1.0f / (float)width);
-  for (int64_t c = (int64_t)threadIdx.x * V; c < width; c += kThreads * V) {
-    float g[V], n[V], wv[V], a[V];
-    vload<V>(g, dy + base + c);
-    vload<V>(n, h + base + c);
-    if (w) vload<V>(wv, w + c);
-    if (add) vload<V>(a, add + base + c);
+  const float c1 = team_sum<kWide>(dot, sh) * (1.0f / (float)width);
+  for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += kWide * 4) {
+    float g[4], n[4], wv[4], a[4];
+    load4(g, dy + base + c, width - c);
+    load4(n, h + base + c, width - c);
+    if (w) load4(wv, w + c, width - c);
+    if (add) load4(a, add + base + c, width - c);
 #pragma unroll
-    for (int e = 0; e < V; e++) {
+    for (int e = 0; e < 4; e++) {
       float o = r * ((w ? g[e] * wv[e] : g[e]) - n[e] * r * c1);
       if (add) o += a[e];
       g[e] = o;
     }
-    vstore<V>(dx + base + c, g);
+    store4(dx + base + c, g, width - c);
   }
 }
 
@@ -311,56 +307,58 @@ __global__ __launch_bounds__(1024) void k_rms_dw_sum(const float* __restrict__ p
   }
 }
 
-template <int T, int U, int V>
+template <int T, int U>
 int fwd(const float* x, const float* res, const float* w, float* y, float* h, float* rstd, int64_t rows, int64_t width, float eps) {
-  const dim3 grid((unsigned)df_ceil_div(rows, kThreads / T));
-  if (res) DF_LAUNCH((k_rms_fwd<T, U, V, true>), grid, dim3(kThreads), 0, stream(), x, res, w, y, h, rstd, rows, (int)width, eps);
-  else DF_LAUNCH((k_rms_fwd<T, U, V, false>), grid, dim3(kThreads), 0, stream(), x, res, w, y, h, rstd, rows, (int)width, eps);
+  const dim3 grid((unsigned)df_ceil_div(rows, threads<T>() / T)), block(threads<T>());
+  if (res) DF_LAUNCH((k_rms_fwd<T, U, true>), grid, block, 0, stream(), x, res, w, y, h, rstd, rows, (int)width, 1.0 / (double)width, eps);
+  else DF_LAUNCH((k_rms_fwd<T, U, false>), grid, block, 0, stream(), x, res, w, y, h, rstd, rows, (int)width, 1.0 / (double)width, eps);
   DF_LAUNCH_CHECK();
   return DFHIP_OK;
 }
 
-template <int T, int U, int V>
+template <int T, int U>
 int bwd(const float* dy, const float* h, const float* rstd, const float* w, const float* add, float* dx, float* partial,
         int blocks, int64_t rows, int64_t width) {
-  DF_LAUNCH((k_rms_bwd<T, U, V>), dim3(blocks), dim3(kThreads), 0, stream(), dy, h, rstd, w, add, dx, partial, rows, (int)width);
+  DF_LAUNCH((k_rms_bwd<T, U>), dim3(blocks), dim3(threads<T>()), 0, stream(), dy, h, rstd, w, add, dx, partial, rows, (int)width);
   DF_LAUNCH_CHECK();
   return DFHIP_OK;
 }
 
-// the team of a row of `width` elements, V elements a load: f(T, U) of the narrowest form that holds it
-#define RMS_FORMS(V, CALL)                                                   \
-  do {                                                                       \
-    const int64_t per = (width + V - 1) / V;                                 \
-    if (per <= 16 * (8 / V)) return CALL(16, 8 / V, V);                      \
-    if (per <= 32 * (16 / V)) return CALL(32, 16 / V, V);                    \
-    if (per <= 64 * (16 / V)) return CALL(64, 16 / V, V);                    \
-    if (per <= 256 * (8 / V)) return CALL(256, 8 / V, V);                    \
-    if (per <= 256 * (16 / V)) return CALL(256, 16 / V, V);                  \
-    if (per <= 256 * (32 / V)) return CALL(256, 32 / V, V);                  \
-    if (per <= 256 * (64 / V)) return CALL(256, 64 / V, V);                  \
+// the team of a row of `width` elements: CALL(T, U) of the narrowest form that holds it
+#define RMS_FORMS(CALL)                      \
+  do {                                       \
+    if (width <= 64) return CALL(16, 1);     \
+    if (width <= 128) return CALL(16, 2);    \
+    if (width <= 256) return CALL(32, 2);    \
+    if (width <= 512) return CALL(32, 4);    \
+    if (width <= 1024) return CALL(64, 4);   \
+    if (width <= 2048) return CALL(256, 2);  \
+    if (width <= 4096) return CALL(256, 4);  \
+    if (width <= 8192) return CALL(1024, 2); \
+    if (width <= 16384) return CALL(1024, 4);\
   } while (0)
 
-template <int V>
 int run_fwd(const float* x, const float* res, const float* w, float* y, float* h, float* rstd, int64_t rows, int64_t width,
             float eps) {
-#define CALL(T, U, V) fwd<T, U, V>(x, res, w, y, h, rstd, rows, width, eps)
-  RMS_FORMS(V, CALL);
+#define CALL(T, U) fwd<T, U>(x, res, w, y, h, rstd, rows, width, eps)
+  RMS_FORMS(CALL);
+  if (width <= 32768) return CALL(1024, 8);        // (the backward pass holds twice as many values a thread: it would spill)
 #undef CALL
-  if (res) DF_LAUNCH((k_rms_fwd_wide<V, true>), dim3((unsigned)rows), dim3(kThreads), 0, stream(), x, res, w, y, h, rstd, width, eps);
-  else DF_LAUNCH((k_rms_fwd_wide<V, false>), dim3((unsigned)rows), dim3(kThreads), 0, stream(), x, res, w, y, h, rstd, width, eps);
+  if (res) DF_LAUNCH(k_rms_fwd_wide<true>, dim3((unsigned)rows), dim3(kWide), 0, stream(), x, res, w, y, h, rstd, width,
+                     1.0 / (double)width, eps);
+  else DF_LAUNCH(k_rms_fwd_wide<false>, dim3((unsigned)rows), dim3(kWide), 0, stream(), x, res, w, y, h, rstd, width,
+                     1.0 / (double)width, eps);
   DF_LAUNCH_CHECK();
   return DFHIP_OK;
 }
 
-template <int V>
 int run_bwd(const float* dy, const float* h, const float* rstd, const float* w, const float* add, float* dx, float* partial,
             int blocks, int64_t rows, int64_t width) {
-#define CALL(T, U, V) bwd<T, U, V>(dy, h, rstd, w, add, dx, partial, blocks, rows, width)
-  RMS_FORMS(V, CALL);
+#define CALL(T, U) bwd<T, U>(dy, h, rstd, w, add, dx, partial, blocks, rows, width)
+  RMS_FORMS(CALL);
 #undef CALL
   if (dx) {
-    DF_LAUNCH(k_rms_bwd_wide<V>, dim3((unsigned)rows), dim3(kThreads), 0, stream(), dy, h, rstd, w, add, dx, width);
+    DF_LAUNCH(k_rms_bwd_wide, dim3((unsigned)rows), dim3(kWide), 0, stream(), dy, h, rstd, w, add, dx, width);
     DF_LAUNCH_CHECK();
   }
   if (partial) {
@@ -369,12 +367,6 @@ int run_bwd(const float* dy, const float* h, const float* rstd, const float* w, 
     DF_LAUNCH_CHECK();
   }
   return DFHIP_OK;
-}
-
-bool aligned16(std::initializer_list<const void*> ps) {
-  uintptr_t a = 0;
-  for (const void* p : ps) a |= (uintptr_t)p;
-  return (a & 15) == 0;
 }
 
 int check_shape(const char* name, int64_t rows, int64_t width) {
@@ -396,9 +388,7 @@ int dfhip_rms_norm_forward(const float* x, const float* residual, const float* w
   if (rows == 0) return DFHIP_OK;
   DF_CHECK_ARG(x && y && (!residual || h), "rms_norm_forward: null array");
   ProfScope prof("rms_norm_fwd", 4.0 * (double)rows * (double)width, (residual ? 16.0 : 8.0) * (double)rows * (double)width);
-  const bool vec = width % 4 == 0 && aligned16({x, residual, weight, y, residual ? h : nullptr});
-  return vec ? run_fwd<4>(x, residual, weight, y, h, rstd, rows, width, eps)
-             : run_fwd<1>(x, residual, weight, y, h, rstd, rows, width, eps);
+  return run_fwd(x, residual, weight, y, h, rstd, rows, width, eps);
 }
 
 int dfhip_rms_norm_backward(const float* dy, const float* h, const float* rstd, const float* weight, const float* add,
@@ -410,17 +400,15 @@ int dfhip_rms_norm_backward(const float* dy, const float* h, const float* rstd, 
   if (rows == 0) return dweight ? dfhip_fill(dweight, width, 0.0f) : DFHIP_OK;
   DF_CHECK_ARG(dy && h && rstd, "rms_norm_backward: null array");
   ProfScope prof("rms_norm_bwd", 8.0 * (double)rows * (double)width, (add ? 16.0 : 12.0) * (double)rows * (double)width);
-  // workgroups that share the rows: two a CU, as many partial rows as workgroups
+  // workgroups that share the rows, and as many partial rows: a team waits for each row's loads, so narrow rows need many of them
   const int64_t teams = width <= 128 ? 16 : width <= 512 ? 8 : width <= 1024 ? 4 : 1;
-  const int blocks = (int)std::min<int64_t>(df_ceil_div(rows, teams), 2 * num_cus());
+  const int blocks = (int)std::min<int64_t>(df_ceil_div(rows, teams), (width <= 128 ? 8 : width <= 1024 ? 4 : 2) * num_cus());
   float* partial = nullptr;
   if (dweight) {
     partial = workspace((size_t)blocks * (size_t)width * sizeof(float));
     if (!partial) return DFHIP_OUT_OF_MEMORY;
   }
-  const bool vec = width % 4 == 0 && aligned16({dy, h, weight, add, dx});
-  st = vec ? run_bwd<4>(dy, h, rstd, weight, add, dx, partial, blocks, rows, width)
-           : run_bwd<1>(dy, h, rstd, weight, add, dx, partial, blocks, rows, width);
+  st = run_bwd(dy, h, rstd, weight, add, dx, partial, blocks, rows, width);
   if (st != DFHIP_OK || !dweight) return st;
   DF_LAUNCH(k_rms_dw_sum, dim3((unsigned)df_ceil_div(width, 64)), dim3(1024), 0, stream(), partial, dweight, blocks, width);
   DF_LAUNCH_CHECK();
