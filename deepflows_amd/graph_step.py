@@ -17,6 +17,7 @@ import sys
 
 import numpy as np
 
+from .optim.clip import clip_grad_norm_
 from .tensor import Graph
 
 
@@ -29,14 +30,20 @@ class CapturedTrainStep:
     captured graph where the collective can be captured (`exchange_captured`), else the graph ends after backward and they
     are enqueued eagerly behind every replay on the same stream."""
 
-    def __init__(self, model, criterion, optimizer, inputs, targets, sync=None, capture_exchange=None, steps_per_graph=1):
+    def __init__(self, model, criterion, optimizer, inputs, targets, sync=None, capture_exchange=None, steps_per_graph=1,
+                 max_grad_norm=None):
         """steps_per_graph = S > 1 (round 6): S consecutive steps in ONE graph -- a graph launch costs 5-8 us of device time
         whatever it holds (tools/probes/queue_probe.hip: 12.9 us for a graph of three empty kernels, 107 us for 58), a fifth of
         the perceptron's 19-us step.  `replay()` still advances ONE step per call: the graph is launched on every S-th call
         and holds that call's step and the S - 1 that follow (the loss it returns is the one of the graph's last step;
         Dropout masks of all S steps are drawn in step order in front of the launch; a tail of fewer than S calls has run
-        the whole graph).  `inputs` / `targets` may be lists of S tensors (one batch per step of the graph)."""
+        the whole graph).  `inputs` / `targets` may be lists of S tensors (one batch per step of the graph).
+
+        max_grad_norm: every step's gradients are scaled down to this common norm (optim.clip_grad_norm_) between the exchange and
+        the optimizer, inside the graph where the optimizer is; `grad_norm` then holds the norm of the last step's."""
         self.S = int(steps_per_graph)
+        self.max_grad_norm, self.grad_norm = max_grad_norm, None
+        self._clip_scale = optimizer.grad_scale
         self._phase = 0
         if self.S not in (1, 2, 4, 8) or (self.S > 1 and sync is not None):
             # (a power of two: Adam's device table of 1 024 steps' scalars is rewritten in front of a launch, never inside a graph)
@@ -86,6 +93,7 @@ class CapturedTrainStep:
                 if sync is not None and with_exchange:
                     sync()
                 if sync is None or with_exchange:
+                    self._clip()
                     optimizer.apply()
                 Graph.free_graph()
         except BaseException:
@@ -99,11 +107,18 @@ class CapturedTrainStep:
         self.feeds, mod.capture_feeds = mod.capture_feeds, None
         self.loss, self.outputs = loss, outputs
         self.grads = [p.grad for p in optimizer.params]     # the buffers backward writes on a replay
-        self.graph = mod.capture_end(keep=(loss, outputs, self._inputs, self._targets, self.grads, self.feeds))
+        self.graph = mod.capture_end(keep=(loss, outputs, self._inputs, self._targets, self.grads, self.feeds, self.grad_norm))
         # the capture only recorded the step: nothing ran, the optimizer's step count is unchanged
+
+    def _clip(self):
+        if self.max_grad_norm is not None:
+            self.grad_norm = clip_grad_norm_(self.optimizer.params, self.max_grad_norm, grad_scale=self._clip_scale)
 
     def replay(self):
         opt = self.optimizer
+        if self.max_grad_norm is not None and opt.grad_scale != self._clip_scale:
+            raise RuntimeError("CapturedTrainStep: optimizer.grad_scale changed after the step was captured, and the captured "
+                               "clipping uses it: capture the step again")
         if self.S > 1:
             # one step per call: the graph of S steps goes out on the first call of every S
             self._phase = (self._phase + 1) % self.S
@@ -126,6 +141,7 @@ class CapturedTrainStep:
             for p, g in zip(opt.params, self.grads):
                 p.grad = g
             self.sync()
+            self._clip()
             opt.apply()
         else:
             opt.note_replayed_apply()               # the captured apply() moved the device's scalar table on
@@ -153,7 +169,8 @@ class OverlappedCapturedTrainStep:
     No collective is inside a graph.  `late_bucket` / `early_bucket` are GradientBuckets over the two
     halves of optimizer.params (workloads.late_and_early_parameters)."""
 
-    def __init__(self, model, criterion, optimizer, inputs, targets, late_bucket, early_bucket):
+    def __init__(self, model, criterion, optimizer, inputs, targets, late_bucket, early_bucket, max_grad_norm=None):
+        self.max_grad_norm = max_grad_norm          # None, or the largest common norm of a step's gradients (optim.clip_grad_norm_)
         mod = inputs.device.mod
         if not (getattr(mod, "fused", False) and hasattr(mod, "capture_begin")):
             raise RuntimeError("OverlappedCapturedTrainStep needs the hip device")
@@ -207,6 +224,8 @@ class OverlappedCapturedTrainStep:
             p.grad = g
         self.early.sync(overlap=True)
         self.late.comm.wait()
+        if self.max_grad_norm is not None:
+            clip_grad_norm_(opt.params, self.max_grad_norm, grad_scale=opt.grad_scale)
         opt.apply()
         opt.t += 1
         return self.loss

@@ -34,7 +34,7 @@ from .data_pipeline import DeviceBatchPipeline, _Window
 
 class EpochTrainer:
     def __init__(self, model, criterion, optimizer, device, num_classes=10, eps=0.05, augment=True, capture=True,
-                 tail="eager", sync=None, max_losses=4096):
+                 tail="eager", sync=None, max_losses=4096, max_grad_norm=None):
         mod = device.mod
         if not (getattr(mod, "fused", False) and hasattr(mod, "upload_async")):
             raise RuntimeError("EpochTrainer needs the hip device")
@@ -42,6 +42,7 @@ class EpochTrainer:
             raise ValueError("tail is 'eager' or 'capture'")
         self.model, self.criterion, self.optimizer, self.device, self.mod = model, criterion, optimizer, device, mod
         self.K, self.eps, self.augment, self.capture, self.tail, self.sync = int(num_classes), eps, augment, capture, tail, sync
+        self.max_grad_norm = max_grad_norm        # None, or the largest norm of a step's gradients (optim.clip_grad_norm_)
         self._slots = {}             # batch shape -> (pipeline, x tensor, y tensor)
         self._captured = {}          # batch shape -> CapturedTrainStep
         self._losses = mod.Array(int(max_losses))
@@ -67,9 +68,10 @@ class EpochTrainer:
                 # (a capture records the step without running it and draws no host random numbers: Dropout masks
                 # are graph inputs that every replay draws, nn/modules/dropout.py)
                 cs = self._captured[shape] = CapturedTrainStep(self.model, self.criterion, self.optimizer, xt, yt,
-                                                               sync=self.sync)
+                                                               sync=self.sync, max_grad_norm=self.max_grad_norm)
             return cs.replay()
-        loss, _ = workloads.train_step(self.model, self.criterion, self.optimizer, xt, yt, sync=self.sync)
+        loss, _ = workloads.train_step(self.model, self.criterion, self.optimizer, xt, yt, sync=self.sync,
+                                       max_grad_norm=self.max_grad_norm)
         Graph.free_graph()
         return loss
 

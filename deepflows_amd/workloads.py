@@ -23,6 +23,7 @@ trained and all-reduced.
 import numpy as np
 
 from . import nn, tensor
+from .optim import clip_grad_norm_
 from .tensor import Graph, Tensor, realize
 
 
@@ -414,14 +415,16 @@ def smooth_one_hot(labels, num_classes=10, eps=0.0):
     return y.astype(np.float32)
 
 
-def train_step(model, criterion, optimizer, inputs, targets, sync=None):
-    """One batch: forward, loss, zero_grad, backward, (gradient all-reduce), optimizer step."""
+def train_step(model, criterion, optimizer, inputs, targets, sync=None, max_grad_norm=None):
+    """One batch: forward, loss, zero_grad, backward, (gradient all-reduce), (clipping), optimizer step."""
     outputs = model(inputs)
     loss = criterion(outputs, targets)
     optimizer.zero_grad()
     loss.backward()
     if sync is not None:
         sync()
+    if max_grad_norm is not None:
+        clip_grad_norm_(optimizer.params, max_grad_norm, grad_scale=optimizer.grad_scale)
     optimizer.step()
     return loss, outputs
 

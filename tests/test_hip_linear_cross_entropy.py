@@ -240,9 +240,23 @@ def test_evaluation_and_training_agree(hip_device):
     Graph.free_graph_all()
 
 
-def test_several_pieces_of_rows(hip_device):
-    """more rows x classes than one piece holds (512 MB of logits): 140 M of them"""
+def test_many_classes_in_a_ragged_last_tile(hip_device):
+    """a class count whose last tiles are ragged, in 140 M logits"""
     _check(hip_device, *_data(1400, 20, 100003, 18, ignored=0.1), label_smoothing=0.1)
+
+
+def test_more_rows_than_one_piece_of_logits_holds(hip_device):
+    """600 M logits are two pieces (of at most 2 GiB each): the second one adds to the first one's dW and db.  The rows are 60
+    different ones, 100 times each in any order, so that the 60 rows' loss, dW and db are theirs too, and dx a hundredth.  dW's
+    bound grows with the root of the rows (10 times), db's N / 64 + 30 and the loss's N / 256 + 12 by less (4 and 3 times)."""
+    x, w, b, t = _data(60, 20, 100003, 22, ignored=0.1)
+    order = np.random.default_rng(23).permutation(np.repeat(np.arange(60), 100))
+    got = _run(hip_device, x[order], w, b, t[order], label_smoothing=0.1)
+    (loss, tloss), (dx, tdx), (dw, tdw), (db, tdb) = _reference(x, w, b, t, e=0.1)
+    _within(got[0], loss, 3 * tloss, "loss")
+    _within(got[1], dx[order] / 100, tdx[order] / 100 + 4 * U * np.abs(dx[order]) / 100, "dx")
+    _within(got[2], dw, 10 * tdw, "dw")
+    _within(got[3], db, 4 * tdb, "db")
 
 
 def test_no_rows(hip_device):

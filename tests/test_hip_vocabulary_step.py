@@ -1,0 +1,205 @@
+"""GPU: the norm, the vocabulary loss and the clipping as they are used together: a residual network whose last norm feeds a head
+with many classes, its gradients clipped, its parameters updated -- eagerly, captured, through the epoch loop.
+
+Against the oracle (the same step in 64 bits, torch on the CPU): 1e-4 relative of the largest value, the framework's bound for
+whole steps; captured steps against eager ones: bit for bit."""
+import numpy as np
+import pytest
+
+from conftest import assert_close
+
+pytestmark = pytest.mark.gpu
+
+V, D, K = 1503, 72, 40
+
+
+def _build(dev, seed=3):
+    from deepflows_amd import nn
+
+    class Network(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.fc0, self.fc1 = nn.Linear(K, D, device=dev), nn.Linear(D, D, device=dev)
+            self.norm0, self.norm1 = nn.RMSNorm(D, device=dev), nn.RMSNorm(D, device=dev)
+
+        def forward(self, x):
+            h = self.fc0(x)
+            y = nn.functional.relu(self.fc1(self.norm0(h)))
+            return self.norm1(y, h)[0]
+
+    np.random.seed(seed)
+    net = Network()
+    head = nn.Linear(D, V, device=dev)
+    return net, nn.LinearCrossEntropyLoss(head, label_smoothing=0.1), list(net.parameters()) + list(head.parameters())
+
+
+def _batches(n, rows):
+    rng = np.random.default_rng(11)
+    out = []
+    for _ in range(n):
+        t = rng.integers(0, V, rows).astype(np.float32)
+        t[rng.random(rows) < 0.2] = -100
+        out.append((rng.standard_normal((rows, K)).astype(np.float32), t))
+    return out
+
+
+def _oracle(arrays, batches, max_norm, lr):
+    """the same steps in 64 bits: (losses, norms, parameters)"""
+    import torch
+    ps = [torch.tensor(a, dtype=torch.float64, requires_grad=True) for a in arrays]
+    w0, b0, w1, b1, g0, g1, wh, bh = ps
+    norm = lambda h, g: h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6) * g
+    losses, norms = [], []
+    for x, t in batches:
+        x, t = torch.tensor(x, dtype=torch.float64), torch.tensor(t).long()
+        h = x @ w0 + b0
+        y = norm(torch.relu(norm(h, g0) @ w1 + b1) + h, g1)
+        loss = torch.nn.functional.cross_entropy(y @ wh + bh, t, ignore_index=-100, label_smoothing=0.1)
+        grads = torch.autograd.grad(loss, ps)
+        total = torch.sqrt(sum((g * g).sum() for g in grads)).item()
+        scale = min(1.0, max_norm / (total + 1e-6))
+        with torch.no_grad():
+            for p, g in zip(ps, grads):
+                p -= lr * scale * g
+        losses.append(loss.item())
+        norms.append(total)
+    return losses, norms, [p.detach().numpy() for p in ps]
+
+
+def test_steps_against_the_oracle(hip_device):
+    from deepflows_amd import optim
+    from deepflows_amd.tensor import Graph, Tensor
+    net, crit, params = _build(hip_device)
+    opt = optim.SGD(params, lr=0.5)
+    named = [net.fc0.weight, net.fc0.bias, net.fc1.weight, net.fc1.bias, net.norm0.weight, net.norm1.weight,
+             crit.linear.weight, crit.linear.bias]
+    batches = _batches(3, 50)
+    want = _oracle([p.numpy() for p in named], batches, 0.2, 0.5)
+    losses, norms = [], []
+    for x, t in batches:
+        loss = crit(net(Tensor(x, device=hip_device)), Tensor(t, device=hip_device))
+        opt.zero_grad()
+        loss.backward()
+        norms.append(float(optim.clip_grad_norm_(opt.params, 0.2).numpy()[0]))
+        opt.step()
+        losses.append(float(loss.numpy()[0]))
+        Graph.free_graph()
+    assert min(want[1]) > 0.2                                  # (the clipping does something)
+    assert_close(losses, want[0], 1e-4, "losses")
+    assert_close(norms, want[1], 1e-4, "norms")
+    for p, w in zip(named, want[2]):
+        assert_close(p.numpy(), w, 1e-4, "parameter")
+
+
+@pytest.mark.parametrize("kind", ["SGD", "Adam"])
+@pytest.mark.parametrize("steps_per_graph", [1, 2])
+def test_captured_steps_equal_eager_ones(hip_device, kind, steps_per_graph):
+    from deepflows_amd import optim, workloads
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+    batches = _batches(4, 37)
+    make = (lambda p: optim.SGD(p, lr=0.3, momentum=0.9)) if kind == "SGD" else (lambda p: optim.Adam(p, lr=1e-2))
+
+    net, crit, params = _build(hip_device)
+    opt = make(params)
+    want = []
+    for x, t in batches:
+        loss, _ = workloads.train_step(net, crit, opt, Tensor(x, device=hip_device), Tensor(t, device=hip_device), max_grad_norm=0.3)
+        want.append(float(loss.numpy()[0]))
+        Graph.free_graph()
+    want_params = [p.numpy().copy() for p in params]
+    Graph.free_graph_all()
+
+    net, crit, params = _build(hip_device)
+    opt = make(params)
+    xs = [Tensor(batches[0][0], device=hip_device) for _ in range(steps_per_graph)]
+    ts = [Tensor(batches[0][1], device=hip_device) for _ in range(steps_per_graph)]
+    step = CapturedTrainStep(net, crit, opt, xs if steps_per_graph > 1 else xs[0], ts if steps_per_graph > 1 else ts[0],
+                             steps_per_graph=steps_per_graph, max_grad_norm=0.3)
+    got = []
+    for k, (x, t) in enumerate(batches):
+        if k % steps_per_graph == 0:
+            for j in range(steps_per_graph):
+                hip_device.mod.from_numpy(batches[k + j][0], xs[j].data._handle)
+                hip_device.mod.from_numpy(batches[k + j][1], ts[j].data._handle)
+        got.append(float(step.replay().numpy()[0]))
+    last = slice(steps_per_graph - 1, None, steps_per_graph)    # (the loss of a graph's last step is what a replay shows)
+    assert got[last] == want[last]
+    assert float(step.grad_norm.numpy()[0]) > 0.0
+    for p, w in zip(params, want_params):
+        assert np.array_equal(p.numpy(), w)
+    step.destroy()
+    Graph.free_graph_all()
+
+
+def test_a_changed_gradient_factor_is_refused(hip_device):
+    from deepflows_amd import optim
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+    net, crit, params = _build(hip_device)
+    opt = optim.SGD(params, lr=0.1)
+    x, t = _batches(1, 8)[0]
+    step = CapturedTrainStep(net, crit, opt, Tensor(x, device=hip_device), Tensor(t, device=hip_device), max_grad_norm=1.0)
+    step.replay()
+    opt.grad_scale = 0.5
+    with pytest.raises(RuntimeError):
+        step.replay()
+    step.destroy()
+    Graph.free_graph_all()
+
+
+def test_gradient_bucket_clipping_and_the_optimizers_factor(hip_device):
+    """gradients that live in a data-parallel bucket (its slices begin at any element), summed over two ranks' worth by hand"""
+    from deepflows_amd import optim, parallel
+    from deepflows_amd.tensor import Graph, Tensor
+
+    class TwoTimes(parallel.Communicator):
+        exchanges, world = True, 2
+
+        def allreduce_sum(self, flat, overlap=False):
+            flat.device.mod.axpy(flat._handle, (flat * 1.0)._handle, 1.0)
+            return flat
+
+    net, crit, params = _build(hip_device)
+    x, t = _batches(1, 20)[0]
+    xt, tt = Tensor(x, device=hip_device), Tensor(t, device=hip_device)
+    crit(net(xt), tt).backward()
+    plain = np.concatenate([p.grad.numpy().reshape(-1) for p in params]).astype(np.float64)
+    Graph.free_graph()
+    for p in params:
+        p.grad = None
+    bucket = parallel.GradientBucket(params, TwoTimes())
+    crit(net(xt), tt).backward()
+    bucket.sync()
+    total = float(optim.clip_grad_norm_(params, 0.1, grad_scale=0.5).numpy()[0])
+    want = np.sqrt((plain ** 2).sum())
+    assert abs(total - want) <= 1e-6 * want
+    got = np.concatenate([p.grad.numpy().reshape(-1) for p in params])
+    assert_close(got, 2 * plain * min(1.0, 0.1 / (want + 1e-6)), 1e-6)
+    bucket.release()
+    Graph.free_graph_all()
+
+
+def test_the_epoch_loop_clips(hip_device):
+    """full batches through the captured step and a ragged one eagerly: the parameters of the plain loop, bit for bit"""
+    from deepflows_amd import nn, optim, workloads
+    from deepflows_amd.tensor import Graph
+    from deepflows_amd.utils.data import data_loader
+    from deepflows_amd.utils.train_loop import EpochTrainer
+    rng = np.random.default_rng(5)
+    x = (rng.standard_normal((40, 3, 32, 32)) * 0.8).astype(np.float32)
+    y = rng.integers(0, 10, 40)
+    finals = []
+    for capture in (True, False):
+        np.random.seed(3)
+        model = workloads.ResNet18(10, device=hip_device, register_blocks=True)
+        opt = optim.Adam(model.parameters(), lr=1e-3)
+        trainer = EpochTrainer(model, nn.CrossEntropyLoss(), opt, hip_device, capture=capture, max_grad_norm=0.05)
+        np.random.seed(9)
+        losses = trainer.run_epoch(data_loader(x, y, 16, shuffle=True), 0, 2)
+        finals.append((losses, [p.numpy().copy() for p in opt.params]))
+        trainer.destroy()
+        Graph.free_graph_all()
+    assert np.array_equal(finals[0][0], finals[1][0])
+    for a, b in zip(finals[0][1], finals[1][1]):
+        assert np.array_equal(a, b)

@@ -111,3 +111,83 @@ def test_linear_cross_entropy_refusals(cpu_oracle):
                      ((x, w, b, Tensor(np.full(4, 0.5), device=cpu_oracle)), {})]:
         with pytest.raises(ValueError):
             F.linear_cross_entropy(*args, **kw)
+
+
+def test_a_clipped_training_step_of_two_ranks(cpu_oracle):
+    """the summed gradients of two ranks with grad_scale = 1/2 are clipped as their mean is"""
+    from deepflows_amd import nn, optim, workloads
+    from deepflows_amd.tensor import Tensor
+    rng = np.random.default_rng(3)
+    x, y = rng.standard_normal((5, 12)).astype(np.float32), np.eye(4, dtype=np.float32)[rng.integers(0, 4, 5)]
+    finals = []
+    for double in (False, True):
+        np.random.seed(1)
+        model = workloads.MLP((12, 16, 4), device=cpu_oracle)
+        opt = optim.SGD(model.parameters(), lr=0.5)
+
+        def sync():
+            if double:
+                opt.grad_scale = 0.5
+                for p in opt.params:
+                    p.grad = p.grad * 2.0
+
+        workloads.train_step(model, nn.CrossEntropyLoss(), opt, Tensor(x, device=cpu_oracle), Tensor(y, device=cpu_oracle),
+                             sync=sync, max_grad_norm=0.01)
+        finals.append([p.numpy() for p in opt.params])
+    for a, b in zip(*finals):
+        assert_close(a, b, 1e-6)
+
+
+def test_two_gloo_ranks_clip_the_mean_of_their_gradients(tmp_path):
+    """three steps through the gradient bucket, whose slices the clipped windows replace: the ranks agree bit for bit, and with one
+    process that clips the averaged gradients itself"""
+    import json
+    import os
+    import subprocess
+    import sys
+
+    import test_data_parallel as dp
+    from conftest import ROOT
+    adam, plain = "optim.Adam(model.parameters(), lr=1e-2, weight_decay=5e-4)", "sync=bucket.sync if world > 1 else None"
+    assert adam in dp.WORKER and plain in dp.WORKER
+    script = tmp_path / "worker.py"
+    script.write_text(dp.WORKER.replace(adam, "optim.SGD(model.parameters(), lr=0.5)").replace(plain, plain + ", max_grad_norm=0.1"))
+    env = dict(os.environ, DF_ROOT=ROOT, DF_OUT=str(tmp_path), MASTER_ADDR="127.0.0.1")
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1",
+                        "--master-port", str(31500 + os.getpid() % 2000), str(script)], env=env, capture_output=True, text=True,
+                       timeout=600)
+    assert r.returncode == 0, r.stderr[-3000:]
+    outs = [json.load(open(tmp_path / f"rank{k}.json")) for k in range(2)]
+    for a, b in zip(outs[0]["params"], outs[1]["params"]):
+        assert np.array_equal(np.array(a), np.array(b))
+
+    from deepflows_amd import backend_api, nn, workloads
+    from deepflows_amd.tensor import Graph, Tensor
+    from oracle.numpy_device import NumpyDevice
+    dev = backend_api.register_device("cpu", NumpyDevice())
+    try:
+        np.random.seed(0)
+        model = workloads.MLP((12, 16, 4), device=dev)
+        params = [p.numpy().astype(np.float64) for p in model.parameters()]
+        rngs, clipped = [np.random.default_rng(100 + r) for r in range(2)], 0
+        for _ in range(3):
+            mean = 0.0
+            for rng in rngs:
+                x = rng.standard_normal((8, 12)).astype(np.float32)
+                y = np.eye(4, dtype=np.float32)[rng.integers(0, 4, 8)]
+                for p, a in zip(model.parameters(), params):
+                    p.data, p.grad = Tensor(a.astype(np.float32), device=dev).data, None
+                nn.CrossEntropyLoss()(model(Tensor(x, device=dev)), Tensor(y, device=dev)).backward()
+                mean = mean + 0.5 * np.concatenate([p.grad.numpy().reshape(-1) for p in model.parameters()]).astype(np.float64)
+                Graph.free_graph()
+            norm = np.sqrt((mean ** 2).sum())
+            clipped += norm > 0.1
+            mean, at = mean * min(1.0, 0.1 / (norm + 1e-6)), 0
+            for k, a in enumerate(params):
+                params[k] = a - 0.5 * mean[at:at + a.size].reshape(a.shape)
+                at += a.size
+        assert clipped == 3
+        for a, want in zip(outs[0]["params"], params):
+            assert_close(np.array(a), want, 1e-5)
+    finally:
+        backend_api.unregister_device("cpu")
