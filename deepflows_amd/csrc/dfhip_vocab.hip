@@ -10,7 +10,7 @@
 //
 // The three products run on the fp16 matrix cores with fp32 accuracy (dfhip_splitgemm.h): x and W are converted once a call,
 // dl where it is formed.  The launches of a call:
-//   k_lce_scan     the largest magnitudes of x and W (finite elements only)
+//   k_lce_scan     the largest magnitudes of x (counted rows) and W, finite elements only
 //   k_lce_split    x, W -> split arrays; the number of counted rows
 //   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> k_lce_pair: the dx
 //                  product and the dW product (db on the side: the column sums of its second operand); with the last piece, the loss
@@ -62,41 +62,70 @@ __device__ __forceinline__ float finite_abs(float v) {
   return a <= 3.4028235e38f ? a : 0.0f;                    // (inf and NaN: 0)
 }
 
-// workgroups 0 .. kScan-1: x, kScan .. 2 kScan - 1: W
-__global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__ x, int64_t nx, const float* __restrict__ w,
-                                                       int64_t nw, Ctl* __restrict__ ctl) {
+__device__ __forceinline__ float finite_abs(const float4& v) {
+  return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+}
+
+// workgroups 0 .. kScan-1: x, kScan .. 2 kScan - 1: W.  The rows of x that are not counted are passed over: padding may hold
+// anything, and a large value in it would cost the counted rows their low bits.
+__global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__ x, int64_t rows, int64_t width,
+                                                       const float* __restrict__ target, float ignore,
+                                                       const float* __restrict__ w, int64_t nw, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
   const bool second = blockIdx.x >= kScan;
-  const float* p = second ? w : x;
-  const int64_t n = second ? nw : nx;
   const int blk = (int)blockIdx.x & (kScan - 1);
   float m = 0.0f;
-  int64_t lo = 0;
-  if ((((uintptr_t)p) & 15) == 0) {
-    const float4* p4 = reinterpret_cast<const float4*>(p);
-    const int64_t n4 = n >> 2, step = (int64_t)kScan * kThreads;
-    int64_t i = (int64_t)blk * kThreads + threadIdx.x;
-    for (; i + 3 * step < n4; i += 4 * step) {
-      float4 v[4];
+  if (!second) {                                           // a wave takes up to 1 024 elements of one row at a time
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t segs = (width + 1023) >> 10;
+    const bool vec = (width & 3) == 0 && (((uintptr_t)x) & 15) == 0;
+    for (int64_t it = (int64_t)blk * (kThreads / 64) + wave; it < rows * segs; it += kScan * (kThreads / 64)) {
+      const int64_t r = segs == 1 ? it : it / segs;
+      const int c0 = (int)(it - r * segs) << 10, n = (int)min(width - c0, (int64_t)1024);
+      const float* p = x + r * width + c0;
+      const float t = target[r];
+      float s = 0.0f;
+      if (vec) {
+        float4 v[4];
 #pragma unroll
-      for (int u = 0; u < 4; u++) v[u] = p4[i + u * step];
+        for (int u = 0; u < 4; u++) {
+          const int c = u * 256 + lane * 4;
+          v[u] = c < n ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll
-      for (int u = 0; u < 4; u++)
-        m = fmaxf(fmaxf(m, fmaxf(finite_abs(v[u].x), finite_abs(v[u].y))), fmaxf(finite_abs(v[u].z), finite_abs(v[u].w)));
+        for (int u = 0; u < 4; u++) s = fmaxf(s, finite_abs(v[u]));
+      } else {
+#pragma unroll 4
+        for (int c = lane; c < n; c += 64) s = fmaxf(s, finite_abs(p[c]));
+      }
+      m = t == ignore ? m : fmaxf(m, s);
     }
-    for (; i < n4; i += step) {
-      const float4 v = p4[i];
-      m = fmaxf(fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y))), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+  } else {
+    int64_t lo = 0;
+    if ((((uintptr_t)w) & 15) == 0) {
+      const float4* p4 = reinterpret_cast<const float4*>(w);
+      const int64_t n4 = nw >> 2, step = (int64_t)kScan * kThreads;
+      int64_t i = (int64_t)blk * kThreads + threadIdx.x;
+      for (; i + 3 * step < n4; i += 4 * step) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = p4[i + u * step];
+#pragma unroll
+        for (int u = 0; u < 4; u++) m = fmaxf(m, finite_abs(v[u]));
+      }
+      for (; i < n4; i += step) m = fmaxf(m, finite_abs(p4[i]));
+      lo = n4 << 2;
     }
-    lo = n4 << 2;
+    for (int64_t i = lo + (int64_t)blk * kThreads + threadIdx.x; i < nw; i += (int64_t)kScan * kThreads)
+      m = fmaxf(m, finite_abs(w[i]));
   }
-  for (int64_t i = lo + (int64_t)blk * kThreads + threadIdx.x; i < n; i += (int64_t)kScan * kThreads) m = fmaxf(m, finite_abs(p[i]));
   m = block_reduce<kThreads>(m, sh, Max());
   if (threadIdx.x == 0) (second ? ctl->max_w : ctl->max_x)[blk] = m;
 }
 
-// workgroups [0, bx): x, [bx, bx + bw): W, the last one: the counted rows.  A wave takes 512 consecutive cells of the padded
-// array at a time, eight a lane; where rows do not begin on 16 bytes it reads them lane by lane and turns them in LDS.
+// workgroups [0, bx): x (zeros for the rows that are not counted), [bx, bx + bw): W, the last one: the number of counted rows.  A
+// wave takes 512 consecutive cells of the padded array at a time, eight a lane; where rows do not begin on 16 bytes it reads them
+// lane by lane and turns them in LDS.
 __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict__ x, int64_t rows, int64_t width,
                                                         const float* __restrict__ w, int64_t classes, char* __restrict__ xs,
                                                         char* __restrict__ ws, const float* __restrict__ target, float ignore,
@@ -106,6 +135,7 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   __shared__ __attribute__((aligned(16))) float turn[kThreads / 64][512];
   if (blockIdx.x == bx + bw) {
     int n = 0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < rows; i += kThreads) n += target[i] != ignore ? 1 : 0;
     n = block_reduce<kThreads>(n, shi, Add());
     if (threadIdx.x == 0) ctl->scale = mean ? 1.0f / (float)max(n, 1) : 1.0f;
@@ -153,11 +183,12 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
 #pragma unroll
       for (int k = 0; k < 8; k++) v[k] = turn[wave][lane * 8 + k];
     }
+    const bool out = !second && r < nr && target[r] == ignore;
     half8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       _Float16 h, l;
-      split(ldexpf(v[k], -e), h, l);
+      split(out ? 0.0f : ldexpf(v[k], -e), h, l);
       hi[k] = h; lo[k] = l;
     }
     char* d = dst + r * pc * 4 + (c >> 5) * 128 + (c & 31) * 2;
@@ -499,7 +530,8 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   ProfScope prof("linear_ce", (grads ? 6.0 : 2.0) * (double)rows * (double)width * (double)classes,
                  4.0 * (grads ? 2.0 : 1.0) * ((double)rows * width + (double)width * classes));
 
-  DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows * width, w, width * classes, ctl);
+  DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows, width, target, ignore, w,
+            width * classes, ctl);
   DF_LAUNCH_CHECK();
   const int64_t bx = std::min<int64_t>(np * dp / 2048, 2048), bw = std::min<int64_t>(dp * vp / 2048, 4096);
   DF_LAUNCH(k_lce_split, dim3((unsigned)(bx + bw + 1)), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p,

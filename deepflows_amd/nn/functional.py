@@ -490,8 +490,7 @@ def rms_norm(input: Tensor, weight=None, eps: float = 1e-6, residual=None):
 
     With `residual` (a tensor of input's shape) the sum h = input + residual is normalised and (y, h) come back: h is what the
     next residual sum starts from.  weight: None or a tensor with as many elements as the last axis.  Zero rows are allowed."""
-    input = realize(input)
-    residual = realize(residual) if residual is not None else None
+    input, weight, residual = realize(input), realize(weight), realize(residual)
     x, device = input.data, input.data._device
     shape = tuple(x.shape)
     if not shape or shape[-1] < 1:
@@ -635,16 +634,33 @@ class _LinearCrossEntropyFused(_FusedNode):
         return out
 
 
+class _CountedRows(tensor.UnaryOperator):
+    """the rows of x that `keep` (rows, 1) marks, zeros in place of the others whatever they hold"""
+
+    def __init__(self, x, keep):
+        self.keep = keep
+        super().__init__(x)
+
+    def forward(self, x):
+        return self._masked(x.data)
+
+    def grad_fn(self, x, grad):
+        return self._masked(grad)
+
+    def _masked(self, a):
+        return backend_api.Btensor(np.where(self.keep, a.numpy(), np.float32(0.0)), device=a.device)
+
+
 def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, reduction: str = 'mean',
                          ignore_index: int = -100, label_smoothing: float = 0.0):
     """cross_entropy(linear(input, weight, bias), target) for many classes: the logits are never kept.
 
     input (N, D), weight (D, V), bias None or V elements, target (N,): class indices as whole numbers (fp32, the device's only
     type, holds them exactly up to 2^24 classes).  Rows whose target is `ignore_index` are not counted; 'mean' divides by the
-    number of counted rows, and a batch without one has loss 0 and zero gradients.  label_smoothing e: the target distribution is
-    (1 - e) onehot + e / V.  On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it
+    number of counted rows, and a batch without one has loss 0 and zero gradients.  What stands in a row of input that is not
+    counted does not matter, NaN and infinities included.  label_smoothing e: the target distribution is (1 - e) onehot + e / V.  On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it
     in time to raise would stall the device); elsewhere it raises ValueError."""
-    input = realize(input)
+    input, weight, bias = realize(input), realize(weight), realize(bias)
     xs, ws, device = tuple(input.shape), tuple(weight.shape), input.device
     if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[0]:
         raise ValueError(f"linear_cross_entropy: input {xs} and weight {ws} do not match")
@@ -676,6 +692,8 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     counted = t != ignore_index
     if np.any(counted & ~((t >= 0) & (t < classes) & (t == np.floor(t)))):
         raise ValueError(f"linear_cross_entropy: a target is neither a class index below {classes} nor {ignore_index}")
+    if not counted.all():
+        input = _CountedRows(input, counted[:, None])
     q = np.zeros((rows, classes), dtype=np.float32)
     q[counted] = label_smoothing / classes
     q[np.nonzero(counted)[0], t[counted].astype(np.int64)] += 1.0 - label_smoothing

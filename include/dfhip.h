@@ -501,7 +501,7 @@ int dfhip_mlp2_ce_backward(const float* x, const float* h, const float* dz1, con
  *     loss (1) = sum of the row losses of the counted rows, divided by their number (at least 1) when mean != 0
  * and, for an upstream gradient of 1, dx (rows, width), dw (width, classes), db (classes); each may be NULL.
  * target (rows): class indices as whole numbers in fp32; rows with target == ignore_index are not counted: no loss, zeros in dx,
- * nothing added to dw and db.  A target that is neither ignore_index nor a whole number in [0, classes) makes the loss and the
+ * nothing added to dw and db, whatever their elements are (NaN too).  A target that is neither ignore_index nor a whole number in [0, classes) makes the loss and the
  * gradients it reaches NaN.  At most 2^24 classes.  Without counted rows the loss and the gradients are 0.
  * Scratch memory comes from the pool and does not grow with rows x classes.  No output may overlap an input. */
 int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, const float* target, float* loss, float* dx,

@@ -147,6 +147,20 @@ def test_rows_that_are_not_counted_leave_their_inputs_alone(hip_device):
         _within(g, want, 4 * tol, "gradient")
 
 
+@pytest.mark.parametrize("D", [32, 37, 2100])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38, -1e30])
+def test_padding_may_hold_anything(hip_device, D, bad):
+    """values that are not finite, or so large that the counted rows would vanish beside them, in rows that are not counted"""
+    x, w, b, t = _data(70, D, 200, 24, ignored=0.4)
+    clean = _run(hip_device, np.where(t[:, None] == -100, np.float32(0), x), w, b, t)
+    y = x.copy()
+    y[t == -100] = bad
+    for a, c in zip(_run(hip_device, y, w, b, t), clean):
+        assert np.array_equal(a, c)
+    ref = _reference(np.where(t[:, None] == -100, np.float32(0), x), w, b, t)
+    _within(clean[0], ref[0][0], ref[0][1], "loss")
+
+
 def test_bad_targets_show(hip_device):
     x, w, b, t = _data(40, 24, 100, 10)
     for bad in (100.0, -1.0, 2.5, np.nan, np.inf, 1e9):

@@ -203,3 +203,40 @@ def test_the_epoch_loop_clips(hip_device):
     assert np.array_equal(finals[0][0], finals[1][0])
     for a, b in zip(finals[0][1], finals[1][1]):
         assert np.array_equal(a, b)
+
+
+def test_the_overlapped_exchange_clips(hip_device):
+    """both halves of the gradients on their way when the clipping begins: the eager step's parameters, bit for bit.  (One rank
+    without a collective: what is checked is that the clipping sees the gradients of both graphs.)"""
+    from deepflows_amd import nn, optim, parallel, workloads
+    from deepflows_amd.graph_step import OverlappedCapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+
+    class Alone(parallel.Communicator):
+        exchanges = True
+
+        def allreduce_sum(self, flat, overlap=False):
+            return flat
+
+    rng = np.random.default_rng(3)
+    xs = Tensor(rng.standard_normal((32, 3, 32, 32)).astype(np.float32), device=hip_device)
+    ys = Tensor(np.eye(10, dtype=np.float32)[rng.integers(0, 10, 32)], device=hip_device)
+    crit, comm, runs = nn.CrossEntropyLoss(), Alone(), []
+    for overlapped in (False, True):
+        np.random.seed(1)
+        m = workloads.ResNet18(device=hip_device, register_blocks=True)
+        o = optim.Adam(workloads.all_block_parameters(m), lr=1e-3)
+        bucket = parallel.GradientBucket(o.params, comm)
+        for _ in range(1 if overlapped else 4):
+            workloads.train_step(m, crit, o, xs, ys, sync=bucket.sync, max_grad_norm=0.1)
+            Graph.free_graph()
+        if overlapped:
+            late, early = workloads.late_and_early_parameters(m, o.params)
+            step = OverlappedCapturedTrainStep(m, crit, o, xs, ys, parallel.GradientBucket(late, comm),
+                                               parallel.GradientBucket(early, comm), max_grad_norm=0.1)
+            for _ in range(3):
+                step.replay()
+        runs.append([p.numpy().copy() for p in o.params])
+        Graph.free_graph_all()
+    for a, b in zip(*runs):
+        assert np.array_equal(a, b)

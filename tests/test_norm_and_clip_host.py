@@ -113,6 +113,25 @@ def test_linear_cross_entropy_refusals(cpu_oracle):
             F.linear_cross_entropy(*args, **kw)
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38])
+def test_rows_that_are_not_counted_may_hold_anything(cpu_oracle, bad):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    rng = np.random.default_rng(4)
+    x, w = rng.standard_normal((5, 6)).astype(np.float32), rng.standard_normal((6, 9)).astype(np.float32)
+    t = np.array([3, -100, 8, -100, 0], np.float32)
+    results = []
+    for fill in (0.0, bad):
+        y = np.where(t[:, None] == -100, np.float32(fill), x)
+        ts = [Tensor(a, device=cpu_oracle, requires_grad=True) for a in (y, w)]
+        loss = F.linear_cross_entropy(*ts, None, Tensor(t, device=cpu_oracle))
+        loss.backward()
+        results.append([loss.numpy()] + [p.grad.numpy() for p in ts])
+    for a, b in zip(*results):
+        assert np.all(np.isfinite(a)) and np.array_equal(a, b)
+    assert not results[1][1][t == -100].any()
+
+
 def test_a_clipped_training_step_of_two_ranks(cpu_oracle):
     """the summed gradients of two ranks with grad_scale = 1/2 are clipped as their mean is"""
     from deepflows_amd import nn, optim, workloads
