@@ -9,7 +9,8 @@
 // gradient of 1: nothing is computed twice (recomputing the logits in a backward pass would be a third more products).
 //
 // The three products run on the fp16 matrix cores with fp32 accuracy (dfhip_splitgemm.h): x and W are converted once a call,
-// dl where it is formed.  The launches of a call:
+// dl where it is formed; for few rows, where W's bytes are what counts, on the fp32 matrix cores (dfhip_fewrows.h, and further
+// down).  The launches of a call:
 //   k_lce_scan     the largest magnitudes of x (counted rows) and W, finite elements only
 //   k_lce_split    x, W -> split arrays; the number of counted rows
 //   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> k_lce_pair: the dx
@@ -20,6 +21,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "dfhip_fewrows.h"
 #include "dfhip_splitgemm.h"
 
 using namespace dfhip;
@@ -374,6 +376,194 @@ __global__ __launch_bounds__(256) void k_lce_pair_rest(Pair p) {
   else rest_body<T, EPI>(p.b, block - p.a.rest * SLICES);
 }
 
+// ---- few rows: W is read as it is (dfhip_fewrows.h) ----------------------------------------------------------------------------
+//   k_few_logits   logits (rows, ld), and of every column tile the rows' largest logit, sum of exponentials and sum (its own three
+//                  numbers: a row is spread over more workgroups than would wait for each other)
+//   k_few_rows     those joined: row losses; dl (times the mean's factor) over the logits
+//   k_few_pair     the dx product, cut along the classes, and the dW product (db on the side); the loss
+//   k_few_rest     the parts of dx added up
+struct Few {
+  dfhip_few::Product logits, dx;
+  const float* bias;
+  float* l;                                // logits, then dl
+  int64_t ld;                              // a multiple of 128
+  float* stat;                             // three arrays of (rows, tiles): largest, sum of exponentials, sum of l - largest
+  int tiles, cols;                         // their number and width
+  const float* target;
+  float ignore, smooth;
+  float *dw, *db, *parts, *loss;
+  const float* rowloss;
+  const Ctl* ctl;
+  int width, cuts, cut, n_dx;              // dx: `cuts` ranges of `cut` classes, n_dx workgroups
+  int strips, dw_cuts, dw_cut, n_dw;       // dW: strips of few_strip() columns, dw_cuts ranges of dw_cut rows of it
+};
+
+__device__ __forceinline__ float half_max(float v) {       // over 32 lanes
+#pragma unroll
+  for (int off = 16; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  return v;
+}
+__device__ __forceinline__ float half_sum(float v) {
+#pragma unroll
+  for (int off = 16; off; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+template <int RB, int CF, int NW>
+__global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
+  __shared__ dfhip_few::f32x4 lds[dfhip_few::lds_pieces<CF, NW>()];
+  const dfhip_few::Product& p = g.logits;
+  const int tile = (int)blockIdx.x, n0 = tile * 32 * CF, i = threadIdx.x & 31;
+  const int c = n0 + CF * i, over = c - min(c, p.n - CF);  // columns by which this lane's loads were moved back
+  float bias[CF];
+#pragma unroll
+  for (int f = 0; f < CF; f++) bias[f] = g.bias && c + f < p.n ? g.bias[c + f] : 0.0f;
+  dfhip_few::across<RB, CF, NW>(p, n0, lds, [&](int row, const float* v) {
+    if (row >= p.rows) return;                             // (uniform in the half wave)
+    float w[CF], m = -INFINITY;                            // -inf behind the last class
+#pragma unroll
+    for (int f = 0; f < CF; f++) {
+      w[f] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < CF; e++) w[f] = f + over == e ? v[e] + bias[f] : w[f];
+      m = fmaxf(m, w[f]);
+    }
+    typedef float vec __attribute__((ext_vector_type(CF)));
+    *reinterpret_cast<vec*>(g.l + (int64_t)row * g.ld + c) = *reinterpret_cast<const vec*>(w);
+    m = half_max(m);
+    const float from = m > -INFINITY ? m : 0.0f;           // (a tile whose classes are all masked: z = 0)
+    float z = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int f = 0; f < CF; f++) {
+      z += exp_of(w[f] - from);
+      t += c + f < p.n ? w[f] - from : 0.0f;
+    }
+    z = half_sum(z);
+    if (g.smooth > 0.0f) t = half_sum(t);
+    if (i == 0) {
+      float* st = g.stat + (int64_t)row * g.tiles + tile;
+      const int64_t n = (int64_t)p.rows * g.tiles;
+      st[0] = m;
+      st[n] = z;
+      st[2 * n] = t;
+    }
+  });
+}
+
+// `chunks` workgroups a row, each of which joins the row's tiles for itself; the one that holds the target's column also makes the
+// row's loss (nobody else touches that column)
+template <bool GRADS>
+__global__ __launch_bounds__(kThreads) void k_few_rows(Few g, int rows, int classes, int mean, int chunk, int chunks,
+                                                       float* __restrict__ rowloss, Ctl* __restrict__ ctl) {
+  __shared__ float sh[kThreads / 64];
+  __shared__ int shi[kThreads / 64];
+  const int row = (int)blockIdx.x / chunks, ch = (int)blockIdx.x % chunks;
+  const float t = g.target[row];
+  float* l = g.l + (int64_t)row * g.ld;
+  const int lo = ch * chunk, hi = min(lo + chunk, (int)g.ld);
+  int n = 0;
+  for (int k = threadIdx.x; k < rows; k += kThreads) n += g.target[k] != g.ignore ? 1 : 0;
+  n = block_reduce<kThreads>(n, shi, Add());
+  const float scale = mean ? 1.0f / (float)max(n, 1) : 1.0f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) ctl->scale = scale;
+  if (t == g.ignore) {
+    if (ch == 0 && threadIdx.x == 0) rowloss[row] = 0.0f;
+    if (GRADS)
+      for (int c = lo + threadIdx.x * 4; c < hi; c += kThreads * 4) *reinterpret_cast<float4*>(l + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    return;
+  }
+  const float *sm = g.stat + (int64_t)row * g.tiles, *sz = sm + (int64_t)rows * g.tiles, *st = sz + (int64_t)rows * g.tiles;
+  const bool ok = t >= 0.0f && t < (float)classes && t == floorf(t);
+  const int ti = ok ? (int)t : 0;
+  const bool owner = ti >= lo && ti < hi;
+  const float lt = owner ? l[ti] : 0.0f;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < g.tiles; k += kThreads) m = fmaxf(m, sm[k]);
+  m = block_reduce<kThreads>(m, sh, Max());
+  float z = 0.0f, s = 0.0f;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < g.tiles; k += kThreads) z += sz[k] * exp_of(sm[k] - m);
+  z = block_reduce<kThreads>(z, sh, Add());
+  if (owner && g.smooth > 0.0f) {
+    for (int k = threadIdx.x; k < g.tiles; k += kThreads)
+      s += sm[k] > -INFINITY ? st[k] + (float)min(g.cols, classes - k * g.cols) * (sm[k] - m) : -INFINITY;
+    s = block_reduce<kThreads>(s, sh, Add());
+  }
+  if (owner && threadIdx.x == 0) {
+    float r = logf(z) - (1.0f - g.smooth) * (lt - m);
+    if (g.smooth > 0.0f) r -= g.smooth * (s / (float)classes);
+    rowloss[row] = ok ? r : NAN;
+  }
+  if (!GRADS) return;
+  const float iz = ok ? scale / z : NAN, q = scale * (g.smooth / (float)classes), p1 = scale * (1.0f - g.smooth);
+  for (int c = lo + threadIdx.x * 4; c < hi; c += kThreads * 4) {
+    const float4 a = *reinterpret_cast<const float4*>(l + c);
+    float v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      v[k] = fmaf(exp_of(v[k] - m), iz, -q);
+      if (c + k == ti) v[k] -= p1;
+      v[k] = c + k < classes ? v[k] : 0.0f;
+    }
+    *reinterpret_cast<float4*>(l + c) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <int KN>
+constexpr int few_strip() { return KN <= 32 ? 512 : 256; }     // columns of dW a workgroup
+template <int KN>
+__global__ __launch_bounds__(kThreads) void k_few_pair(Few g, int rows, int classes) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * 32 * dfhip_few::kPitch];
+  constexpr int CF = few_strip<KN>() / 128;
+  const int lane = threadIdx.x & 63;
+  int block = (int)blockIdx.x;
+  if (block < g.n_dx) {
+    // (consecutive workgroups go to the eight XCDs in turn: the column tiles of one range of classes on one XCD, side by side,
+    // so that dl comes out of its L2)
+    const int tiles = (g.width + 127) >> 7, tile = (block >> 3) % tiles, cut = (block >> 3) / tiles * 8 + (block & 7), k0 = cut * g.cut;
+    if (cut >= g.cuts) return;
+    dfhip_few::along<(KN + 31) / 32>(g.dx, tile * 128, k0, min(k0 + g.cut, classes), lds, g.parts + (int64_t)cut * rows * g.width);
+    return;
+  }
+  block -= g.n_dx;
+  if (block < g.n_dw) {
+    // (consecutive workgroups go to the eight XCDs in turn; a strip's neighbours share lines where rows begin anywhere: each XCD
+    // gets a run of strips)
+    const int per = g.n_dw >> 3, id = (block & 7) * per + (block >> 3);
+    const int strip = id / g.dw_cuts, cut = id % g.dw_cuts;
+    const int n0 = (strip * 4 + (int)(threadIdx.x >> 6)) * 32 * CF, d0 = cut * g.dw_cut;
+    if (n0 >= classes || strip >= g.strips) return;
+    const uint64_t counted = __ballot(lane < rows && g.target[min(lane, rows - 1)] != g.ignore);
+    dfhip_few::outer<KN, CF>(g.logits.a, rows, g.width, g.l, g.ld, g.dw, cut == 0 ? g.db : nullptr, classes, n0, d0,
+                         min(d0 + g.dw_cut, g.width), counted);
+    return;
+  }
+  loss_body<kThreads>(g.rowloss, g.ctl, g.loss, rows, lds);
+}
+
+// 64 elements of dx a workgroup, each of its waves a quarter of the parts
+__global__ __launch_bounds__(kThreads) void k_few_rest(const float* __restrict__ parts, float* __restrict__ dx, int n, int cuts) {
+  __shared__ float sh[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at = (int)blockIdx.x * 64 + lane;
+  const int per = (cuts + 3) / 4, z1 = min(cuts, (wave + 1) * per);
+  float v = 0.0f;
+  if (at < n) {
+    int z = wave * per;
+    for (; z + 8 <= z1; z += 8) {
+      float q[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) q[k] = parts[(int64_t)(z + k) * n + at];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v += q[k];
+    }
+    for (; z < z1; z++) v += parts[(int64_t)z * n + at];
+  }
+  sh[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && at < n) dx[at] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+}
+
 __global__ __launch_bounds__(kThreads) void k_lce_scale(const float* __restrict__ src, const float* __restrict__ scalar,
                                                         float* __restrict__ dst, int64_t n) {
   const float s = scalar[0];
@@ -489,6 +679,106 @@ int rows_pass(float* logits, const float* target, int n, int launch_rows, float*
   return DFHIP_OK;
 }
 
+// Which calls go this way (measured, microseconds, this way / the split products):
+//   up to 32 rows: all.  loss and gradients, 32 rows: 256 x 1000 21 / 23, 1024 x 16384 65 / 93, 1024 x 50001 180 / 331,
+//     2048 x 99991 691 / 1275; the loss alone: 13 / 18, 27 / 54, 54 / 179, 199 / 670
+//   33 to 64 rows, where the fp32 matrix cores begin to count: the loss alone from 3 M elements of W (64 rows: 2048 x 1000 34 / 26,
+//     64 x 50001 23 / 40, 1024 x 16384 40 / 54, 1024 x 50001 87 / 179), with gradients from 32 M (1024 x 16384 103 / 91,
+//     1024 x 50001 279 / 319, 2048 x 99991 1066 / 1267)
+inline bool few_rows(int64_t rows, int64_t width, int64_t classes, bool grads) {
+  if (classes < 4 || rows > dfhip_few::kMost) return false;
+  return rows <= 32 || width * classes >= (grads ? (int64_t)32 << 20 : (int64_t)3 << 20);
+}
+
+template <int RB>
+int few_logits(const Few& g) {
+  if (g.cols == 32) DF_LAUNCH((k_few_logits<RB, 1, 8>), dim3((unsigned)g.tiles), dim3(512), 0, stream(), g);
+  else DF_LAUNCH((k_few_logits<RB, 4, 4>), dim3((unsigned)g.tiles), dim3(256), 0, stream(), g);
+  DF_LAUNCH_CHECK();
+  return DFHIP_OK;
+}
+
+int few_rows_forward(const float* x, const float* w, const float* bias, const float* target, float* loss, float* dx, float* dw,
+                     float* db, int rows, int width, int classes, float ignore, float smooth, int mean) {
+  const bool grads = dx || dw || db;
+  const int64_t ld = df_ceil_div(classes, 128) * 128;
+  const int cols = df_ceil_div(classes, 128) < num_cus() ? 32 : 128, tiles = (int)df_ceil_div(classes, cols);
+  // dx: about two workgroups a CU, two windows each at least; at most 256 parts
+  const int dx_tiles = (int)df_ceil_div(width, 128);
+  int cuts = std::max(1, std::min(std::min(256, 2 * num_cus() / dx_tiles), (int)df_ceil_div(classes, 2 * dfhip_few::kWindow)));
+  const int cut = (int)df_ceil_div(df_ceil_div(classes, cuts), dfhip_few::kWindow) * dfhip_few::kWindow;
+  cuts = (int)df_ceil_div(classes, cut);
+  Held logits, small, parts;
+  const int64_t stats = 3 * (int64_t)rows * tiles;
+  int st = small.take((int64_t)(sizeof(Ctl) / 4) + rows + stats);
+  if (st == DFHIP_OK) st = logits.take(rows * ld);
+  if (st == DFHIP_OK && dx && cuts > 1) st = parts.take((int64_t)cuts * rows * width);
+  if (st != DFHIP_OK) return st;
+  Ctl* ctl = reinterpret_cast<Ctl*>(small.p);
+  float* rowloss = small.p + sizeof(Ctl) / 4;
+  Few g = {};
+  g.logits = {x, w, width, classes, rows, classes, width};
+  g.dx = {logits.p, w, ld, classes, rows, width, classes};
+  g.bias = bias;
+  g.l = logits.p;
+  g.ld = ld;
+  g.stat = rowloss + rows;
+  g.tiles = tiles;
+  g.cols = cols;
+  g.target = target;
+  g.ignore = ignore;
+  g.smooth = smooth;
+  g.dw = dw;
+  g.db = db;
+  g.parts = cuts > 1 ? parts.p : dx;
+  g.loss = loss;
+  g.rowloss = rowloss;
+  g.ctl = ctl;
+  g.width = width;
+  st = rows <= 32 ? few_logits<1>(g) : few_logits<2>(g);
+  if (st != DFHIP_OK) return st;
+  const int chunk = grads ? std::max(4096, (int)df_ceil_div(df_ceil_div(ld, 64), 1024) * 1024) : (int)ld;
+  const int chunks = (int)df_ceil_div(ld, chunk);
+  if (grads)
+    DF_LAUNCH(k_few_rows<true>, dim3((unsigned)(rows * chunks)), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks,
+              rowloss, ctl);
+  else
+    DF_LAUNCH(k_few_rows<false>, dim3((unsigned)rows), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks, rowloss,
+              ctl);
+  DF_LAUNCH_CHECK();
+  if (!grads) {
+    DF_LAUNCH(k_lce_loss, dim3(1), dim3(1024), 0, stream(), rowloss, ctl, loss, (int64_t)rows);
+    DF_LAUNCH_CHECK();
+    return DFHIP_OK;
+  }
+  if (dx) {
+    g.cuts = cuts;
+    g.cut = cut;
+    g.n_dx = dx_tiles * (int)df_ceil_div(cuts, 8) * 8;
+  }
+  if (dw || db) {
+    g.strips = (int)df_ceil_div(classes, rows <= 32 ? few_strip<32>() : few_strip<64>());
+    // dW: about four workgroups a CU, 32 rows each at least
+    const int want = dw ? std::max(1, std::min((int)df_ceil_div(width, 32), 4 * num_cus() / g.strips)) : 1;
+    g.dw_cut = (int)df_ceil_div(df_ceil_div(width, want), 32) * 32;
+    g.dw_cuts = dw ? (int)df_ceil_div(width, g.dw_cut) : 1;
+    g.n_dw = (int)df_ceil_div((int64_t)g.strips * g.dw_cuts, 8) * 8;
+  }
+  const dim3 grid((unsigned)(g.n_dx + g.n_dw + 1));
+#define FEW(KN) DF_LAUNCH((k_few_pair<KN>), grid, dim3(kThreads), 0, stream(), g, rows, classes)
+  if (rows <= 8) FEW(8);
+  else if (rows <= 32) FEW(32);
+  else FEW(64);
+#undef FEW
+  DF_LAUNCH_CHECK();
+  if (dx && cuts > 1) {
+    const int n = rows * width;
+    DF_LAUNCH(k_few_rest, dim3((unsigned)df_ceil_div(n, 64)), dim3(kThreads), 0, stream(), parts.p, dx, n, cuts);
+    DF_LAUNCH_CHECK();
+  }
+  return DFHIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -513,6 +803,12 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     return st;
   }
   const bool grads = dx || dw || db;
+  if (few_rows(rows, width, classes, grads)) {
+    ProfScope prof("linear_ce", (grads ? 6.0 : 2.0) * (double)rows * (double)width * (double)classes,
+                   4.0 * ((grads ? 3.0 : 1.0) * (double)width * classes + 2.0 * (double)rows * width));
+    return few_rows_forward(x, w, bias, target, loss, dx, dw, db, (int)rows, (int)width, (int)classes, (float)ignore_index,
+                            (float)label_smoothing, mean);
+  }
   const int64_t np = padded(rows), dp = padded(width), vp = padded(classes);
   // pieces of about the same length, a multiple of 256 rows
   const int64_t cap = std::max<int64_t>(256, kPieceBytes / (4 * vp) / 256 * 256), pieces = df_ceil_div(rows, cap);

@@ -4,6 +4,7 @@ nn.LinearCrossEntropyLoss; dfhip_linear_ce_forward) against the definition in 64
 Tolerances, from the arithmetic (u = 2^-24).  A product of K terms a b is formed from operands that carry at most 2^-22 relative
 each (or a floor of 2^-39 of the array's largest magnitude A, B) and summed in fp32 in at most 3 K roundings, independent of each
 other: |error| <= (12 + 6 sqrt(3 K)) u sum|a b| + 2^-38 (A sum|b| + B sum|a|), six standard deviations.
+Few rows are multiplied in fp32 as they are: operands without an error, K roundings, inside the same bound.
   E   = the largest such error of a row's logits, plus u |l| for the bias;
   row loss: the log-sum-exp and the target's logit move by at most E each, the sums over V (depth V / 256 + 20) and the last
         operations add u (V / 256 + 40) (1 + |lse - l_t|), the smoothing term another E + u (V/256 + 20) mean|l - m|;
@@ -115,6 +116,91 @@ def test_values_and_gradients(hip_device, N, D, V):
 def test_smoothing_reductions_and_rows_that_are_not_counted(hip_device, reduction, smoothing, ignore):
     x, w, b, t = _data(150, 70, 333, 5, ignored=0.3, ignore=ignore)
     _check(hip_device, x, w, b, t, reduction=reduction, label_smoothing=smoothing, ignore_index=ignore)
+
+
+# few rows go another way (the fp32 matrix cores, W as it is): one to 64 rows, 32- and 128-column tiles, classes and widths that
+# end inside a tile, a step, a window
+FEW = [(1, 8, 4), (1, 300, 1003), (2, 7, 5), (5, 37, 33), (8, 64, 127), (9, 65, 129), (20, 129, 1000), (32, 8, 4097), (32, 515, 700),
+       (3, 16, 32641), (17, 45, 33003), (32, 130, 50001), (1, 2100, 32770)]
+
+
+@pytest.mark.parametrize("N,D,V", FEW)
+def test_few_rows(hip_device, N, D, V):
+    _check(hip_device, *_data(N, D, V, N + D + V, ignored=0.2 if N > 4 else 0.0, bias=D % 2 == 1), label_smoothing=0.1 if V % 2 else 0.0)
+
+
+def test_33_to_64_rows_of_a_large_product(hip_device):
+    _check(hip_device, *_data(45, 700, 48001, 25, ignored=0.1), label_smoothing=0.1)
+
+
+@pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001)])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_evaluation_of_few_rows(hip_device, N, D, V, smoothing):
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x, w, b, t = _data(N, D, V, 26, ignored=0.3 if N > 1 else 0.0)
+    with no_grad():
+        loss = F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, w, b, t)], label_smoothing=smoothing)
+    ref = _reference(x, w, b, t, e=smoothing)
+    _within(float(loss.numpy()[0]), ref[0][0], ref[0][1], "loss")
+
+
+@pytest.mark.parametrize("V", [300, 33000])
+def test_few_rows_with_masked_classes(hip_device, V):
+    """a bias that takes out whole column tiles, the first and the last among them"""
+    x, w, b, t = _data(12, 40, V, 27)
+    out = np.zeros(V, bool)
+    out[:200] = out[-40:] = out[210::5] = True
+    t[:] = np.nonzero(~out)[0][t.astype(int) % int((~out).sum())]
+    ref = _reference(x, w[:, ~out], b[:, ~out], np.searchsorted(np.nonzero(~out)[0], t).astype(np.float32))
+    for low in (-np.inf, np.finfo(np.float32).min):
+        c = b.copy()
+        c[0, out] = low
+        loss, dx, dw, db = _run(hip_device, x, w, c, t)
+        _within(loss, ref[0][0], ref[0][1], "loss")
+        _within(dx, ref[1][0], 2 * ref[1][1], "dx")
+        _within(dw[:, ~out], ref[2][0], 2 * ref[2][1], "dw")
+        assert not dw[:, out].any() and not db[0, out].any()
+
+
+@pytest.mark.parametrize("V", [90, 33000])
+def test_few_rows_that_are_not_finite_or_not_counted(hip_device, V):
+    x, w, b, t = _data(21, 30, V, 28)
+    t[5] = t[20] = -100
+    clean = _run(hip_device, np.where(t[:, None] == -100, np.float32(0), x), w, b, t)
+    for bad in (np.nan, np.inf, 3e38):
+        y = x.copy()
+        y[t == -100] = bad
+        for a, c in zip(_run(hip_device, y, w, b, t), clean):
+            assert np.array_equal(a, c)
+        y = x.copy()
+        y[11, 3] = bad if bad != 3e38 else -np.inf
+        loss, dx, _, _ = _run(hip_device, y, w, b, t)
+        assert np.isnan(loss) and np.all(np.isnan(dx[11])) and np.all(np.isfinite(np.delete(dx, 11, 0)[t[np.arange(21) != 11] != -100]))
+    for bad in (float(V), -1.0, 2.5, np.nan):
+        u = t.copy()
+        u[17] = bad
+        loss, dx, dw, db = _run(hip_device, x, w, b, u)
+        assert np.isnan(loss) and np.all(np.isnan(dx[17])) and np.all(np.isnan(dw)) and np.all(np.isnan(db))
+        assert np.all(np.isfinite(np.delete(dx, 17, axis=0)))
+    t[:] = -100
+    loss, dx, dw, db = _run(hip_device, x, w, b, t)
+    assert loss == 0.0 and not dx.any() and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("N,D,V", [(9, 48, 210), (25, 33, 33003)])
+def test_one_gradient_of_few_rows_at_a_time(hip_device, which, N, D, V):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    x, w, b, t = _data(N, D, V, 29)
+    ts = [Tensor(a, device=hip_device, requires_grad=k == which) for k, a in enumerate((x, w, b))]
+    F.linear_cross_entropy(*ts, Tensor(t, device=hip_device)).backward()
+    want, tol = _reference(x, w, b, t)[1 + which]
+    _within(ts[which].grad.numpy(), want, tol, "gradient")
+    assert all(ts[k].grad is None for k in range(3) if k != which)
+    Graph.free_graph_all()
 
 
 def test_without_a_bias(hip_device):
@@ -321,12 +407,12 @@ def test_two_sweeps_over_a_retained_graph_and_a_held_gradient(hip_device):
 
 
 def test_inside_a_captured_graph(hip_device):
-    """two graphs over different shapes captured one after the other, replayed in turn on changed inputs with eager calls between"""
+    """graphs over different shapes captured one after the other, replayed in turn on changed inputs with eager calls between"""
     from deepflows_amd.nn import functional as F
     from deepflows_amd.tensor import Graph, Tensor
     mod = hip_device.mod
     made = []
-    for k, (N, D, V) in enumerate([(96, 64, 1500), (40, 100, 333)]):
+    for k, (N, D, V) in enumerate([(96, 64, 1500), (40, 100, 333), (16, 100, 2003)]):
         x, w, b, t = _data(N, D, V, 30 + k, ignored=0.2)
         leaves = [Tensor(a, device=hip_device, requires_grad=True) for a in (x, w, b)]
         tt = Tensor(t, device=hip_device)
