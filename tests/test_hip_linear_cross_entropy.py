@@ -133,7 +133,7 @@ def test_33_to_64_rows_of_a_large_product(hip_device):
     _check(hip_device, *_data(45, 700, 48001, 25, ignored=0.1), label_smoothing=0.1)
 
 
-@pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001)])
+@pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001), (100, 700, 48001)])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
 def test_evaluation_of_few_rows(hip_device, N, D, V, smoothing):
     from deepflows_amd.autograd import no_grad
