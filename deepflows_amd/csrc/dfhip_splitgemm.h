@@ -46,7 +46,65 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(r == r ? r : 0.0f);    // (inf - inf, NaN: no low half)
 }
 
-enum { EPI_BIAS = 0, EPI_STORE = 1, EPI_ADD = 2 };
+// e^x for x <= 0: 2^(x log2(e)) with the product's rounding error and the constant's own put back to first order (|x| times
+// 2^-24 otherwise), results below 2^-126 as 0.  Half the instructions of expf, whose range checks nothing here needs.
+__device__ __forceinline__ float exp_of(float x) {
+  constexpr double kLog2e = 1.4426950408889634;
+  constexpr float hi = (float)kLog2e, lo = (float)(kLog2e - (double)(float)kLog2e);
+  x = x < -200.0f ? -200.0f : x;                           // (-inf; a NaN stays one)
+  const float t = x * hi, e = fmaf(x, lo, fmaf(x, hi, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, e * 0.6931471805599453f, p);
+}
+
+// over LANES (8, 16 or 32) neighbouring lanes, the result in all of them, in the vector unit
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int LANES, class F>
+__device__ __forceinline__ float lanes_reduce(float v, F f) {
+  v = f(v, moved<0xB1>(v));                        // quad_perm 1 0 3 2
+  v = f(v, moved<0x4E>(v));                        // quad_perm 2 3 0 1
+  v = f(v, moved<0x141>(v));                       // row_half_mirror: the other four of eight
+  if (LANES > 8) v = f(v, moved<0x140>(v));        // row_mirror: the other eight of sixteen
+  if (LANES > 16) {                                // odd and even rows of sixteen: each pair's even row twice, its odd row twice
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  return v;
+}
+// What a row of softmax needs of LANES x N of its logits, N a lane: the largest one, the sum of exponentials from there, and (`sum`)
+// the sum of l - largest, in all of the lanes.  w is -inf where there is no class (`in`).
+struct RowPart { float m, z, t; };
+template <int N, int LANES>
+__device__ __forceinline__ RowPart row_part(const float* w, const bool* in, bool sum) {
+  RowPart p;
+  float m = w[0];
+#pragma unroll
+  for (int f = 1; f < N; f++) m = fmaxf(m, w[f]);
+  p.m = lanes_reduce<LANES>(m, [](float a, float b) { return fmaxf(a, b); });
+  const float from = p.m > -INFINITY ? p.m : 0.0f; // (all masked: z = 0)
+  p.z = p.t = 0.0f;
+#pragma unroll
+  for (int f = 0; f < N; f++) p.z += exp_of(w[f] - from);
+  const auto add = [](float a, float b) { return a + b; };
+  p.z = lanes_reduce<LANES>(p.z, add);
+  if (sum) {
+#pragma unroll
+    for (int f = 0; f < N; f++) p.t += in[f] ? w[f] - from : 0.0f;
+    p.t = lanes_reduce<LANES>(p.t, add);
+  }
+  return p;
+}
+// ... into three arrays `stride` apart
+__device__ __forceinline__ void store_part(float* at, int64_t stride, const RowPart& p) {
+  at[0] = p.m;
+  at[stride] = p.z;
+  at[2 * stride] = p.t;
+}
+
+enum { EPI_BIAS = 0, EPI_STORE = 1, EPI_ADD = 2, EPI_STATS = 3 };
 
 // Tiles [0, full) are formed by one workgroup each.  The `rest` tiles behind them -- what would be a last round that leaves most
 // of the chip idle -- are cut along the reduction into `splits` parts of `ksteps_split` steps; their partial tiles go to `parts`
@@ -66,7 +124,14 @@ struct Gemm {
   const float* scale;
   float* colsum;                         // or NULL: column sums of b (n), scaled by 2^exp_c * scale; added where EPI_ADD (b across)
   float* parts;                          // (rest * splits) x (BM * BN + BN)
+  // EPI_STATS: nothing of the product (+ bias) is stored but, of each row's runs of `unit<T>()` columns, row_part's numbers in three
+  // arrays of (m, units), and the targets' elements
+  float* stat;
+  int units, sum;
+  const float* target;
+  float* lt;
 };
+template <int T> constexpr int unit() { return T == 64 ? 32 : 64; }      // a wave's columns
 
 // place of a tile: bands of eight tile rows, down the band first
 __device__ __forceinline__ void place(const Gemm& g, int tile, int& tm, int& tn) {
@@ -77,7 +142,7 @@ __device__ __forceinline__ void place(const Gemm& g, int tile, int& tm, int& tn)
 
 template <int EPI>
 __device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
-  return EPI == EPI_BIAS && g.bias && n < g.n ? g.bias[n] : 0.0f;
+  return (EPI == EPI_BIAS || EPI == EPI_STATS) && g.bias && n < g.n ? g.bias[n] : 0.0f;
 }
 // One value of row m (c: its place) and column n.  STREAM: past the caches, where a wave's stores fill whole lines -- a round of
 // 256 x 256 tiles writes 64 MB that nothing reads soon, and the operands' lines stay (eval 1500 x 1024 x 30011: 373 -> 355 us).
@@ -88,6 +153,85 @@ __device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias,
   if (EPI == EPI_ADD) *c += v;
   else if (STREAM) __builtin_nontemporal_store(v, c);
   else *c = v;
+}
+// EPI_STATS for one row: four columns a lane from n
+template <int T>
+__device__ __forceinline__ void emit_stats(const Gemm& g, int e, const float* bias, int64_t m, int64_t n, const float* v) {
+  constexpr int LANES = unit<T>() / 4;
+  float w[4];
+  bool in[4];
+#pragma unroll
+  for (int f = 0; f < 4; f++) {
+    in[f] = n + f < g.n;
+    w[f] = in[f] ? ldexpf(v[f], e) + bias[f] : -INFINITY;
+  }
+  const RowPart p = row_part<4, LANES>(w, in, g.sum != 0);
+  if (m >= g.m) return;
+  const int64_t u = n / unit<T>();
+  if ((threadIdx.x & (LANES - 1)) == 0 && u < g.units) store_part(g.stat + m * g.units + u, (int64_t)g.m * g.units, p);
+  const float t = g.target[m];
+#pragma unroll
+  for (int f = 0; f < 4; f++)
+    if (in[f] && t == (float)(int)(n + f)) g.lt[m] = w[f];
+}
+// EPI_STATS for a wave's TM x TN tiles from row m0 and column n0: 32 rows at a time through LDS of its own, half a row a lane -- a
+// row's sums across the lanes that hold it would be twelve steps for two values, and their code, once for each of 64 rows, longer
+// than the instruction cache.
+template <int T, int TM, int TN>
+__device__ __forceinline__ void wave_stats(const Gemm& g, int e, const float* bias, int64_t m0, int64_t n0, const f32x16 (*acc)[TN],
+                                           float* own) {
+  static_assert(TN * 32 == unit<T>(), "a run");
+  constexpr int PITCH = TN * 32 + 4, HALF = TN * 16;
+  const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5, row = lane >> 1, c0 = (lane & 1) * HALF;
+  const int64_t u = n0 / unit<T>();
+  const int valid = (int)min(max((int64_t)g.n - n0 - c0, (int64_t)0), (int64_t)HALF);
+  bool in[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) in[j] = n0 + j * 32 + i32 < g.n;
+  float targets[TM];
+#pragma unroll
+  for (int i = 0; i < TM; i++) targets[i] = g.target[min(m0 + i * 32 + row, (int64_t)g.m - 1)];
+#pragma unroll 1
+  for (int i = 0; i < TM; i++) {
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < TM; k++)
+      if (i == k) {
+        t = targets[k];
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+#pragma unroll
+          for (int j = 0; j < TN; j++)
+            own[(8 * (r >> 2) + 4 * h + (r & 3)) * PITCH + j * 32 + i32] = in[j] ? ldexpf(acc[k][j][r], e) + bias[j] : -INFINITY;
+      }
+    const float* p = own + row * PITCH + c0;
+    float w[HALF];
+#pragma unroll
+    for (int c = 0; c < HALF; c += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + c);
+      w[c] = v.x; w[c + 1] = v.y; w[c + 2] = v.z; w[c + 3] = v.w;
+    }
+    float m = w[0];
+#pragma unroll
+    for (int c = 1; c < HALF; c++) m = fmaxf(m, w[c]);
+    m = fmaxf(m, moved<0xB1>(m));                  // (the row's other half is the neighbour)
+    const float from = m > -INFINITY ? m : 0.0f;
+    RowPart part = {m, 0.0f, 0.0f};
+    if (g.sum) {
+#pragma unroll
+      for (int c = 0; c < HALF; c++) part.t += c < valid ? w[c] - from : 0.0f;
+      part.t += moved<0xB1>(part.t);
+    }
+#pragma unroll
+    for (int c = 0; c < HALF; c++) part.z += exp_of(w[c] - from);
+    part.z += moved<0xB1>(part.z);
+    const int64_t at = m0 + i * 32 + row;
+    if (at < g.m) {
+      if ((lane & 1) == 0 && u < g.units) store_part(g.stat + at * g.units + u, (int64_t)g.m * g.units, part);
+      const float d = t - (float)(int)(n0 + c0);   // (exact: whole numbers up to 2^24; another target is refused later)
+      if (d >= 0.0f && d < (float)valid) g.lt[at] = p[(int)d];
+    }
+  }
 }
 template <int EPI>
 __device__ __forceinline__ void emit_colsum(const Gemm& g, float sc, int64_t n, float v) {
@@ -356,6 +500,11 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
   float bias[TN];
 #pragma unroll
   for (int j = 0; j < TN; j++) bias[j] = bias_of<EPI>(g, n + j * 32);
+  if constexpr (EPI == EPI_STATS) {
+    __syncthreads();                               // (the last step's operands have been read)
+    wave_stats<T, TM, TN>(g, e, bias, m0 + wm, n0 + wn, acc, reinterpret_cast<float*>(lds) + wave * (32 * (TN * 32 + 4)));
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
@@ -403,6 +552,10 @@ __device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
   float bias[4];
 #pragma unroll
   for (int k = 0; k < 4; k++) bias[k] = bias_of<EPI>(g, n + k);
+  if constexpr (EPI == EPI_STATS) {
+    emit_stats<T>(g, e, bias, m0 + cell / BN, n, v);
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 4; k++) emit<EPI, false>(g, e, sc, bias[k], m0 + cell / BN, n + k, g.c + (m0 + cell / BN) * g.ldc + n + k, v[k]);
   if (g.colsum && tm == 0 && slice == 0 && (int)threadIdx.x < BN) {
@@ -503,7 +656,7 @@ inline void apply(Gemm& g, const Plan& p, int64_t m, int64_t n) {
   g.splits = p.splits;
   g.ksteps = p.ksteps;
   g.ksteps_split = p.ksteps_split;
-  g.m = g.c ? (int)m : 0;                          // (column sums alone: nothing of the product is stored)
+  g.m = g.c || g.stat ? (int)m : 0;                // (column sums alone: nothing of the product is stored)
   g.n = (int)n;
 }
 inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.tile * p.tile + p.tile); }

@@ -15,7 +15,8 @@
 //   k_lce_split    x, W -> split arrays; the number of counted rows
 //   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> k_lce_pair: the dx
 //                  product and the dW product (db on the side: the column sums of its second operand); with the last piece, the loss
-//   (k_lce_loss    the loss, where there are no gradients)
+//   without gradients: the product's epilogue leaves what the softmax needs of every 64 logits and the targets' (none is stored),
+//                  k_few_rows joins them, k_lce_loss
 //
 // Measured.  8192 x 1024 x 50001 with gradients, 6.65 ms: logits 2.08 ms and the pair 3.85 ms, 1.21 and 1.31 PFLOP/s of fp16 (the
 // library's 8192^3 fp16 product: 1.18; at that rate the three products alone are 6.42 ms, in fp32 16.4), rows 0.68 ms (3.3 GB, 4.8
@@ -205,25 +206,13 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   }
 }
 
-// e^x for x <= 0: 2^(x log2(e)) with the product's rounding error and the constant's own put back to first order (|x| times
-// 2^-24 otherwise), results below 2^-126 as 0.  Half the instructions of expf, whose range checks nothing here needs.
-__device__ __forceinline__ float exp_of(float x) {
-  constexpr double kLog2e = 1.4426950408889634;
-  constexpr float hi = (float)kLog2e, lo = (float)(kLog2e - (double)(float)kLog2e);
-  x = x < -200.0f ? -200.0f : x;                           // (-inf; a NaN stays one)
-  const float t = x * hi, e = fmaf(x, lo, fmaf(x, hi, -t));
-  const float p = __builtin_amdgcn_exp2f(t);
-  return fmaf(p, e * 0.6931471805599453f, p);
-}
-
 // A workgroup a row: the row's loss, and dl (times 2^kTop) over its logits as a split array.  `cells` is the padded row, a
 // multiple of 256; a row that is not counted, or lies behind the last one (blockIdx.x >= rows), becomes zeros.
 // U > 0: U groups of eight logits a thread hold the row in registers (T * 8 * U >= cells), one pass over memory each way;
 // U = 0: any length, the row read three times.
 template <int T, int U>
 __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, const float* __restrict__ target, int rows,
-                                                float* __restrict__ rowloss, int classes, int cells, float ignore, float smooth,
-                                                int grads) {
+                                                float* __restrict__ rowloss, int classes, int cells, float ignore, float smooth) {
   __shared__ float sh[T / 64];
   float* l = logits + (int64_t)blockIdx.x * cells;
   const bool exists = (int)blockIdx.x < rows;
@@ -242,8 +231,7 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   };
   if (t == ignore) {
     if (threadIdx.x == 0 && exists) rowloss[blockIdx.x] = 0.0f;
-    if (grads)
-      for (int c = threadIdx.x * 4; c < cells; c += T * 4) *reinterpret_cast<float4*>(l + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = threadIdx.x * 4; c < cells; c += T * 4) *reinterpret_cast<float4*>(l + c) = make_float4(0.f, 0.f, 0.f, 0.f);
     return;
   }
   const bool ok = t >= 0.0f && t < (float)classes && t == floorf(t);
@@ -312,7 +300,6 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
     if (smooth > 0.0f) r -= smooth * (s / (float)classes);
     rowloss[blockIdx.x] = ok ? r : NAN;
   }
-  if (!grads) return;
   const float top = (float)(1 << kTop), iz = ok ? top / z : NAN, q = top * (smooth / (float)classes), p1 = top * (1.0f - smooth);
   for (int i = 0; i < trips; i++) {
     if (U == 0) {
@@ -383,8 +370,7 @@ __global__ __launch_bounds__(256) void k_lce_pair_rest(Pair p) {
 }
 
 // ---- few rows: W is read as it is (dfhip_fewrows.h) ----------------------------------------------------------------------------
-//   k_few_logits   logits (rows, ld), and of every column tile the rows' largest logit, sum of exponentials and sum (its own three
-//                  numbers: a row is spread over more workgroups than would wait for each other)
+//   k_few_logits   logits (rows, ld), and of every column tile the rows' largest logit, sum of exponentials and sum (row_part)
 //   k_few_rows     those joined: row losses; dl (times the mean's factor) over the logits
 //   k_few_pair     the dx product, cut along the classes, and the dW product (db on the side); the loss
 //   k_few_rest     the parts of dx added up
@@ -395,6 +381,7 @@ struct Few {
   int64_t ld;                              // a multiple of 128
   float* stat;                             // three arrays of (rows, tiles): largest, sum of exponentials, sum of l - largest
   int tiles, cols;                         // their number and width
+  const float* lt;                         // the targets' logits, or NULL: they are in l
   const float* target;
   float ignore, smooth;
   float *dw, *db, *parts, *loss;
@@ -403,17 +390,6 @@ struct Few {
   int width, cuts, cut, n_dx;              // dx: `cuts` ranges of `cut` classes, n_dx workgroups
   int strips, dw_cuts, dw_cut, n_dw;       // dW: strips of few_strip() columns, dw_cuts ranges of dw_cut rows of it
 };
-
-__device__ __forceinline__ float half_max(float v) {       // over 32 lanes
-#pragma unroll
-  for (int off = 16; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-  return v;
-}
-__device__ __forceinline__ float half_sum(float v) {
-#pragma unroll
-  for (int off = 16; off; off >>= 1) v += __shfl_xor(v, off);
-  return v;
-}
 
 template <int RB, int CF, int NW>
 __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
@@ -432,39 +408,26 @@ __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
   dfhip_few::across<RB, CF, NW>(p, n0, lds, [&](int row, const float* v) {
     if (row >= p.rows) return;                             // (uniform in the half wave)
     row += row0;
-    float w[CF], m = -INFINITY;                            // -inf behind the last class
+    float w[CF];                                           // -inf behind the last class
 #pragma unroll
     for (int f = 0; f < CF; f++) {
       w[f] = -INFINITY;
 #pragma unroll
       for (int e = 0; e < CF; e++) w[f] = f + over == e ? v[e] + bias[f] : w[f];
-      m = fmaxf(m, w[f]);
     }
     typedef float vec __attribute__((ext_vector_type(CF)));
     *reinterpret_cast<vec*>(g.l + (int64_t)row * g.ld + c) = *reinterpret_cast<const vec*>(w);
-    m = half_max(m);
-    const float from = m > -INFINITY ? m : 0.0f;           // (a tile whose classes are all masked: z = 0)
-    float z = 0.0f, t = 0.0f;
+    bool in[CF];
 #pragma unroll
-    for (int f = 0; f < CF; f++) {
-      z += exp_of(w[f] - from);
-      t += c + f < p.n ? w[f] - from : 0.0f;
-    }
-    z = half_sum(z);
-    if (g.smooth > 0.0f) t = half_sum(t);
-    if (i == 0) {
-      float* st = g.stat + (int64_t)row * g.tiles + tile;
-      const int64_t n = (int64_t)g.logits.rows * g.tiles;
-      st[0] = m;
-      st[n] = z;
-      st[2 * n] = t;
-    }
+    for (int f = 0; f < CF; f++) in[f] = c + f < p.n;
+    const RowPart part = row_part<CF, 32>(w, in, g.smooth > 0.0f);
+    if (i == 0) store_part(g.stat + (int64_t)row * g.tiles + tile, (int64_t)g.logits.rows * g.tiles, part);
   });
 }
 
 // `chunks` workgroups a row, each of which joins the row's tiles for itself; the one that holds the target's column also makes the
 // row's loss (nobody else touches that column)
-template <bool GRADS>
+template <bool GRADS, bool COUNT>
 __global__ __launch_bounds__(kThreads) void k_few_rows(Few g, int rows, int classes, int mean, int chunk, int chunks,
                                                        float* __restrict__ rowloss, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
@@ -473,11 +436,14 @@ __global__ __launch_bounds__(kThreads) void k_few_rows(Few g, int rows, int clas
   const float t = g.target[row];
   float* l = g.l + (int64_t)row * g.ld;
   const int lo = ch * chunk, hi = min(lo + chunk, (int)g.ld);
-  int n = 0;
-  for (int k = threadIdx.x; k < rows; k += kThreads) n += g.target[k] != g.ignore ? 1 : 0;
-  n = block_reduce<kThreads>(n, shi, Add());
-  const float scale = mean ? 1.0f / (float)max(n, 1) : 1.0f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) ctl->scale = scale;
+  float scale = 1.0f;
+  if (COUNT) {
+    int n = 0;
+    for (int k = threadIdx.x; k < rows; k += kThreads) n += g.target[k] != g.ignore ? 1 : 0;
+    n = block_reduce<kThreads>(n, shi, Add());
+    if (mean) scale = 1.0f / (float)max(n, 1);
+    if (blockIdx.x == 0 && threadIdx.x == 0) ctl->scale = scale;
+  }
   if (t == g.ignore) {
     if (ch == 0 && threadIdx.x == 0) rowloss[row] = 0.0f;
     if (GRADS)
@@ -488,7 +454,7 @@ __global__ __launch_bounds__(kThreads) void k_few_rows(Few g, int rows, int clas
   const bool ok = t >= 0.0f && t < (float)classes && t == floorf(t);
   const int ti = ok ? (int)t : 0;
   const bool owner = ti >= lo && ti < hi;
-  const float lt = owner ? l[ti] : 0.0f;
+  const float lt = owner ? (g.lt ? g.lt[row] : l[ti]) : 0.0f;
   float m = -INFINITY;
 #pragma unroll 4
   for (int k = threadIdx.x; k < g.tiles; k += kThreads) m = fmaxf(m, sm[k]);
@@ -595,15 +561,15 @@ int room(Held& h, int64_t& held, int64_t need) {   // scratch that grows as need
   return h.take(need);
 }
 
-template <int T>
+template <int T, int EPI>
 int launch_logits(const Gemm& g) {
   static bool done = false;
-  const int st = allow_lds((const void*)k_split_gemm<T, false, true, EPI_BIAS>, lds_bytes<T>(), done);
+  const int st = allow_lds((const void*)k_split_gemm<T, false, true, EPI>, lds_bytes<T>(), done);
   if (st != DFHIP_OK) return st;
-  DF_LAUNCH((k_split_gemm<T, false, true, EPI_BIAS>), dim3((unsigned)groups(g)), dim3(threads<T>()), lds_bytes<T>(), stream(), g);
+  DF_LAUNCH((k_split_gemm<T, false, true, EPI>), dim3((unsigned)groups(g)), dim3(threads<T>()), lds_bytes<T>(), stream(), g);
   DF_LAUNCH_CHECK();
   if (g.rest) {
-    DF_LAUNCH((k_split_rest<T, EPI_BIAS>), dim3((unsigned)g.rest * (T * T / 1024)), dim3(256), 0, stream(), g);
+    DF_LAUNCH((k_split_rest<T, EPI>), dim3((unsigned)g.rest * (T * T / 1024)), dim3(256), 0, stream(), g);
     DF_LAUNCH_CHECK();
   }
   return DFHIP_OK;
@@ -675,10 +641,10 @@ const Choice* choose(int64_t rows, int64_t width, int64_t classes, bool dx, int6
 }
 
 int rows_pass(float* logits, const float* target, int n, int launch_rows, float* rowloss, int classes, int cells, float ignore,
-              float smooth, int grads) {
+              float smooth) {
 #define ROWS(T, U)                                                                                                        \
   DF_LAUNCH((k_lce_rows<T, U>), dim3((unsigned)launch_rows), dim3(T), 0, stream(), logits, target, n, rowloss, classes,   \
-            cells, ignore, smooth, grads)
+            cells, ignore, smooth)
   if (cells <= 2048) ROWS(256, 1);
   else if (cells <= 4096) ROWS(256, 2);
   else if (cells <= 8192) ROWS(1024, 1);
@@ -755,10 +721,10 @@ int few_rows_forward(const float* x, const float* w, const float* bias, const fl
   const int chunk = grads ? std::max(4096, (int)df_ceil_div(df_ceil_div(ld, 64), 1024) * 1024) : (int)ld;
   const int chunks = (int)df_ceil_div(ld, chunk);
   if (grads)
-    DF_LAUNCH(k_few_rows<true>, dim3((unsigned)(rows * chunks)), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks,
+    DF_LAUNCH((k_few_rows<true, true>), dim3((unsigned)(rows * chunks)), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks,
               rowloss, ctl);
   else
-    DF_LAUNCH(k_few_rows<false>, dim3((unsigned)rows), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks, rowloss,
+    DF_LAUNCH((k_few_rows<false, true>), dim3((unsigned)rows), dim3(kThreads), 0, stream(), g, rows, classes, mean, chunk, chunks, rowloss,
               ctl);
   DF_LAUNCH_CHECK();
   if (!grads) {
@@ -826,14 +792,15 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   }
   const int64_t np = padded(rows), dp = padded(width), vp = padded(classes);
   // pieces of about the same length, a multiple of 256 rows
-  const int64_t cap = std::max<int64_t>(256, kPieceBytes / (4 * vp) / 256 * 256), pieces = df_ceil_div(rows, cap);
+  const int64_t row_bytes = grads ? 4 * vp : 12 * df_ceil_div(classes, 32);
+  const int64_t cap = std::max<int64_t>(256, kPieceBytes / row_bytes / 256 * 256), pieces = df_ceil_div(rows, cap);
   const int64_t piece = padded(df_ceil_div(rows, pieces));
   Held xs, ws, logits, small, parts;
   int64_t held = 0;
   int st = small.take((int64_t)(sizeof(Ctl) / 4) + rows);
   if (st == DFHIP_OK) st = xs.take(np * dp);
   if (st == DFHIP_OK) st = ws.take(dp * vp);
-  if (st == DFHIP_OK) st = logits.take(piece * vp);
+  if (st == DFHIP_OK) st = logits.take(grads ? piece * vp : piece * (1 + 3 * df_ceil_div(classes, 32)));
   if (st != DFHIP_OK) return st;
   Ctl* ctl = reinterpret_cast<Ctl*>(small.p);
   float* rowloss = small.p + sizeof(Ctl) / 4;
@@ -856,23 +823,48 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     g.lda = dp * 4;
     g.b = (const char*)ws.p;
     g.ldb = vp * 4;
-    g.c = logits.p;
-    g.ldc = vp;
     g.bias = bias;
     g.exp_a = &ctl->ex;
     g.exp_b = &ctl->ew;
     const Choice* how = choose(n, width, classes, dx != nullptr, dw ? width : db ? 1 : 0);
     DF_CHECK_ARG(how, "linear_ce_forward: too many tiles");
+    if (grads) {
+      g.c = logits.p;
+      g.ldc = vp;
+    } else {                                       // the softmax's parts instead of the logits
+      g.units = (int)df_ceil_div(classes, how->logits.tile == 64 ? unit<64>() : unit<256>());
+      g.lt = logits.p;
+      g.stat = logits.p + n;
+      g.target = target + r0;
+      g.sum = label_smoothing > 0.0;
+    }
     apply(g, how->logits, n, classes);
     st = room(parts, held, std::max(parts_floats(how->logits), parts_floats(how->a) + parts_floats(how->b)));
     if (st != DFHIP_OK) return st;
     g.parts = parts.p;
-    st = with_tile(how->logits, [&](auto t) { return launch_logits<decltype(t)::value>(g); });
+    st = with_tile(how->logits, [&](auto t) {
+      constexpr int T = decltype(t)::value;
+      return grads ? launch_logits<T, EPI_BIAS>(g) : launch_logits<T, EPI_STATS>(g);
+    });
     if (st != DFHIP_OK) return st;
-    st = rows_pass(logits.p, target + r0, (int)n, (int)(grads ? df_ceil_div(n, 32) * 32 : n), rowloss + r0, (int)classes, (int)vp,
-                   ignore, (float)label_smoothing, grads ? 1 : 0);
+    if (!grads) {
+      Few f = {};
+      f.stat = g.stat;
+      f.tiles = g.units;
+      f.cols = how->logits.tile == 64 ? unit<64>() : unit<256>();
+      f.lt = g.lt;
+      f.ld = classes;
+      f.target = g.target;
+      f.ignore = ignore;
+      f.smooth = (float)label_smoothing;
+      DF_LAUNCH((k_few_rows<false, false>), dim3((unsigned)n), dim3(kThreads), 0, stream(), f, (int)n, (int)classes, mean,
+                (int)classes, 1, rowloss + r0, ctl);
+      DF_LAUNCH_CHECK();
+      continue;
+    }
+    st = rows_pass(logits.p, target + r0, (int)n, (int)(df_ceil_div(n, 32) * 32), rowloss + r0, (int)classes, (int)vp, ignore,
+                   (float)label_smoothing);
     if (st != DFHIP_OK) return st;
-    if (!grads) continue;
     Pair p = {};
     p.a.exp_c = p.b.exp_c = -kTop;
     p.a.scale = p.b.scale = &ctl->scale;

@@ -133,9 +133,10 @@ def test_33_to_64_rows_of_a_large_product(hip_device):
     _check(hip_device, *_data(45, 700, 48001, 25, ignored=0.1), label_smoothing=0.1)
 
 
-@pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001), (100, 700, 48001)])
+@pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001), (100, 700, 48001),
+                                   (70, 8, 3), (130, 100, 257), (300, 64, 4099), (700, 520, 9001), (70, 2000, 300), (257, 33, 64)])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
-def test_evaluation_of_few_rows(hip_device, N, D, V, smoothing):
+def test_evaluation_keeps_no_logits(hip_device, N, D, V, smoothing):
     from deepflows_amd.autograd import no_grad
     from deepflows_amd.nn import functional as F
     from deepflows_amd.tensor import Tensor
@@ -146,10 +147,14 @@ def test_evaluation_of_few_rows(hip_device, N, D, V, smoothing):
     _within(float(loss.numpy()[0]), ref[0][0], ref[0][1], "loss")
 
 
+@pytest.mark.parametrize("N", [12, 90])
 @pytest.mark.parametrize("V", [300, 33000])
-def test_few_rows_with_masked_classes(hip_device, V):
+def test_masked_runs_of_classes(hip_device, N, V):
     """a bias that takes out whole column tiles, the first and the last among them"""
-    x, w, b, t = _data(12, 40, V, 27)
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x, w, b, t = _data(N, 40, V, 27)
     out = np.zeros(V, bool)
     out[:200] = out[-40:] = out[210::5] = True
     t[:] = np.nonzero(~out)[0][t.astype(int) % int((~out).sum())]
@@ -162,6 +167,8 @@ def test_few_rows_with_masked_classes(hip_device, V):
         _within(dx, ref[1][0], 2 * ref[1][1], "dx")
         _within(dw[:, ~out], ref[2][0], 2 * ref[2][1], "dw")
         assert not dw[:, out].any() and not db[0, out].any()
+        with no_grad():
+            _within(float(F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, w, c, t)]).numpy()[0]), *ref[0], "loss")
 
 
 @pytest.mark.parametrize("V", [90, 33000])
@@ -357,6 +364,27 @@ def test_more_rows_than_one_piece_of_logits_holds(hip_device):
     _within(got[1], dx[order] / 100, tdx[order] / 100 + 4 * U * np.abs(dx[order]) / 100, "dx")
     _within(got[2], dw, 10 * tdw, "dw")
     _within(got[3], db, 4 * tdb, "db")
+
+
+def test_evaluation_of_bad_targets_and_rows(hip_device):
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    for N in (20, 100):
+        x, w, b, t = _data(N, 24, 400, 31, ignored=0.2)
+        def value(x, t):
+            with no_grad():
+                return float(F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, w, b, t)]).numpy()[0])
+        for bad in (400.0, -1.0, 2.5, np.nan, np.inf, 1e9):
+            u = t.copy()
+            u[7] = bad
+            assert np.isnan(value(x, u))
+        y = x.copy()
+        y[t == -100] = np.nan
+        assert value(y, t) == value(x, t)
+        y[np.nonzero(t != -100)[0][0], 3] = np.nan
+        assert np.isnan(value(y, t))
+        assert value(x, np.full_like(t, -100)) == 0.0
 
 
 def test_no_rows(hip_device):
