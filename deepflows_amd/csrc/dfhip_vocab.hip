@@ -12,7 +12,7 @@
 // dl where it is formed; for few rows, where W's bytes are what counts, on the fp32 matrix cores (dfhip_fewrows.h, and further
 // down).  The launches of a call:
 //   k_lce_scan     the largest magnitudes of x (counted rows) and W, finite elements only
-//   k_lce_split    x, W -> split arrays; the number of counted rows
+//   k_lce_split    x, W -> split arrays; the number of counted rows (a large W may need it twice)
 //   per piece:     logits product (+ bias) -> k_lce_rows (losses; dl over the logits, as a split array) -> k_lce_pair: the dx
 //                  product and the dW product (db on the side: the column sums of its second operand); with the last piece, the loss
 //   without gradients: the product's epilogue leaves what the softmax needs of every 64 logits and the targets' (none is stored),
@@ -38,13 +38,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kScan = 512;                                 // workgroups (= partial maxima) a tensor
+constexpr int64_t kSampled = (int64_t)16 << 20;            // from this many elements of W on its scale comes from a sample
 constexpr int64_t kPieceBytes = (int64_t)2 << 30;          // the logits of one piece of the rows
 
 // what the launches of one call hand to each other
 struct Ctl {
   float scale;                                             // 1 / number of counted rows, or 1
   int ex, ew;                                              // x = 2^ex * split array, W likewise
-  int pad;
+  unsigned found;                                          // 0, or W's largest finite magnitude where a sample missed it
   float max_x[kScan], max_w[kScan];
 };
 
@@ -76,12 +77,14 @@ __device__ __forceinline__ float finite_abs(const float4& v) {
 }
 
 // workgroups 0 .. kScan-1: x, kScan .. 2 kScan - 1: W.  The rows of x that are not counted are passed over: padding may hold
-// anything, and a large value in it would cost the counted rows their low bits.
+// anything, and a large value in it would cost the counted rows their low bits.  `sample`: of W every sixteenth piece of 64 elements
+// is read, another one in every row of pieces; the conversion finds out whether that was enough.
 __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__ x, int64_t rows, int64_t width,
                                                        const float* __restrict__ target, float ignore,
-                                                       const float* __restrict__ w, int64_t nw, Ctl* __restrict__ ctl) {
+                                                       const float* __restrict__ w, int64_t nw, int sample, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
   const bool second = blockIdx.x >= kScan;
+  if (blockIdx.x == 0 && threadIdx.x == 0) ctl->found = 0;
   const int blk = (int)blockIdx.x & (kScan - 1);
   float m = 0.0f;
   if (!second) {                                           // a wave takes up to 1 024 elements of one row at a time
@@ -109,6 +112,21 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
       }
       m = t == ignore ? m : fmaxf(m, s);
     }
+  } else if (sample) {
+    // (64 elements of 1 024: their place moves on from one to the next, or all would lie on the same few memory channels)
+    const int64_t runs = nw >> 10, step = kScan * (kThreads / 16);
+    const int lane = threadIdx.x & 15;
+    int64_t i = (int64_t)blk * (kThreads / 16) + (threadIdx.x >> 4);
+    for (; i < runs; i += 4 * step) {
+      dfhip_few::f32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int64_t r = min(i + u * step, runs - 1);
+        v[u] = *reinterpret_cast<const dfhip_few::f32x4u*>(w + (r << 10) + ((r * 5) & 15) * 64 + lane * 4);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[u][0]), finite_abs(v[u][1])), fmaxf(finite_abs(v[u][2]), finite_abs(v[u][3]))));
+    }
   } else {
     int64_t lo = 0;
     if ((((uintptr_t)w) & 15) == 0) {
@@ -135,14 +153,21 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
 // workgroups [0, bx): x (zeros for the rows that are not counted), [bx, bx + bw): W, the last one: the number of counted rows.  A
 // wave takes 512 consecutive cells of the padded array at a time, eight a lane; where rows do not begin on 16 bytes it reads them
 // lane by lane and turns them in LDS.
+//
+// `sample`: W's scale came from a sixteenth of it.  It leaves the largest element seen a factor of four below the largest fp16
+// number; larger ones are found on the way.  Should there be any (AGAIN: this kernel's second launch, for W alone,
+// which otherwise ends at once), W is converted once more with the scale that it asks for.
+constexpr float kHalfMax = 65504.0f;
+template <bool AGAIN>
 __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict__ x, int64_t rows, int64_t width,
                                                         const float* __restrict__ w, int64_t classes, char* __restrict__ xs,
                                                         char* __restrict__ ws, const float* __restrict__ target, float ignore,
-                                                        int mean, int64_t bx, int64_t bw, Ctl* __restrict__ ctl) {
+                                                        int mean, int64_t bx, int64_t bw, int sample, Ctl* __restrict__ ctl) {
   __shared__ float sh[kThreads / 64];
   __shared__ int shi[kThreads / 64];
   __shared__ __attribute__((aligned(16))) float turn[kThreads / 64][512];
-  if (blockIdx.x == bx + bw) {
+  if (AGAIN && ctl->found == 0) return;
+  if (!AGAIN && blockIdx.x == bx + bw) {
     int n = 0;
 #pragma unroll 8
     for (int64_t i = threadIdx.x; i < rows; i += kThreads) n += target[i] != ignore ? 1 : 0;
@@ -153,11 +178,16 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   const bool second = blockIdx.x >= bx;
   const float* part = second ? ctl->max_w : ctl->max_x;
   float m = 0.0f;
+  if (AGAIN) {
+    m = __uint_as_float(ctl->found);
+  } else {
 #pragma unroll
-  for (int u = 0; u < kScan / kThreads; u++) m = fmaxf(m, part[threadIdx.x + u * kThreads]);
-  m = block_reduce<kThreads>(m, sh, Max());
+    for (int u = 0; u < kScan / kThreads; u++) m = fmaxf(m, part[threadIdx.x + u * kThreads]);
+    m = block_reduce<kThreads>(m, sh, Max());
+  }
   const int e = m > 0.0f ? ilogbf(m) - kTop : 0;
   if (threadIdx.x == 0 && blockIdx.x == (second ? bx : 0)) (second ? ctl->ew : ctl->ex) = e;
+  float largest = 0.0f;
   const float* src = second ? w : x;
   char* dst = second ? ws : xs;
   const int64_t nr = second ? width : rows, nc = second ? classes : width;
@@ -193,6 +223,9 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
       for (int k = 0; k < 8; k++) v[k] = turn[wave][lane * 8 + k];
     }
     const bool out = !second && r < nr && target[r] == ignore;
+    if (!AGAIN && sample && second)
+#pragma unroll
+      for (int k = 0; k < 8; k++) largest = fmaxf(largest, finite_abs(v[k]));
     half8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -203,6 +236,11 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
     char* d = dst + r * pc * 4 + (c >> 5) * 128 + (c & 31) * 2;
     *reinterpret_cast<half8*>(d) = hi;
     *reinterpret_cast<half8*>(d + 64) = lo;
+  }
+  if (!AGAIN && sample && second) {
+    largest = block_reduce<kThreads>(largest, sh, Max());
+    // (a largest value: the order does not matter.  Only those that count: 4 096 of these are 33 us)
+    if (threadIdx.x == 0 && ldexpf(largest, -e) > kHalfMax) atomicMax(&ctl->found, __float_as_uint(largest));
   }
 }
 
@@ -808,13 +846,19 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   ProfScope prof("linear_ce", (grads ? 6.0 : 2.0) * (double)rows * (double)width * (double)classes,
                  4.0 * (grads ? 2.0 : 1.0) * ((double)rows * width + (double)width * classes));
 
-  DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows, width, target, ignore, w,
-            width * classes, ctl);
+  const int sample = width * classes >= kSampled;
+  DF_LAUNCH(k_lce_scan, dim3(2 * kScan), dim3(kThreads), 0, stream(), x, rows, width, target, ignore, w, width * classes, sample,
+            ctl);
   DF_LAUNCH_CHECK();
   const int64_t bx = std::min<int64_t>(np * dp / 2048, 2048), bw = std::min<int64_t>(dp * vp / 2048, 4096);
-  DF_LAUNCH(k_lce_split, dim3((unsigned)(bx + bw + 1)), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p,
-            (char*)ws.p, target, ignore, mean, bx, bw, ctl);
+  DF_LAUNCH((k_lce_split<false>), dim3((unsigned)(bx + bw + 1)), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p,
+            (char*)ws.p, target, ignore, mean, bx, bw, sample, ctl);
   DF_LAUNCH_CHECK();
+  if (sample) {
+    DF_LAUNCH((k_lce_split<true>), dim3(1024), dim3(kThreads), 0, stream(), x, rows, width, w, classes, (char*)xs.p, (char*)ws.p,
+              target, ignore, mean, (int64_t)0, (int64_t)1024, sample, ctl);
+    DF_LAUNCH_CHECK();
+  }
 
   for (int64_t r0 = 0; r0 < rows; r0 += piece) {
     const int64_t n = std::min(piece, rows - r0);

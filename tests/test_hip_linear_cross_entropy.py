@@ -298,6 +298,15 @@ def test_operands_of_any_magnitude(hip_device, sx, sw):
     _check(hip_device, (x * np.float32(sx)), (w * np.float32(sw)), b, t)
 
 
+@pytest.mark.parametrize("factor", [1.0, 3.0, 300.0, 1e6])
+@pytest.mark.parametrize("place", [0, 1, 5 * 64 + 1024, 16777215])
+def test_a_large_weight_whose_largest_element_is_one_of_many(hip_device, factor, place):
+    """16.8 M weights, whose scale is found from a sample: single elements that it holds, or does not, far above the others"""
+    x, w, b, t = _data(140, 512, 32769, 32)
+    w.reshape(-1)[place] = np.abs(w).max() * np.float32(factor)
+    _check(hip_device, x, w, b, t)
+
+
 def test_large_logits(hip_device):
     """probabilities of 0 and 1 to the last bit"""
     x, w, b, t = _data(64, 50, 400, 14)
