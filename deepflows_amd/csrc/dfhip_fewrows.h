@@ -1,9 +1,9 @@
-// fp32 products of FEW rows (64 a workgroup) with a large matrix W on the fp32 matrix cores.
+// fp32 products of FEW rows (at most 64) with a large matrix W on the fp32 matrix cores.
 //
 // What bounds them is reading W, or writing a gradient of its size: 32 rows are 64 operations for the 4 bytes of an element, and
 // the fp32 matrix cores form 121 in the time that HBM takes for them (153 TFLOP/s, 5.07 TB/s).  So W is read as it is, once a
-// product, into the matrix operands: the split products (dfhip_splitgemm.h) read W to find its scale, read and write it to convert
-// it and read it again, 16 bytes an element instead of 4.
+// product, into the matrix operands: the split products (dfhip_splitgemm.h) read and write it to convert it and read it again, 12
+// bytes an element instead of 4 (16 where they read all of it for its scale).
 //
 // 32 x 32 x 2 MFMA; the order of the reduction is free, so a lane's operands are 16-byte pieces of memory:
 //   rows' side       lane (i, h): four elements of row i from k + 4 h: element s belongs to product s, which takes k + s and k + 4 + s
@@ -19,7 +19,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));      // rows of any width begin on any element
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kMost = 64;                          // rows of a workgroup
+constexpr int kMost = 64;                          // rows
 
 // rows x n outputs over kn; `a` (rows, lda), `b` (kn, ldb), along: (n, ldb)
 struct Product {

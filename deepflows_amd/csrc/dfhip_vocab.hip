@@ -18,9 +18,9 @@
 //   without gradients: the product's epilogue leaves what the softmax needs of every 64 logits and the targets' (none is stored),
 //                  k_few_rows joins them, k_lce_loss
 //
-// Measured.  8192 x 1024 x 50001 with gradients, 6.65 ms: logits 2.08 ms and the pair 3.85 ms, 1.21 and 1.31 PFLOP/s of fp16 (the
+// Measured.  8192 x 1024 x 50001 with gradients, 6.6 ms: logits 2.08 ms and the pair 3.85 ms, 1.21 and 1.31 PFLOP/s of fp16 (the
 // library's 8192^3 fp16 product: 1.18; at that rate the three products alone are 6.42 ms, in fp32 16.4), rows 0.68 ms (3.3 GB, 4.8
-// TB/s), conversion 0.13.  2048 x 768 x 32000: 0.90 ms; 509 x 512 x 10007: 89 us; 1500 x 1024 x 30011, the loss alone: 361 us.
+// TB/s), conversion 0.09.  2048 x 768 x 32000: 0.89 ms; 509 x 512 x 10007: 86 us; 1500 x 1024 x 30011, the loss alone: 0.30 ms.
 // Largest error of any result against 64 bits, relative to the result's largest value: 1.8e-6 at 8192 x 1024 x 50001, where the
 // fp32 composition (library products) has 5.4e-6; 7e-7 and 4.3e-6 at 2048 x 768 x 32000.
 #include <math.h>
@@ -432,20 +432,14 @@ struct Few {
 template <int RB, int CF, int NW>
 __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
   __shared__ dfhip_few::f32x4 lds[dfhip_few::lds_pieces<CF, NW>()];
-  // (64 rows a workgroup; a tile's workgroups eight numbers apart, on the same XCD, where W comes out of the L2 for the second)
-  const int sets = (g.logits.rows + 63) >> 6, block = (int)blockIdx.x;
-  const int tile = (block >> 3) / sets * 8 + (block & 7), row0 = (block >> 3) % sets * 64, n0 = tile * 32 * CF, i = threadIdx.x & 31;
-  if (tile >= g.tiles) return;
-  dfhip_few::Product p = g.logits;
-  p.a += (int64_t)row0 * p.lda;
-  p.rows = min(p.rows - row0, 64);
+  const dfhip_few::Product& p = g.logits;
+  const int tile = (int)blockIdx.x, n0 = tile * 32 * CF, i = threadIdx.x & 31;
   const int c = n0 + CF * i, over = c - min(c, p.n - CF);  // columns by which this lane's loads were moved back
   float bias[CF];
 #pragma unroll
   for (int f = 0; f < CF; f++) bias[f] = g.bias && c + f < p.n ? g.bias[c + f] : 0.0f;
   dfhip_few::across<RB, CF, NW>(p, n0, lds, [&](int row, const float* v) {
     if (row >= p.rows) return;                             // (uniform in the half wave)
-    row += row0;
     float w[CF];                                           // -inf behind the last class
 #pragma unroll
     for (int f = 0; f < CF; f++) {
@@ -459,7 +453,7 @@ __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
 #pragma unroll
     for (int f = 0; f < CF; f++) in[f] = c + f < p.n;
     const RowPart part = row_part<CF, 32>(w, in, g.smooth > 0.0f);
-    if (i == 0) store_part(g.stat + (int64_t)row * g.tiles + tile, (int64_t)g.logits.rows * g.tiles, part);
+    if (i == 0) store_part(g.stat + (int64_t)row * g.tiles + tile, (int64_t)p.rows * g.tiles, part);
   });
 }
 
@@ -696,21 +690,20 @@ int rows_pass(float* logits, const float* target, int n, int launch_rows, float*
 }
 
 // Which calls go this way (measured, microseconds, this way / the split products):
-//   up to 32 rows: all.  loss and gradients, 32 rows: 256 x 1000 21 / 23, 1024 x 16384 65 / 93, 1024 x 50001 180 / 331,
-//     2048 x 99991 691 / 1275; the loss alone: 13 / 18, 27 / 54, 54 / 179, 199 / 670
+//   up to 32 rows: all.  loss and gradients, 32 rows: 256 x 1000 21 / 23, 1024 x 16384 65 / 93, 1024 x 50001 180 / 284,
+//     2048 x 99991 691 / 1137; the loss alone: 13 / 18, 27 / 54, 54 / 140, 199 / 540
 //   33 to 64 rows, where the fp32 matrix cores begin to count: the loss alone from 3 M elements of W (64 rows: 2048 x 1000 34 / 26,
-//     64 x 50001 23 / 40, 1024 x 16384 40 / 54, 1024 x 50001 87 / 179), with gradients from 32 M (1024 x 16384 103 / 91,
-//     1024 x 50001 279 / 319, 2048 x 99991 1066 / 1267)
-//   65 to 128 rows: the loss alone from 32 M (128 rows: 1024 x 34001 124 / 130, 1024 x 50001 157 / 181, 2048 x 99991 505 / 688)
+//     64 x 50001 23 / 36, 1024 x 5003 25 / 34, 1024 x 50001 85 / 139), with gradients from 48 M (1024 x 34001 220 / 196,
+//     1024 x 50001 277 / 284, 2048 x 50001 513 / 584)
+//   more rows would be as fast at best (128, the loss alone: 1024 x 34001 119 / 104, 1024 x 50001 151 / 139, 2048 x 99991 496 / 546)
 inline bool few_rows(int64_t rows, int64_t width, int64_t classes, bool grads) {
-  if (classes < 4 || rows > (grads ? 1 : 2) * dfhip_few::kMost) return false;
-  if (rows > dfhip_few::kMost) return width * classes >= (int64_t)32 << 20;
-  return rows <= 32 || width * classes >= (grads ? (int64_t)32 << 20 : (int64_t)3 << 20);
+  if (classes < 4 || rows > dfhip_few::kMost) return false;
+  return rows <= 32 || width * classes >= (grads ? (int64_t)48 << 20 : (int64_t)3 << 20);
 }
 
 template <int RB>
 int few_logits(const Few& g) {
-  const dim3 grid((unsigned)(df_ceil_div(g.tiles, 8) * 8 * df_ceil_div(g.logits.rows, 64)));
+  const dim3 grid((unsigned)g.tiles);
   if (g.cols == 32) DF_LAUNCH((k_few_logits<RB, 1, 8>), grid, dim3(512), 0, stream(), g);
   else DF_LAUNCH((k_few_logits<RB, 4, 4>), grid, dim3(256), 0, stream(), g);
   DF_LAUNCH_CHECK();

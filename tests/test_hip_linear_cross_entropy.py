@@ -129,8 +129,9 @@ def test_few_rows(hip_device, N, D, V):
     _check(hip_device, *_data(N, D, V, N + D + V, ignored=0.2 if N > 4 else 0.0, bias=D % 2 == 1), label_smoothing=0.1 if V % 2 else 0.0)
 
 
-def test_33_to_64_rows_of_a_large_product(hip_device):
-    _check(hip_device, *_data(45, 700, 48001, 25, ignored=0.1), label_smoothing=0.1)
+@pytest.mark.parametrize("D", [700, 1100])
+def test_33_to_64_rows_of_a_large_product(hip_device, D):
+    _check(hip_device, *_data(45, D, 48001, 25, ignored=0.1), label_smoothing=0.1)
 
 
 @pytest.mark.parametrize("N,D,V", [(1, 90, 700), (40, 65, 50001), (64, 700, 5001), (30, 40, 33001), (100, 700, 48001),
