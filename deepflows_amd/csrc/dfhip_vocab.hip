@@ -38,7 +38,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kScan = 512;                                 // workgroups (= partial maxima) a tensor
-constexpr int64_t kSampled = (int64_t)16 << 20;            // from this many elements of W on its scale comes from a sample
+// From this many elements of W on its scale comes from a sample: at 1024 x 16384 the full scan is 11.6 us, the sample 4.6 and the
+// launch that looks whether it was enough 4.8; at 1024 x 50001 41 and 5.4 + 4.9.
+constexpr int64_t kSampled = (int64_t)16 << 20;
 constexpr int64_t kPieceBytes = (int64_t)2 << 30;          // the logits of one piece of the rows
 
 // what the launches of one call hand to each other
