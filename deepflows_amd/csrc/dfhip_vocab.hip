@@ -41,7 +41,8 @@ constexpr int kScan = 512;                                 // workgroups (= part
 // From this many elements of W on its scale comes from a sample: at 1024 x 16384 the full scan is 11.6 us, the sample 4.6 and the
 // launch that looks whether it was enough 4.8; at 1024 x 50001 41 and 5.4 + 4.9.
 constexpr int64_t kSampled = (int64_t)16 << 20;
-constexpr int64_t kPieceBytes = (int64_t)2 << 30;          // the logits of one piece of the rows
+constexpr int64_t kPieceBytes = (int64_t)2 << 30;          // the logits (or the softmax's parts) of one piece of the rows
+constexpr int64_t kPieceRows = 1 << 22;                    // a workgroup a row: 2^32 threads a launch are too many
 
 // what the launches of one call hand to each other
 struct Ctl {
@@ -826,7 +827,8 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
   const int64_t np = padded(rows), dp = padded(width), vp = padded(classes);
   // pieces of about the same length, a multiple of 256 rows
   const int64_t row_bytes = grads ? 4 * vp : 12 * df_ceil_div(classes, 32);
-  const int64_t cap = std::max<int64_t>(256, kPieceBytes / row_bytes / 256 * 256), pieces = df_ceil_div(rows, cap);
+  const int64_t cap = std::min<int64_t>(kPieceRows, std::max<int64_t>(256, kPieceBytes / row_bytes / 256 * 256));
+  const int64_t pieces = df_ceil_div(rows, cap);
   const int64_t piece = padded(df_ceil_div(rows, pieces));
   Held xs, ws, logits, small, parts;
   int64_t held = 0;
