@@ -32,14 +32,13 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, grad_scale=1.0, error_i
     seen, live, grads = set(), [], []
     for p in params:
         g = p.grad
-        if g is None or id(p) in seen:
-            continue
-        seen.add(id(p))
-        live.append(p)
-        grads.append((g.data if isinstance(g, Tensor) else g).compact())
-    device = grads[0].device if grads else (params[0].device if params else backend_api.default_device())
+        if g is not None and id(p) not in seen:
+            seen.add(id(p))
+            live.append(p)
+            grads.append((g.data if isinstance(g, Tensor) else g).compact())
+    device = grads[0]._device if grads else (params[0].device if params else backend_api.default_device())
     for g in grads:
-        if g.device != device:
+        if g._device is not device and g._device != device:
             raise ValueError("clip_grad_norm_: the gradients are on different devices")
     mod = device.mod
     if error_if_nonfinite and getattr(mod, "capturing", False):
@@ -47,17 +46,19 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, grad_scale=1.0, error_i
     if not hasattr(mod, "clip_grad_norm"):
         return _primitive(live, grads, device, max_norm, norm_type, grad_scale, error_if_nonfinite)
     norm = BackendTensor.make((1,), device=device)
-    places, end = [], 0
-    for g in grads:
-        places.append(end)
-        end += -(-g._handle.size // _ALIGN) * _ALIGN
-    flat = mod.Array(end)
-    outs = [_ArrayView(flat, at, g._handle.size) for at, g in zip(places, grads)]
-    mod.clip_grad_norm([g._handle for g in grads], outs, norm._handle, max_norm, norm_type == math.inf, grad_scale)
+    handles = [g._handle for g in grads]
+    sizes = [h.size for h in handles]
+    flat = mod.Array(sum([-(-n // _ALIGN) for n in sizes]) * _ALIGN)
+    outs, at = [], 0
+    for n in sizes:
+        outs.append(_ArrayView(flat, at, n))
+        at += -(-n // _ALIGN) * _ALIGN
+    mod.clip_grad_norm(handles, outs, norm._handle, max_norm, norm_type == math.inf, grad_scale)
     if error_if_nonfinite:
         _refuse_nonfinite(float(norm.numpy()[0]))
     for p, g, out in zip(live, grads, outs):
-        p.grad = _like(p.grad, BackendTensor.make(g.shape, device=device, handle=out))
+        new = BackendTensor.make(g._shape, g._strides, device, out)      # (compact, as g is)
+        p.grad = Tensor(new) if isinstance(p.grad, Tensor) else new
     return Tensor(norm)
 
 
