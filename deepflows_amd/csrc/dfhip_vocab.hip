@@ -695,13 +695,16 @@ int rows_pass(float* logits, const float* target, int n, int launch_rows, float*
 // Which calls go this way (measured, microseconds, this way / the split products):
 //   up to 32 rows: all.  loss and gradients, 32 rows: 256 x 1000 21 / 23, 1024 x 16384 65 / 93, 1024 x 50001 180 / 284,
 //     2048 x 99991 691 / 1137; the loss alone: 13 / 18, 27 / 54, 54 / 140, 199 / 540
-//   33 to 64 rows, where the fp32 matrix cores begin to count: the loss alone from 3 M elements of W (64 rows: 2048 x 1000 34 / 26,
-//     64 x 50001 23 / 36, 1024 x 5003 25 / 34, 1024 x 50001 85 / 139), with gradients from 48 M (1024 x 34001 220 / 196,
-//     1024 x 50001 277 / 284, 2048 x 50001 513 / 584)
+//   33 to 64 rows, where the fp32 matrix cores begin to count: the loss alone where the reduction is short or W large (64 rows:
+//     256 x 1000 15 / 18, 1024 x 1000 22 / 22, 2048 x 1000 34 / 26, 1024 x 5003 25 / 34, 1024 x 50001 85 / 139); with gradients
+//     where W is very large (1024 x 34001 220 / 196, 1024 x 50001 277 / 284, 2048 x 50001 513 / 584), and where the launches are
+//     what counts, four instead of six (100 x 500 22 / 21, 256 x 1000 24.5 / 24, 512 x 2000 28.6 / 29.5, 64 x 50001 52 / 61, but
+//     1024 x 1000 34 / 31, 256 x 16384 47 / 45; the host, where it is slower than the device, saves 5 us of 38)
 //   more rows would be as fast at best (128, the loss alone: 1024 x 34001 119 / 104, 1024 x 50001 151 / 139, 2048 x 99991 496 / 546)
 inline bool few_rows(int64_t rows, int64_t width, int64_t classes, bool grads) {
   if (classes < 4 || rows > dfhip_few::kMost) return false;
-  return rows <= 32 || width * classes >= (grads ? (int64_t)48 << 20 : (int64_t)3 << 20);
+  const int64_t size = width * classes, M = 1 << 20;
+  return rows <= 32 || (grads ? size >= 48 * M || (width <= 512 && size <= 7 * M / 2) : size >= 3 * M || width <= 1024);
 }
 
 template <int RB>
@@ -718,9 +721,9 @@ int few_rows_forward(const float* x, const float* w, const float* bias, const fl
   const bool grads = dx || dw || db;
   const int64_t ld = df_ceil_div(classes, 128) * 128;
   const int cols = df_ceil_div(classes, 128) < num_cus() ? 32 : 128, tiles = (int)df_ceil_div(classes, cols);
-  // dx: about two workgroups a CU, two windows each at least; at most 256 parts
-  const int dx_tiles = (int)df_ceil_div(width, 128);
-  int cuts = std::max(1, std::min(std::min(256, 2 * num_cus() / dx_tiles), (int)df_ceil_div(classes, 2 * dfhip_few::kWindow)));
+  // dx: about two workgroups a CU, at most 256 parts; two windows each at least, one where that makes less than 32 of them
+  const int dx_tiles = (int)df_ceil_div(width, 128), windows = (int)df_ceil_div(classes, dfhip_few::kWindow);
+  int cuts = std::max(1, std::min(std::min(256, 2 * num_cus() / dx_tiles), std::max((windows + 1) / 2, std::min(windows, 32))));
   const int cut = (int)df_ceil_div(df_ceil_div(classes, cuts), dfhip_few::kWindow) * dfhip_few::kWindow;
   cuts = (int)df_ceil_div(classes, cut);
   Held logits, small, parts;

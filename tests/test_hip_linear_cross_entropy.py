@@ -121,7 +121,7 @@ def test_smoothing_reductions_and_rows_that_are_not_counted(hip_device, reductio
 # few rows go another way (the fp32 matrix cores, W as it is): one to 64 rows, 32- and 128-column tiles, classes and widths that
 # end inside a tile, a step, a window
 FEW = [(1, 8, 4), (1, 300, 1003), (2, 7, 5), (5, 37, 33), (8, 64, 127), (9, 65, 129), (20, 129, 1000), (32, 8, 4097), (32, 515, 700),
-       (3, 16, 32641), (17, 45, 33003), (32, 130, 50001), (1, 2100, 32770)]
+       (33, 100, 500), (64, 256, 1000), (50, 70, 4), (64, 512, 2001), (47, 33, 50001), (3, 16, 32641), (17, 45, 33003), (32, 130, 50001), (1, 2100, 32770)]
 
 
 @pytest.mark.parametrize("N,D,V", FEW)
