@@ -21,6 +21,12 @@ from .optim.clip import clip_grad_norm_
 from .tensor import Graph
 
 
+def _checked_norm(max_grad_norm):
+    if max_grad_norm is not None and not max_grad_norm >= 0.0:
+        raise ValueError(f"max_grad_norm must be None or >= 0, got {max_grad_norm}")
+    return max_grad_norm
+
+
 class CapturedTrainStep:
     """forward + loss + zero_grad + backward (+ optimizer update) captured on `inputs`'s device.
     `inputs` / `targets` are device tensors whose buffers the graph reads on every replay (refill
@@ -42,7 +48,7 @@ class CapturedTrainStep:
         max_grad_norm: every step's gradients are scaled down to this common norm (optim.clip_grad_norm_) between the exchange and
         the optimizer, inside the graph where the optimizer is; `grad_norm` then holds the norm of the last step's."""
         self.S = int(steps_per_graph)
-        self.max_grad_norm, self.grad_norm = max_grad_norm, None
+        self.max_grad_norm, self.grad_norm = _checked_norm(max_grad_norm), None
         self._clip_scale = optimizer.grad_scale
         self._phase = 0
         if self.S not in (1, 2, 4, 8) or (self.S > 1 and sync is not None):
@@ -170,7 +176,7 @@ class OverlappedCapturedTrainStep:
     halves of optimizer.params (workloads.late_and_early_parameters)."""
 
     def __init__(self, model, criterion, optimizer, inputs, targets, late_bucket, early_bucket, max_grad_norm=None):
-        self.max_grad_norm = max_grad_norm          # None, or the largest common norm of a step's gradients (optim.clip_grad_norm_)
+        self.max_grad_norm = _checked_norm(max_grad_norm)      # None, or the largest common norm of a step's gradients
         mod = inputs.device.mod
         if not (getattr(mod, "fused", False) and hasattr(mod, "capture_begin")):
             raise RuntimeError("OverlappedCapturedTrainStep needs the hip device")

@@ -482,6 +482,41 @@ def test_inside_a_captured_graph(hip_device):
     Graph.free_graph_all()
 
 
+def test_a_captured_large_weight_whose_scale_moves(hip_device):
+    """replays over weights that need the second conversion, and again over ones that do not"""
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    mod = hip_device.mod
+    x, w, b, t = _data(70, 512, 32801, 33)
+    leaves = [Tensor(a, device=hip_device, requires_grad=True) for a in (x, w, b)]
+    tt = Tensor(t, device=hip_device)
+
+    def step():
+        for p in leaves:
+            p.grad = None
+        loss = F.linear_cross_entropy(*leaves, tt)
+        loss.backward()
+        return [loss.data] + [p.grad for p in leaves]
+
+    step()
+    mod.capture_begin()
+    got = step()
+    graph = mod.capture_end(keep=got)
+    for factor in (1.0, 1000.0, 1.0, 50.0):
+        v = w.copy()
+        v[3, 777] = np.abs(w).max() * np.float32(factor)
+        mod.from_numpy(v, leaves[1].data._handle)
+        graph.replay()
+        replayed = [g.numpy().copy() for g in got]
+        for a, c in zip(replayed, step()):
+            assert np.array_equal(a, c.numpy())
+        ref = _reference(x, v, b, t)
+        _within(float(replayed[0][0]), ref[0][0], ref[0][1], "loss")
+        _within(replayed[1], ref[1][0], ref[1][1], "dx")
+    graph.destroy()
+    Graph.free_graph_all()
+
+
 def test_refusals(hip_device):
     from deepflows_amd.nn import functional as F
     from deepflows_amd.tensor import Tensor

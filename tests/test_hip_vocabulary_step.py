@@ -230,6 +230,63 @@ def test_the_epoch_loop_clips(hip_device):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("inside", [True, False])
+def test_a_captured_step_clips_behind_the_exchange(hip_device, inside):
+    """the gradients of a bucket, clipped in the captured graph or eagerly behind its replays: the eager steps' parameters"""
+    from deepflows_amd import optim, parallel, workloads
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+
+    class Doubling(parallel.Communicator):
+        exchanges, world = True, 2
+
+        def allreduce_sum(self, flat, overlap=False):
+            flat.device.mod.axpy(flat._handle, (flat * 1.0)._handle, 1.0)
+            return flat
+
+    batches, runs = _batches(4, 30), []
+    for captured in (False, True):
+        net, crit, params = _build(hip_device)
+        opt = optim.SGD(params, lr=0.3, momentum=0.9)
+        opt.grad_scale = 0.5
+        bucket = parallel.GradientBucket(opt.params, Doubling())
+        x, t = (Tensor(a, device=hip_device) for a in batches[0])
+        step = None
+        if captured:
+            step = CapturedTrainStep(net, crit, opt, x, t, sync=bucket.sync, capture_exchange=inside, max_grad_norm=0.2)
+            assert step.exchange_captured == inside
+        norms = []
+        for bx, bt in batches:
+            hip_device.mod.from_numpy(bx, x.data._handle)
+            hip_device.mod.from_numpy(bt, t.data._handle)
+            if captured:
+                step.replay()
+                norms.append(float(step.grad_norm.numpy()[0]))
+            else:
+                workloads.train_step(net, crit, opt, x, t, sync=bucket.sync, max_grad_norm=0.2)
+                Graph.free_graph()
+        assert all(n > 0.2 for n in norms)
+        runs.append([p.numpy().copy() for p in params])
+        if step is not None:
+            step.destroy()
+        bucket.release()
+        Graph.free_graph_all()
+    for a, b in zip(*runs):
+        assert np.array_equal(a, b)
+
+
+def test_a_negative_norm_is_refused_before_anything_is_captured(hip_device):
+    from deepflows_amd import optim
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+    net, crit, params = _build(hip_device)
+    x, t = (Tensor(a, device=hip_device) for a in _batches(1, 8)[0])
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError):
+            CapturedTrainStep(net, crit, optim.SGD(params, lr=0.1), x, t, max_grad_norm=bad)
+    Graph.free_graph_all()
+
+
 def test_the_overlapped_exchange_clips(hip_device):
     """both halves of the gradients on their way when the clipping begins: the eager step's parameters, bit for bit.  (One rank
     without a collective: what is checked is that the clipping sees the gradients of both graphs.)"""
