@@ -10,9 +10,7 @@ Three operators, each with its gradient where it has one:
 functions; `exact` computes it in 64 bits from the definitions.  Everything is fp32, the framework's only type; class indices
 come as the whole numbers a 32-bit float holds exactly, as every array of the framework does.
 """
-import functools
 import math
-import types
 
 import torch
 
@@ -249,87 +247,83 @@ class _Results(list):
         return (torch.as_tensor(_Shown(a), device="cuda") for a in list.__iter__(self))
 
 
-@functools.lru_cache(maxsize=None)
-def _package():
-    """the package and two nodes of the tape that stand for the rest of a network: they take y (and h) in and hand given
-    gradients back"""
-    import deepflows_amd
-    from deepflows_amd import tensor
-    from deepflows_amd.autograd import no_grad
-    from deepflows_amd.backend_selection import BackendTensor
-    from deepflows_amd.nn import functional
-
-    class One(tensor.UnaryOperator):
-        def __init__(self, y, dy):
-            self.dy = dy
-            super().__init__(y)
-
-        def forward(self, x):
-            return BackendTensor.make((1,), device=x.device)
-
-        def grad_fn(self, node, grad):
-            return self.dy
-
-    class Two(tensor.BinaryOperator):
-        def __init__(self, y, h, dy, dh):
-            self.dy, self.dh = dy, dh
-            super().__init__(y, h)
-
-        def forward(self, x, y):
-            return BackendTensor.make((1,), device=x.device)
-
-        def grad_fn(self, node, grad):
-            return self.dy if node is self.parents[0] else self.dh
-
-    return types.SimpleNamespace(Tensor=tensor.Tensor, Graph=tensor.Graph, BackendTensor=BackendTensor, no_grad=no_grad,
-                                 F=functional, nn=deepflows_amd.nn, optim=deepflows_amd.optim,
-                                 device=deepflows_amd.backend_api.Device("hip"), One=One, Two=Two)
-
-
 def _array(t):
-    t, d = t.contiguous(), _package()
-    return d.BackendTensor.make(tuple(t.shape), device=d.device, handle=_Shared(t))
+    from deepflows_amd import backend_api
+    from deepflows_amd.backend_selection import BackendTensor
+    t = t.contiguous()
+    return BackendTensor.make(tuple(t.shape), device=backend_api.Device("hip"), handle=_Shared(t))
 
 
 def _parameters(grads):
-    d = _package()
-    return [d.nn.Parameter(d.Tensor(g)) for g in grads]
+    from deepflows_amd import nn
+    from deepflows_amd.tensor import Tensor
+    return [nn.Parameter(Tensor(g)) for g in grads]
 
 
 def _leaf(a, train):
-    return _package().Tensor(a, device=a.device, requires_grad=train) if a is not None else None
+    from deepflows_amd.tensor import Tensor
+    return Tensor(a, device=a.device, requires_grad=train) if a is not None else None
 
 
 def _own_loss(case, s):
-    d, train = _package(), case["train"]
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph
+    train = case["train"]
     x, w, b, t = _leaf(s["x"], train), _leaf(s["w"], train), _leaf(s.get("b"), train), _leaf(s["target"], False)
     if not train:
-        with d.no_grad():
-            return _Results([d.F.linear_cross_entropy(x, w, b, t, label_smoothing=case["smoothing"]).data])
-    loss = d.F.linear_cross_entropy(x, w, b, t, label_smoothing=case["smoothing"])
+        with no_grad():
+            return _Results([F.linear_cross_entropy(x, w, b, t, label_smoothing=case["smoothing"]).data])
+    loss = F.linear_cross_entropy(x, w, b, t, label_smoothing=case["smoothing"])
     loss.backward()
-    d.Graph.free_graph_all()
+    Graph.free_graph_all()
     return _Results([loss.data] + [p.grad for p in (x, w, b) if p is not None])
 
 
 def _own_norm(case, s):
-    d, train = _package(), case["train"]
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph
+    train = case["train"]
     x, w, r = _leaf(s["x"], train), _leaf(s["w"], train), _leaf(s.get("r"), train)
     if not train:
-        with d.no_grad():
-            y = d.F.rms_norm(x, w, NORM_EPS, residual=r)
+        with no_grad():
+            y = F.rms_norm(x, w, NORM_EPS, residual=r)
         return _Results([y.data] if r is None else [v.data for v in y])
-    y = d.F.rms_norm(x, w, NORM_EPS, residual=r)
+    y = F.rms_norm(x, w, NORM_EPS, residual=r)
     y, h = y if r is not None else (y, None)
-    (d.One(y, s["dy"]) if h is None else d.Two(y, h, s["dy"], s["dh"])).backward()
-    d.Graph.free_graph_all()
+    _rest(y, h, s["dy"], s.get("dh")).backward()
+    Graph.free_graph_all()
     return _Results([y.data] + ([h.data] if h is not None else []) + [x.grad, w.grad])
 
 
+def _rest(y, h, dy, dh):
+    """the rest of a network: a node of the tape that takes y (and h) in and hands the given gradients back"""
+    from deepflows_amd.backend_selection import BackendTensor
+    from deepflows_amd import tensor
+
+    class One(tensor.UnaryOperator):
+        def forward(self, x):
+            return BackendTensor.make((1,), device=x.device)
+
+        def grad_fn(self, node, grad):
+            return dy
+
+    class Two(tensor.BinaryOperator):
+        def forward(self, x, y):
+            return BackendTensor.make((1,), device=x.device)
+
+        def grad_fn(self, node, grad):
+            return dy if node is self.parents[0] else dh
+
+    return One(y) if h is None else Two(y, h)
+
+
 def _own_clip(case, s):
+    from deepflows_amd import optim
     for p, g in zip(s["params"], s["grads"]):
         p.grad = g
-    total = _package().optim.clip_grad_norm_(s["params"], case["max_norm"], norm_type=float(case["kind"]))
+    total = optim.clip_grad_norm_(s["params"], case["max_norm"], norm_type=float(case["kind"]))
     return _Results([total.data] + [p.grad for p in s["params"]])
 
 
