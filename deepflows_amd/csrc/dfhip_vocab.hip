@@ -48,7 +48,7 @@ constexpr int64_t kPieceRows = 1 << 22;                    // a workgroup a row:
 struct Ctl {
   float scale;                                             // 1 / number of counted rows, or 1
   int ex, ew;                                              // x = 2^ex * split array, W likewise
-  unsigned found;                                          // 0, or W's largest finite magnitude where a sample missed it
+  unsigned found;                                          // 0, or W's largest finite magnitude where a sample's scale does not hold it
   float max_x[kScan], max_w[kScan];
 };
 
@@ -81,7 +81,7 @@ __device__ __forceinline__ float finite_abs(const float4& v) {
 
 // workgroups 0 .. kScan-1: x, kScan .. 2 kScan - 1: W.  The rows of x that are not counted are passed over: padding may hold
 // anything, and a large value in it would cost the counted rows their low bits.  `sample`: of W every sixteenth piece of 64 elements
-// is read, another one in every row of pieces; the conversion finds out whether that was enough.
+// is read; the conversion finds out whether that was enough.
 __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__ x, int64_t rows, int64_t width,
                                                        const float* __restrict__ target, float ignore,
                                                        const float* __restrict__ w, int64_t nw, int sample, Ctl* __restrict__ ctl) {
@@ -116,7 +116,9 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
       m = t == ignore ? m : fmaxf(m, s);
     }
   } else if (sample) {
-    // (64 elements of 1 024: their place moves on from one to the next, or all would lie on the same few memory channels)
+    // (64 elements of 1 024, their place among them by a multiplicative hash of the run's number: at one place all would lie on the
+    // same few memory channels, and a place that follows the number's last bits repeats from row to row of W where the number of
+    // classes is a multiple of 16 384)
     const int64_t runs = nw >> 10, step = kScan * (kThreads / 16);
     const int lane = threadIdx.x & 15;
     int64_t i = (int64_t)blk * (kThreads / 16) + (threadIdx.x >> 4);
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const int64_t r = min(i + u * step, runs - 1);
-        v[u] = *reinterpret_cast<const dfhip_few::f32x4u*>(w + (r << 10) + ((r * 5) & 15) * 64 + lane * 4);
+        v[u] = *reinterpret_cast<const dfhip_few::f32x4u*>(w + (r << 10) + (((unsigned)r * 2654435769u) >> 28) * 64 + lane * 4);
       }
 #pragma unroll
       for (int u = 0; u < 4; u++) m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[u][0]), finite_abs(v[u][1])), fmaxf(finite_abs(v[u][2]), finite_abs(v[u][3]))));
@@ -158,8 +160,9 @@ __global__ __launch_bounds__(kThreads) void k_lce_scan(const float* __restrict__
 // lane by lane and turns them in LDS.
 //
 // `sample`: W's scale came from a sixteenth of it.  It leaves the largest element seen a factor of four below the largest fp16
-// number; larger ones are found on the way.  Should there be any (AGAIN: this kernel's second launch, for W alone,
-// which otherwise ends at once), W is converted once more with the scale that it asks for.
+// number; larger ones are found on the way, and so is any element that is not zero where the sample held none to take a scale from.
+// Should there be any (AGAIN: this kernel's second launch, for W alone, which otherwise ends at once), W is converted once more with
+// the scale that it asks for.
 constexpr float kHalfMax = 65504.0f;
 template <bool AGAIN>
 __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict__ x, int64_t rows, int64_t width,
@@ -243,7 +246,8 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   if (!AGAIN && sample && second) {
     largest = block_reduce<kThreads>(largest, sh, Max());
     // (a largest value: the order does not matter.  Only those that count: 4 096 of these are 33 us)
-    if (threadIdx.x == 0 && ldexpf(largest, -e) > kHalfMax) atomicMax(&ctl->found, __float_as_uint(largest));
+    const float most = m > 0.0f ? kHalfMax : 0.0f;
+    if (threadIdx.x == 0 && ldexpf(largest, -e) > most) atomicMax(&ctl->found, __float_as_uint(largest));
   }
 }
 

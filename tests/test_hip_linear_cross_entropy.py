@@ -538,3 +538,63 @@ def test_refusals(hip_device):
                                           (8, 6, (1 << 24) + 1, -100, 0.0), (8, 6, 10, 1 << 25, 0.0), (8, 6, 10, -100, -0.1)]:
         with pytest.raises(ValueError):
             mod.linear_ce_forward(h(x), h(w), None, h(t), h(one), None, None, None, rows, width, classes, ign, sm, True)
+
+
+def _sparse_weight(D, V, seed):
+    x, _, b, t = _data(70, D, V, seed)
+    return x, np.zeros((D, V), np.float32), b, t, np.random.default_rng(seed + 1)
+
+
+@pytest.mark.parametrize("magnitude", [1.0, 1e-5, 1e-10])
+@pytest.mark.parametrize("piece", [0, 1, 7, 15, 5 * 16 + 9])
+def test_a_large_weight_that_is_zero_but_for_a_few_elements(hip_device, magnitude, piece):
+    """16.8 M weights, 64 neighbours of which are not zero: whichever elements a scale is sampled from, most of these pieces are not
+    among them.  (The bounds are relative to the weight's magnitude: dx is as small as it is.)"""
+    x, w, b, t, rng = _sparse_weight(512, 32768, 40)
+    w.reshape(-1)[piece * 64:piece * 64 + 64] = magnitude * rng.uniform(0.5, 1.0, 64)
+    _check(hip_device, x, w, b, t)
+
+
+@pytest.mark.parametrize("V", [32768, 49152])
+@pytest.mark.parametrize("magnitude", [1e-4, 1e-6])
+def test_a_large_weight_of_few_columns(hip_device, V, magnitude):
+    """a head that starts at zero and some of whose classes are filled in, at numbers of classes that are multiples of 16 384"""
+    x, w, b, t, rng = _sparse_weight(512, V, 42)
+    w[:, 64:128] = magnitude * rng.standard_normal((512, 64))
+    _check(hip_device, x, w, b, t)
+
+
+def test_a_captured_large_weight_that_comes_and_goes(hip_device):
+    """replays over weights that are zero at most places, everywhere, and nowhere"""
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    mod = hip_device.mod
+    x, w, b, t, rng = _sparse_weight(512, 32768, 44)
+    leaves = [Tensor(a, device=hip_device, requires_grad=True) for a in (x, w, b)]
+    tt = Tensor(t, device=hip_device)
+
+    def step():
+        for p in leaves:
+            p.grad = None
+        loss = F.linear_cross_entropy(*leaves, tt)
+        loss.backward()
+        return [loss.data] + [p.grad for p in leaves]
+
+    step()
+    mod.capture_begin()
+    got = step()
+    graph = mod.capture_end(keep=got)
+    block, full = w.copy(), (0.05 * rng.standard_normal(w.shape)).astype(np.float32)
+    block[7, 512:576] = 1e-6 * rng.standard_normal(64)
+    for v in (block, full, w, block):
+        mod.from_numpy(v, leaves[1].data._handle)
+        graph.replay()
+        replayed = [g.numpy().copy() for g in got]
+        for a, c in zip(replayed, step()):
+            assert np.array_equal(a, c.numpy())
+        ref = _reference(x, v, b, t)
+        _within(float(replayed[0][0]), ref[0][0], ref[0][1], "loss")
+        _within(replayed[1], ref[1][0], ref[1][1], "dx")
+        _within(replayed[2], ref[2][0], ref[2][1], "dw")
+    graph.destroy()
+    Graph.free_graph_all()
