@@ -26,6 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWide = 1024;
+// A launch holds fewer than 2^32 threads: more workgroups than these (of up to 1 024) are several launches.
+constexpr int64_t kGroups = 1 << 21;
 template <int T> constexpr int threads() { return T > kThreads ? T : kThreads; }
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -282,12 +284,13 @@ __global__ __launch_bounds__(kThreads) void k_rms_dw_wide(const float* __restric
   partial[(int64_t)blockIdx.y * width + c] = s;
 }
 
-// dw[c] = sum over the partial rows, in the order of the rows within 16 groups and then of the groups; 64 columns a workgroup
+// dw[c] = sum over the partial rows, in the order of the rows within 16 groups and then of the groups; 64 columns a workgroup from
+// column `first` on
 __global__ __launch_bounds__(1024) void k_rms_dw_sum(const float* __restrict__ partial, float* __restrict__ dw, int n_partial,
-                                                     int64_t width) {
+                                                     int64_t width, int64_t first) {
   __shared__ float sh[16][64];
   const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t c = first + (int64_t)blockIdx.x * 64 + lane;
   float s = 0.0f;
   if (c < width) {
     int p = grp;
@@ -307,13 +310,30 @@ __global__ __launch_bounds__(1024) void k_rms_dw_sum(const float* __restrict__ p
   }
 }
 
+// launch(first, n) over [0, total), `most` at a time
+template <class F>
+int in_pieces(int64_t total, int64_t most, F launch) {
+  for (int64_t first = 0; first < total; first += most) {
+    launch(first, std::min(total - first, most));
+    DF_LAUNCH_CHECK();
+  }
+  return DFHIP_OK;
+}
+
 template <int T, int U>
 int fwd(const float* x, const float* res, const float* w, float* y, float* h, float* rstd, int64_t rows, int64_t width, float eps) {
-  const dim3 grid((unsigned)df_ceil_div(rows, threads<T>() / T)), block(threads<T>());
-  if (res) DF_LAUNCH((k_rms_fwd<T, U, true>), grid, block, 0, stream(), x, res, w, y, h, rstd, rows, (int)width, 1.0 / (double)width, eps);
-  else DF_LAUNCH((k_rms_fwd<T, U, false>), grid, block, 0, stream(), x, res, w, y, h, rstd, rows, (int)width, 1.0 / (double)width, eps);
-  DF_LAUNCH_CHECK();
-  return DFHIP_OK;
+  constexpr int64_t TEAMS = threads<T>() / T;
+  return in_pieces(rows, kGroups * TEAMS, [&](int64_t r0, int64_t n) {
+    const dim3 grid((unsigned)df_ceil_div(n, TEAMS)), block(threads<T>());
+    const int64_t at = r0 * width;
+    float* rs = rstd ? rstd + r0 : nullptr;
+    if (res)
+      DF_LAUNCH((k_rms_fwd<T, U, true>), grid, block, 0, stream(), x + at, res + at, w, y + at, h + at, rs, n, (int)width,
+                1.0 / (double)width, eps);
+    else
+      DF_LAUNCH((k_rms_fwd<T, U, false>), grid, block, 0, stream(), x + at, nullptr, w, y + at, nullptr, rs, n, (int)width,
+                1.0 / (double)width, eps);
+  });
 }
 
 template <int T, int U>
@@ -344,12 +364,14 @@ int run_fwd(const float* x, const float* res, const float* w, float* y, float* h
   RMS_FORMS(CALL);
   if (width <= 32768) return CALL(1024, 8);        // (the backward pass holds twice as many values a thread: it would spill)
 #undef CALL
-  if (res) DF_LAUNCH(k_rms_fwd_wide<true>, dim3((unsigned)rows), dim3(kWide), 0, stream(), x, res, w, y, h, rstd, width,
-                     1.0 / (double)width, eps);
-  else DF_LAUNCH(k_rms_fwd_wide<false>, dim3((unsigned)rows), dim3(kWide), 0, stream(), x, res, w, y, h, rstd, width,
-                     1.0 / (double)width, eps);
-  DF_LAUNCH_CHECK();
-  return DFHIP_OK;
+  return in_pieces(rows, kGroups, [&](int64_t r0, int64_t n) {
+    const int64_t at = r0 * width;
+    float* rs = rstd ? rstd + r0 : nullptr;
+    if (res) DF_LAUNCH(k_rms_fwd_wide<true>, dim3((unsigned)n), dim3(kWide), 0, stream(), x + at, res + at, w, y + at, h + at, rs, width,
+                       1.0 / (double)width, eps);
+    else DF_LAUNCH(k_rms_fwd_wide<false>, dim3((unsigned)n), dim3(kWide), 0, stream(), x + at, nullptr, w, y + at, nullptr, rs, width,
+                   1.0 / (double)width, eps);
+  });
 }
 
 int run_bwd(const float* dy, const float* h, const float* rstd, const float* w, const float* add, float* dx, float* partial,
@@ -358,8 +380,12 @@ int run_bwd(const float* dy, const float* h, const float* rstd, const float* w, 
   RMS_FORMS(CALL);
 #undef CALL
   if (dx) {
-    DF_LAUNCH(k_rms_bwd_wide, dim3((unsigned)rows), dim3(kWide), 0, stream(), dy, h, rstd, w, add, dx, width);
-    DF_LAUNCH_CHECK();
+    const int st = in_pieces(rows, kGroups, [&](int64_t r0, int64_t n) {
+      const int64_t at = r0 * width;
+      DF_LAUNCH(k_rms_bwd_wide, dim3((unsigned)n), dim3(kWide), 0, stream(), dy + at, h + at, rstd + r0, w, add ? add + at : nullptr,
+                dx + at, width);
+    });
+    if (st != DFHIP_OK) return st;
   }
   if (partial) {
     DF_LAUNCH(k_rms_dw_wide, dim3((unsigned)df_ceil_div(width, kThreads), (unsigned)blocks), dim3(kThreads), 0, stream(), dy, h,
@@ -410,9 +436,9 @@ int dfhip_rms_norm_backward(const float* dy, const float* h, const float* rstd, 
   }
   st = run_bwd(dy, h, rstd, weight, add, dx, partial, blocks, rows, width);
   if (st != DFHIP_OK || !dweight) return st;
-  DF_LAUNCH(k_rms_dw_sum, dim3((unsigned)df_ceil_div(width, 64)), dim3(1024), 0, stream(), partial, dweight, blocks, width);
-  DF_LAUNCH_CHECK();
-  return DFHIP_OK;
+  return in_pieces(width, kGroups * 64, [&](int64_t first, int64_t n) {
+    DF_LAUNCH(k_rms_dw_sum, dim3((unsigned)df_ceil_div(n, 64)), dim3(1024), 0, stream(), partial, dweight, blocks, width, first);
+  });
 }
 
 }  // extern "C"

@@ -289,3 +289,43 @@ def test_inside_a_captured_graph(hip_device):
             assert np.array_equal(a, b)
     graph.destroy()
     Graph.free_graph_all()
+
+
+def test_more_rows_than_one_launch_holds(hip_device):
+    """2^28 + 5 rows of one element: sixteen threads a row would be a launch of more than 2^32 threads.  The rows differ at the places
+    where one launch could end and the next begin; y = x w / sqrt(x^2 + eps), dx = w dy (1 - y^2 / w^2) / sqrt(x^2 + eps)."""
+    from deepflows_amd import tensor
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    rows, eps = (1 << 28) + 5, 1.0
+    places = [(k << 24) - 3 for k in range(1, 17)] + [0, rows - 6]
+    xd = hip_device.full((rows, 1), 2.0)
+    value = {}
+    for k, at in enumerate(places):
+        for j in range(6):
+            value[at + j] = 0.25 * (1 + k) - 0.125 * j
+            xd[at + j:at + j + 1, :] = value[at + j]
+    x = Tensor(xd, requires_grad=True)
+    w = Tensor(np.array([3.0], np.float32), device=hip_device, requires_grad=True)
+    y = F.rms_norm(x, w, eps)
+    yd = y.data
+
+    class Rest(tensor.UnaryOperator):
+        def forward(self, x):
+            return hip_device.full((1,), 0.0)
+
+        def grad_fn(self, node, grad):
+            return hip_device.full((rows, 1), 1.0)
+
+    Rest(y).backward()
+    middle = 12345678
+    value[middle] = 2.0
+    for at in places + [middle]:
+        n = 1 if at == middle else 6
+        v = np.array([value[at + j] for j in range(n)], np.float64)
+        inv = 1 / np.sqrt(v * v + eps)
+        _within(yd[at:at + n, :].compact().numpy()[:, 0], 3 * v * inv, 5 * U * np.abs(3 * v * inv) + 1e-37, f"y from {at}")
+        want = 3 * inv * (1 - (v * inv) ** 2)
+        # (g - n c with c = g n: both terms up to 3 inv, eight roundings)
+        _within(x.grad[at:at + n, :].compact().numpy()[:, 0], want, 24 * U * inv * (1 + (v * inv) ** 2), f"dx from {at}")
+    Graph.free_graph_all()
