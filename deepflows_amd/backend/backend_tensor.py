@@ -11,6 +11,7 @@ and the CPU-baseline leg of bench.py register the NumPy oracle device explicitly
 """
 import math
 from functools import lru_cache, reduce as _reduce
+from operator import index
 
 import numpy as np
 
@@ -142,11 +143,12 @@ def default_device():
 
 @lru_cache(maxsize=4096)
 def _layout(shape):
-    """(row-major strides, number of elements) of a shape; a training loop asks for the same few shapes every step"""
+    """(row-major strides, number of elements) of a shape; a training loop asks for the same few shapes every step.  In Python's
+    whole numbers: shapes of narrower integers are the same key, and theirs would overflow for everyone."""
     strides, acc = [], 1
     for extent in reversed(shape):
         strides.append(acc)
-        acc *= extent
+        acc *= index(extent)
     return tuple(reversed(strides)), acc
 
 

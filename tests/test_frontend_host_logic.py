@@ -312,3 +312,22 @@ def test_device_modules_follow_the_references_protocol():
     for name in ref["cuda_module"]["functions"]:
         assert hasattr(HipModule, name), f"HipModule lacks {name} (exported by the reference's CUDA module)"
     assert ref["cuda_module"]["classes"] == ["Array"] and hasattr(HipModule, "Array")
+
+
+@pytest.mark.parametrize("first", [np.int16, np.int32, np.int64])
+def test_shapes_of_narrow_integers_have_whole_sizes(cpu_oracle, first):
+    """equal shapes are one entry of the layout cache whatever their elements' types: neither caller's arithmetic may overflow"""
+    from deepflows_amd.backend.backend_tensor import _layout
+    from deepflows_amd.backend_selection import BackendTensor
+    _layout.cache_clear()
+    extent = 1 << 14 if first is np.int16 else 1 << 16
+    narrow = (first(extent), first(extent), first(4))
+    with np.errstate(over="ignore"):
+        assert BackendTensor.compact_strides(narrow) == (4 * extent, 4, 1)
+    strides, size = _layout((extent, extent, 4))
+    assert strides == (4 * extent, 4, 1) and size == 4 * extent * extent
+    assert all(type(v) is int for v in strides + (size,))
+    t = BackendTensor.make((first(3), first(5)), device=cpu_oracle)
+    assert t.is_compact() and t._handle.size == 15
+    with pytest.raises(TypeError):
+        BackendTensor.compact_strides((2.5, 3))
