@@ -67,6 +67,7 @@ __device__ __forceinline__ X block_reduce(X v, X* sh, F f) {
 struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct Add {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+  __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
   __device__ __forceinline__ int operator()(int a, int b) const { return a + b; }
 };
 
@@ -373,18 +374,19 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   }
 }
 
-// loss = sum of the row losses times the scale, in a fixed order; one workgroup of T threads
+// loss = sum of the row losses times the scale, in a fixed order; one workgroup of T threads.  In double: a thread adds rows / T values of
+// one sign, and in fp32 2 M rows drift by up to 5e-4.
 template <int T>
 __device__ __forceinline__ void loss_body(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl, float* __restrict__ loss,
-                                          int64_t rows, float* sh) {
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows; i += T) s += rowloss[i];
+                                          int64_t rows, double* sh) {
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < rows; i += T) s += (double)rowloss[i];
   s = block_reduce<T>(s, sh, Add());
-  if (threadIdx.x == 0) loss[0] = s * ctl->scale;
+  if (threadIdx.x == 0) loss[0] = (float)(s * (double)ctl->scale);
 }
 __global__ __launch_bounds__(1024) void k_lce_loss(const float* __restrict__ rowloss, const Ctl* __restrict__ ctl,
                                                    float* __restrict__ loss, int64_t rows) {
-  __shared__ float sh[1024 / 64];
+  __shared__ double sh[1024 / 64];
   loss_body<1024>(rowloss, ctl, loss, rows, sh);
 }
 
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(threads<T>()) void k_lce_pair(Pair p) {
   const int block = (int)blockIdx.x;
   if (block < p.na) gemm_body<T, false, false, EPI_STORE>(p.a, block, lds);
   else if (block < p.na + p.nb) gemm_body<T, true, true, EPI>(p.b, block - p.na, lds);
-  else loss_body<threads<T>()>(p.rowloss, p.ctl, p.loss, p.rows, reinterpret_cast<float*>(lds));
+  else loss_body<threads<T>()>(p.rowloss, p.ctl, p.loss, p.rows, reinterpret_cast<double*>(lds));
 }
 template <int T, int EPI>
 __global__ __launch_bounds__(256) void k_lce_pair_rest(Pair p) {
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(kThreads) void k_few_pair(Few g, int rows, int clas
                          min(d0 + g.dw_cut, g.width), counted);
     return;
   }
-  loss_body<kThreads>(g.rowloss, g.ctl, g.loss, rows, lds);
+  loss_body<kThreads>(g.rowloss, g.ctl, g.loss, rows, reinterpret_cast<double*>(lds));
 }
 
 // 64 elements of dx a workgroup, each of its waves a quarter of the parts

@@ -598,3 +598,31 @@ def test_a_captured_large_weight_that_comes_and_goes(hip_device):
         _within(replayed[2], ref[2][0], ref[2][1], "dw")
     graph.destroy()
     Graph.free_graph_all()
+
+
+@pytest.mark.parametrize("log2", [7, 19, 21])
+@pytest.mark.parametrize("train", [True, False])
+def test_the_mean_of_equal_rows_is_a_row(hip_device, train, log2):
+    """2^k equal rows have one row's loss: their sum is exact in double, 2^-k is too, so what is left is one rounding of a number that
+    needs none.  (The row's own rounding cancels: 128 rows of the same inputs, by the same products, say what it is.)"""
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Graph, Tensor
+    _, w, b, _ = _data(1, 4, 9, 45)
+
+    def value(N):
+        x, t = np.tile(np.array([[0.3, -1.2, 0.7, 0.1]], np.float32), (N, 1)), np.full(N, 3.0, np.float32)
+        leaves = [Tensor(a, device=hip_device, requires_grad=train) for a in (x, w, b)]
+        if train:
+            loss = F.linear_cross_entropy(*leaves, Tensor(t, device=hip_device))
+        else:
+            with no_grad():
+                loss = F.linear_cross_entropy(*leaves, Tensor(t, device=hip_device))
+        out = loss.numpy()[0]
+        Graph.free_graph_all()
+        return out
+
+    one = value(128)
+    want = _reference(np.array([[0.3, -1.2, 0.7, 0.1]], np.float32), w, b, np.array([3.0], np.float32))[0]
+    _within(float(one), *want, "loss")
+    assert value(1 << log2) == one
