@@ -1,6 +1,8 @@
 """Clipping the gradients of a network by their common norm (extension; the reference has none)."""
 import math
 
+import numpy as np
+
 from .. import backend_api
 from ..backend_selection import BackendTensor
 from ..parallel import _ArrayView
@@ -72,15 +74,16 @@ def _refuse_nonfinite(norm):
 
 
 def _primitive(live, grads, device, max_norm, norm_type, grad_scale, error_if_nonfinite):
-    """the same over the device primitives, a scalar read back per gradient"""
+    """the same over the device primitives, every gradient read back: the squares of fp32 values need double"""
     if norm_type == math.inf:
         parts = [float((g.maximum(-g)).max().numpy().reshape(-1)[0]) for g in grads if g.size]
         total = math.nan if any(math.isnan(v) for v in parts) else max(parts, default=0.0)
     else:
-        total = math.sqrt(sum(float((g * g).sum().numpy().reshape(-1)[0]) for g in grads if g.size))
+        total = math.sqrt(sum(float(np.square(g.numpy(), dtype=np.float64).sum()) for g in grads if g.size))
     total *= grad_scale
     if error_if_nonfinite:
-        _refuse_nonfinite(total)
+        with np.errstate(over="ignore"):
+            _refuse_nonfinite(float(np.float32(total)))      # (the norm as it is returned)
     coef = max_norm / (total + 1e-6)
     coef = 1.0 if coef > 1.0 else coef
     for p, g in zip(live, grads):

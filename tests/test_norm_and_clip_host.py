@@ -210,3 +210,20 @@ def test_two_gloo_ranks_clip_the_mean_of_their_gradients(tmp_path):
             assert_close(np.array(a), want, 1e-5)
     finally:
         backend_api.unregister_device("cpu")
+
+
+@pytest.mark.parametrize("magnitude", [1e30, 1e-30, 3e38, 1e-44])
+def test_clip_of_magnitudes_whose_squares_no_float_holds(cpu_oracle, magnitude):
+    """the norm is held in double: 2 roundings (it and the factor) and the product's, u = 2^-24 each"""
+    from deepflows_amd import optim
+    rng = np.random.default_rng(6)
+    arrays = [(magnitude * rng.uniform(0.25, 1.0, s)).astype(np.float32) for s in ((3, 4), (7,))]
+    params = _params(cpu_oracle, arrays)
+    norm = math.sqrt(sum(float((a.astype(np.float64) ** 2).sum()) for a in arrays))
+    most = 0.5 * norm
+    total = optim.clip_grad_norm_(params, most, error_if_nonfinite=norm < 3.4e38)
+    want = np.float32(norm) if norm < 3.4e38 else np.inf
+    assert abs(float(total.numpy()[0]) - want) <= 2 ** -23 * want + 2 ** -149 or float(total.numpy()[0]) == want
+    for a, p in zip(arrays, params):
+        expected = a.astype(np.float64) * min(1.0, most / (norm + 1e-6))
+        assert np.all(np.abs(p.grad.numpy() - expected) <= 2 ** -22 * np.abs(expected) + 2 ** -149)
