@@ -46,10 +46,11 @@ class CapturedTrainStep:
         the whole graph).  `inputs` / `targets` may be lists of S tensors (one batch per step of the graph).
 
         max_grad_norm: every step's gradients are scaled down to this common norm (optim.clip_grad_norm_) between the exchange and
-        the optimizer, inside the graph where the optimizer is; `grad_norm` then holds the norm of the last step's."""
+        the optimizer, inside the graph where the optimizer is (a replay then refuses another norm or another
+        optimizer.grad_scale); `grad_norm` then holds the norm of the last step's."""
         self.S = int(steps_per_graph)
         self.max_grad_norm, self.grad_norm = _checked_norm(max_grad_norm), None
-        self._clip_scale = optimizer.grad_scale
+        self._recorded_clip = None                  # (max_grad_norm, grad_scale) where the clipping is inside the graph
         self._phase = 0
         if self.S not in (1, 2, 4, 8) or (self.S > 1 and sync is not None):
             # (a power of two: Adam's device table of 1 024 steps' scalars is rewritten in front of a launch, never inside a graph)
@@ -88,6 +89,7 @@ class CapturedTrainStep:
 
     def _capture(self, model, criterion, optimizer, inputs, targets, with_exchange):
         mod, sync = self.mod, self.sync
+        self.grad_norm = self._recorded_clip = None
         mod.capture_feeds = []                      # host-drawn inputs of the step (Dropout masks), in forward order
         mod.capture_begin()
         try:
@@ -110,6 +112,8 @@ class CapturedTrainStep:
                 pass
             Graph.free_graph()
             raise
+        if sync is None or with_exchange:
+            self._recorded_clip = self._clip_settings()
         self.feeds, mod.capture_feeds = mod.capture_feeds, None
         self.loss, self.outputs = loss, outputs
         self.grads = [p.grad for p in optimizer.params]     # the buffers backward writes on a replay
@@ -118,13 +122,16 @@ class CapturedTrainStep:
 
     def _clip(self):
         if self.max_grad_norm is not None:
-            self.grad_norm = clip_grad_norm_(self.optimizer.params, self.max_grad_norm, grad_scale=self._clip_scale)
+            self.grad_norm = clip_grad_norm_(self.optimizer.params, self.max_grad_norm, grad_scale=self.optimizer.grad_scale)
+
+    def _clip_settings(self):
+        return None if self.max_grad_norm is None else (self.max_grad_norm, self.optimizer.grad_scale)
 
     def replay(self):
         opt = self.optimizer
-        if self.max_grad_norm is not None and opt.grad_scale != self._clip_scale:
-            raise RuntimeError("CapturedTrainStep: optimizer.grad_scale changed after the step was captured, and the captured "
-                               "clipping uses it: capture the step again")
+        if (self.sync is None or self.exchange_captured) and self._clip_settings() != self._recorded_clip:
+            raise RuntimeError("CapturedTrainStep: max_grad_norm or optimizer.grad_scale changed after the step was captured, and the "
+                               "captured clipping uses them: capture the step again")
         if self.S > 1:
             # one step per call: the graph of S steps goes out on the first call of every S
             self._phase = (self._phase + 1) % self.S

@@ -42,7 +42,8 @@ class EpochTrainer:
             raise ValueError("tail is 'eager' or 'capture'")
         self.model, self.criterion, self.optimizer, self.device, self.mod = model, criterion, optimizer, device, mod
         self.K, self.eps, self.augment, self.capture, self.tail, self.sync = int(num_classes), eps, augment, capture, tail, sync
-        self.max_grad_norm = max_grad_norm        # None, or the largest norm of a step's gradients (optim.clip_grad_norm_)
+        # None, or the largest norm of a step's gradients (optim.clip_grad_norm_); may be changed between steps
+        self.max_grad_norm = max_grad_norm
         self._slots = {}             # batch shape -> (pipeline, x tensor, y tensor)
         self._captured = {}          # batch shape -> CapturedTrainStep
         self._losses = mod.Array(int(max_losses))
@@ -63,6 +64,10 @@ class EpochTrainer:
         use_graph = self.capture and (shape == self._main_shape or self.tail == "capture")
         if use_graph:
             cs = self._captured.get(shape)
+            if cs is not None and cs.max_grad_norm != self.max_grad_norm:
+                del self._captured[shape]            # (the norm is part of the graph)
+                cs.destroy()
+                cs = None
             if cs is None:
                 from ..graph_step import CapturedTrainStep
                 # (a capture records the step without running it and draws no host random numbers: Dropout masks

@@ -322,3 +322,90 @@ def test_the_overlapped_exchange_clips(hip_device):
         Graph.free_graph_all()
     for a, b in zip(*runs):
         assert np.array_equal(a, b)
+
+
+def test_a_changed_norm_of_a_captured_step_is_refused(hip_device):
+    from deepflows_amd import optim
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+    net, crit, params = _build(hip_device)
+    x, t = (Tensor(a, device=hip_device) for a in _batches(1, 8)[0])
+    for first, second in ((1.0, 2.0), (1.0, None), (None, 1.0)):
+        step = CapturedTrainStep(net, crit, optim.SGD(params, lr=0.1), x, t, max_grad_norm=first)
+        step.replay()
+        step.max_grad_norm = second
+        with pytest.raises(RuntimeError):
+            step.replay()
+        step.max_grad_norm = first
+        step.replay()
+        step.destroy()
+    Graph.free_graph_all()
+
+
+def test_the_epoch_loop_clips_to_the_norm_it_has_now(hip_device):
+    """another norm for the second epoch and none for the third, captured and eagerly: the same losses and parameters, bit for bit"""
+    from deepflows_amd import nn, optim, workloads
+    from deepflows_amd.tensor import Graph
+    from deepflows_amd.utils.data import data_loader
+    from deepflows_amd.utils.train_loop import EpochTrainer
+    rng = np.random.default_rng(6)
+    x = (rng.standard_normal((40, 3, 32, 32)) * 0.8).astype(np.float32)
+    y = rng.integers(0, 10, 40)
+    finals = []
+    for capture in (True, False):
+        np.random.seed(4)
+        model = workloads.ResNet18(10, device=hip_device, register_blocks=True)
+        opt = optim.SGD(model.parameters(), lr=0.1)
+        trainer = EpochTrainer(model, nn.CrossEntropyLoss(), opt, hip_device, capture=capture, max_grad_norm=0.05)
+        losses = []
+        for epoch, norm in enumerate((0.05, 0.5, None)):
+            trainer.max_grad_norm = norm
+            np.random.seed(9 + epoch)
+            losses.append(trainer.run_epoch(data_loader(x, y, 16, shuffle=True), epoch, 3))
+        finals.append((losses, [p.numpy().copy() for p in opt.params]))
+        trainer.destroy()
+        Graph.free_graph_all()
+    for a, b in zip(*[f[0] for f in finals]):
+        assert np.array_equal(a, b)
+    for a, b in zip(*[f[1] for f in finals]):
+        assert np.array_equal(a, b)
+
+
+def test_a_step_that_clips_behind_its_graph_follows_both_settings(hip_device):
+    """the exchange outside the graph, and the clipping behind it: another norm or factor between replays is what the eager step does"""
+    from deepflows_amd import optim, parallel, workloads
+    from deepflows_amd.graph_step import CapturedTrainStep
+    from deepflows_amd.tensor import Graph, Tensor
+
+    class Same(parallel.Communicator):
+        exchanges = True
+
+        def allreduce_sum(self, flat, overlap=False):
+            return flat
+
+    batches, runs = _batches(3, 24), []
+    for captured in (False, True):
+        net, crit, params = _build(hip_device)
+        opt = optim.SGD(params, lr=0.3)
+        bucket = parallel.GradientBucket(opt.params, Same())
+        x, t = (Tensor(a, device=hip_device) for a in batches[0])
+        step = None
+        if captured:
+            step = CapturedTrainStep(net, crit, opt, x, t, sync=bucket.sync, capture_exchange=False, max_grad_norm=0.2)
+        for (bx, bt), norm, factor in zip(batches, (0.2, 0.1, 0.4), (1.0, 0.5, 2.0)):
+            hip_device.mod.from_numpy(bx, x.data._handle)
+            hip_device.mod.from_numpy(bt, t.data._handle)
+            opt.grad_scale = factor
+            if captured:
+                step.max_grad_norm = norm
+                step.replay()
+            else:
+                workloads.train_step(net, crit, opt, x, t, sync=bucket.sync, max_grad_norm=norm)
+                Graph.free_graph()
+        runs.append([p.numpy().copy() for p in params])
+        if step is not None:
+            step.destroy()
+        bucket.release()
+        Graph.free_graph_all()
+    for a, b in zip(*runs):
+        assert np.array_equal(a, b)
