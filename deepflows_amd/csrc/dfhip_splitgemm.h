@@ -75,10 +75,13 @@ __device__ __forceinline__ float lanes_reduce(float v, F f) {
   return v;
 }
 // What a row of softmax needs of LANES x N of its logits, N a lane: the largest one, the sum of exponentials from there, and (`sum`)
-// the sum of l - largest, in all of the lanes.  w is -inf where there is no class (`in`).
+// the sum of l - largest times kDown, in all of the lanes.  w is -inf where there is no class (`in`).  At most 1 / kDown of them: the
+// scaled sum of finite values is finite, those of classes that a bias of the type's lowest value masks among them.
+constexpr float kDown = 1.0f / 128;
 struct RowPart { float m, z, t; };
 template <int N, int LANES>
 __device__ __forceinline__ RowPart row_part(const float* w, const bool* in, bool sum) {
+  static_assert(N * LANES * kDown <= 1.0f, "kDown");
   RowPart p;
   float m = w[0];
 #pragma unroll
@@ -92,7 +95,7 @@ __device__ __forceinline__ RowPart row_part(const float* w, const bool* in, bool
   p.z = lanes_reduce<LANES>(p.z, add);
   if (sum) {
 #pragma unroll
-    for (int f = 0; f < N; f++) p.t += in[f] ? w[f] - from : 0.0f;
+    for (int f = 0; f < N; f++) p.t += in[f] ? (w[f] - from) * kDown : 0.0f;
     p.t = lanes_reduce<LANES>(p.t, add);
   }
   return p;
@@ -180,7 +183,7 @@ __device__ __forceinline__ void emit_stats(const Gemm& g, int e, const float* bi
 template <int T, int TM, int TN>
 __device__ __forceinline__ void wave_stats(const Gemm& g, int e, const float* bias, int64_t m0, int64_t n0, const f32x16 (*acc)[TN],
                                            float* own) {
-  static_assert(TN * 32 == unit<T>(), "a run");
+  static_assert(TN * 32 == unit<T>() && TN * 32 * kDown <= 1.0f, "a run");
   constexpr int PITCH = TN * 32 + 4, HALF = TN * 16;
   const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5, row = lane >> 1, c0 = (lane & 1) * HALF;
   const int64_t u = n0 / unit<T>();
@@ -219,7 +222,7 @@ __device__ __forceinline__ void wave_stats(const Gemm& g, int e, const float* bi
     RowPart part = {m, 0.0f, 0.0f};
     if (g.sum) {
 #pragma unroll
-      for (int c = 0; c < HALF; c++) part.t += c < valid ? w[c] - from : 0.0f;
+      for (int c = 0; c < HALF; c++) part.t += c < valid ? (w[c] - from) * kDown : 0.0f;
       part.t += moved<0xB1>(part.t);
     }
 #pragma unroll

@@ -252,6 +252,9 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
   }
 }
 
+// 2^-k, 2^k >= classes: what the terms of a mean over the classes are scaled by, so that no sum of finite ones passes the largest float
+__device__ __forceinline__ float mean_scale(int classes) { return ldexpf(1.0f, -(32 - __clz(classes - 1))); }
+
 // A workgroup a row: the row's loss, and dl (times 2^kTop) over its logits as a split array.  `cells` is the padded row, a
 // multiple of 256; a row that is not counted, or lies behind the last one (blockIdx.x >= rows), becomes zeros.
 // U > 0: U groups of eight logits a thread hold the row in registers (T * 8 * U >= cells), one pass over memory each way;
@@ -317,6 +320,7 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   }
   m = block_reduce<T>(m, sh, Max());
   float z = 0.0f, s = 0.0f;
+  const float down = mean_scale(classes);
   for (int i = 0; i < trips; i++) {
     if (U == 0) load(i);
     const int c0 = first();
@@ -326,10 +330,10 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
       if (smooth > 0.0f) {
         if (c + 8 <= classes) {
 #pragma unroll
-          for (int k = 0; k < 8; k++) s += v[u][k] - m;
+          for (int k = 0; k < 8; k++) s = fmaf(v[u][k] - m, down, s);
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; k++) s += c + k < classes ? v[u][k] - m : 0.0f;
+          for (int k = 0; k < 8; k++) s = fmaf(c + k < classes ? v[u][k] - m : 0.0f, down, s);
         }
       }
 #pragma unroll
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
   if (smooth > 0.0f) s = block_reduce<T>(s, sh, Add());
   if (threadIdx.x == 0) {
     float r = logf(z) - (1.0f - smooth) * (lt - m);
-    if (smooth > 0.0f) r -= smooth * (s / (float)classes);
+    if (smooth > 0.0f) r -= smooth * (s / ((float)classes * down));
     rowloss[blockIdx.x] = ok ? r : NAN;
   }
   const float top = (float)(1 << kTop), iz = ok ? top / z : NAN, q = top * (smooth / (float)classes), p1 = top * (1.0f - smooth);
@@ -426,7 +430,7 @@ struct Few {
   const float* bias;
   float* l;                                // logits, then dl
   int64_t ld;                              // a multiple of 128
-  float* stat;                             // three arrays of (rows, tiles): largest, sum of exponentials, sum of l - largest
+  float* stat;                             // three arrays of (rows, tiles): largest, sum of exponentials, kDown * sum of l - largest
   int tiles, cols;                         // their number and width
   const float* lt;                         // the targets' logits, or NULL: they are in l
   const float* target;
@@ -501,17 +505,18 @@ __global__ __launch_bounds__(kThreads) void k_few_rows(Few g, int rows, int clas
   for (int k = threadIdx.x; k < g.tiles; k += kThreads) m = fmaxf(m, sm[k]);
   m = block_reduce<kThreads>(m, sh, Max());
   float z = 0.0f, s = 0.0f;
+  const float down = mean_scale(classes);
 #pragma unroll 4
   for (int k = threadIdx.x; k < g.tiles; k += kThreads) z += sz[k] * exp_of(sm[k] - m);
   z = block_reduce<kThreads>(z, sh, Add());
   if (owner && g.smooth > 0.0f) {
     for (int k = threadIdx.x; k < g.tiles; k += kThreads)
-      s += sm[k] > -INFINITY ? st[k] + (float)min(g.cols, classes - k * g.cols) * (sm[k] - m) : -INFINITY;
+      s += sm[k] > -INFINITY ? st[k] * (down / kDown) + (float)min(g.cols, classes - k * g.cols) * down * (sm[k] - m) : -INFINITY;
     s = block_reduce<kThreads>(s, sh, Add());
   }
   if (owner && threadIdx.x == 0) {
     float r = logf(z) - (1.0f - g.smooth) * (lt - m);
-    if (g.smooth > 0.0f) r -= g.smooth * (s / (float)classes);
+    if (g.smooth > 0.0f) r -= g.smooth * (s / ((float)classes * down));
     rowloss[row] = ok ? r : NAN;
   }
   if (!GRADS) return;

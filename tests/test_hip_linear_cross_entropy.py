@@ -626,3 +626,28 @@ def test_the_mean_of_equal_rows_is_a_row(hip_device, train, log2):
     want = _reference(np.array([[0.3, -1.2, 0.7, 0.1]], np.float32), w, b, np.array([3.0], np.float32))[0]
     _within(float(one), *want, "loss")
     assert value(1 << log2) == one
+
+
+@pytest.mark.parametrize("N", [12, 45, 90])
+@pytest.mark.parametrize("V", [2, 9, 300, 33000, 60001])
+def test_smoothing_over_several_classes_of_the_lowest_value(hip_device, N, V):
+    """Masked classes of the type's lowest value and a smoothed target: the loss is e / V times their sum, large but finite although
+    the sum itself is no float.  Its terms have one sign: each a rounding, their sum V / 256 + 40, a few for the rest."""
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    x, w, b, t = _data(N, 40, V, 46)
+    low = np.finfo(np.float32).min
+    out = np.zeros(V, bool)
+    out[1::3] = True
+    if V > 1000:
+        out[200:500] = True                                    # whole runs of classes
+    t[:] = np.nonzero(~out)[0][t.astype(int) % int((~out).sum())]
+    b[0, out] = low
+    want = _reference(x, w, b, t, e=0.1)[0][0]
+    assert np.isfinite(np.float32(want))
+    tol = (V / 256 + 60) * U * want
+    _within(_run(hip_device, x, w, b, t, label_smoothing=0.1)[0], want, tol, "loss")
+    with no_grad():
+        loss = F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, w, b, t)], label_smoothing=0.1)
+    _within(float(loss.numpy()[0]), want, tol, "loss alone")
