@@ -1,11 +1,14 @@
-// fp32 products on the fp16 matrix cores: every operand is held as TWO fp16 values whose sum carries 22 bits of it, and a
-// product is formed from three of the four partial products, accumulated in fp32.
+// fp32 products on the fp16 matrix cores: every operand is held as TWO fp16 values that carry 23 bits of it, and a product is formed
+// from three of the four partial products, accumulated in fp32.
 //
-//   v 2^-e = hi + lo,  hi = fp16(v 2^-e),  lo = fp16(v 2^-e - hi):  |error| <= 2^-22 |v| (and 2^-39 of the array's largest
-//   magnitude A, with e chosen so that A 2^-e lies in [2^13, 2^14): from there down to 2^-17 A both halves are normal numbers)
-//   a b = hi hi' + hi lo' + lo hi'  (+ lo lo' <= 2^-22 |a b|, left out)
-// (the scheme is published: Ootomo and Yokota, "Recovering single precision accuracy from Tensor Cores while surpassing the FP32
-// theoretical peak performance", 2022).  Against fp32 MFMA (157 TFLOP/s) the fp16 rate is 16 times as high, a third of it is left:
+//   v 2^-e = hi + 2^-11 lo,  hi = fp16(v 2^-e),  lo = fp16(2^11 (v 2^-e - hi)):  |error| <= 2^-23 |v|, with a floor of 2^-49 of the
+//   array's largest magnitude A, for e such that A 2^-e lies in [2^13, 2^14): lo is a normal number wherever hi is one, down to
+//   2^-28 A, and keeps what a hi below that cannot hold.  (Unscaled, lo would leave the normal numbers at 2^-17 A, and elements
+//   below 2^-39 A would vanish: the gradient of a class that is hardly ever likely, beside those of the others.)
+//   a b = hi hi' + 2^-11 (hi lo' + lo hi')  (+ 2^-22 lo lo' <= 2^-22 |a b|, left out)
+// The two sums are two sets of accumulators, joined at the end.
+// (The scheme is published: Ootomo and Yokota, "Recovering single precision accuracy from Tensor Cores while surpassing the FP32
+// theoretical peak performance", 2022.)  Against fp32 MFMA (157 TFLOP/s) the fp16 rate is 16 times as high, a third of it is left:
 // measured error and time beside the caller, dfhip_vocab.hip.
 //
 // STORAGE ("split array"): a padded row-major array of 4-byte cells, columns in blocks of 32: 128 bytes that hold the block's 32
@@ -15,10 +18,13 @@
 //   the reduction runs across them ("K across"): a tile is 32 rows of 4 T bytes, read with the transposing LDS loads
 //   (ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 halves, each lane receives the 4 rows of its column).
 //
-// KERNEL: workgroup tile T x T, K step 32, LDS buffers filled by 16-byte global-to-LDS copies issued NS - 1 steps ahead; one
-// barrier a step.  32 x 32 x 16 MFMA.  T = 256: 8 waves of 128 x 64, two buffers, one workgroup a CU; T = 128: 4 waves of 64 x 64,
-// two buffers, two workgroups a CU; T = 64: 4 waves of 32 x 32, four buffers (short reductions and few tiles wait for memory, not
-// for the matrix cores).  LDS positions are XOR-permuted at 16-byte granularity by the ROW (the copy's source address is permuted,
+// KERNEL: workgroup tile BM x BN, K step 32, LDS buffers filled by 16-byte global-to-LDS copies issued NS - 1 steps ahead; one
+// barrier a step.  32 x 32 x 16 MFMA.  T = 256: 256 x 128 by eight waves of 64 x 64, two buffers, one workgroup a CU; T = 128:
+// 128 x 128 by four waves of 64 x 64, two buffers, two workgroups a CU; T = 64: 64 x 64 by four waves of 32 x 32, four buffers (short
+// reductions and few tiles wait for memory, not for the matrix cores).
+// The second set of accumulators is what the tiles are small for: one set allowed 256 x 256 by waves of 128 x 64, whose operands cross
+// the LDS two thirds as often (8192 x 1024 x 50001: 6.6 ms against 7.07).  Those waves with both sets, one a SIMD (256 x 128 by four):
+// 110 us where eight waves take 96; a third buffer: 99.  LDS positions are XOR-permuted at 16-byte granularity by the ROW (the copy's source address is permuted,
 // its LDS side is linear): 16 lanes that read the same piece of 16 rows, or 32 lanes that read 4 rows transposed, touch every bank
 // once (SQ_LDS_BANK_CONFLICT reads 0).
 // LDS reads: three products share two fragments a side, so the LDS moves half the bytes an fp16 GEMM of the same rate would.
@@ -35,14 +41,15 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTop = 13;                 // the largest magnitude of an operand is scaled into [2^13, 2^14)
+constexpr float kLow = 1.0f / 2048;      // what a low half stands for
 constexpr int kPad = 256;                // rows and columns of a split array are padded with zeros to a multiple of this
 
 __host__ __device__ inline int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
 
-// one scaled value as hi + lo; what is not finite stays in hi alone
+// one scaled value as hi + kLow lo; what is not finite stays in hi alone
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
-  const float r = v - (float)hi;
+  const float r = (v - (float)hi) * (1.0f / kLow);
   lo = (_Float16)(r == r ? r : 0.0f);    // (inf - inf, NaN: no low half)
 }
 
@@ -136,11 +143,12 @@ struct Gemm {
 };
 template <int T> constexpr int unit() { return T == 64 ? 32 : 64; }      // a wave's columns
 
-// place of a tile: bands of eight tile rows, down the band first
+// place of a tile: bands of kBand tile rows, down the band first
+constexpr int kBand = 4;
 __device__ __forceinline__ void place(const Gemm& g, int tile, int& tm, int& tn) {
-  const int band = tile / (8 * g.tiles_n), in = tile - band * 8 * g.tiles_n, high = min(8, g.tiles_m - band * 8);
+  const int band = tile / (kBand * g.tiles_n), in = tile - band * kBand * g.tiles_n, high = min(kBand, g.tiles_m - band * kBand);
   tn = in / high;
-  tm = band * 8 + in - tn * high;
+  tm = band * kBand + in - tn * high;
 }
 
 template <int EPI>
@@ -148,7 +156,8 @@ __device__ __forceinline__ float bias_of(const Gemm& g, int64_t n) {
   return (EPI == EPI_BIAS || EPI == EPI_STATS) && g.bias && n < g.n ? g.bias[n] : 0.0f;
 }
 // One value of row m (c: its place) and column n.  STREAM: past the caches, where a wave's stores fill whole lines -- a round of
-// 256 x 256 tiles writes 64 MB that nothing reads soon, and the operands' lines stay (eval 1500 x 1024 x 30011: 373 -> 355 us).
+// 256 workgroups writes 32 MB that nothing reads soon, and the operands' lines stay (1500 x 1024 x 30011 logits written: 373 -> 355 us
+// with 256 x 256 tiles).
 template <int EPI, bool STREAM>
 __device__ __forceinline__ void emit(const Gemm& g, int e, float sc, float bias, int64_t m, int64_t n, float* c, float v) {
   if (EPI != EPI_BIAS && (m >= g.m || n >= g.n)) return;
@@ -327,11 +336,14 @@ struct Reader {
 };
 
 template <int T> struct Tile;
-template <> struct Tile<256> { static constexpr int WM = 2, WN = 4, NS = 2; };
-template <> struct Tile<128> { static constexpr int WM = 2, WN = 2, NS = 2; };
-template <> struct Tile<64> { static constexpr int WM = 2, WN = 2, NS = 4; };
+template <> struct Tile<256> { static constexpr int BM = 256, BN = 128, WM = 4, WN = 2, NS = 2; };
+template <> struct Tile<128> { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, NS = 2; };
+template <> struct Tile<64> { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, NS = 4; };
+constexpr int tile_columns(int tile) { return tile == 64 ? 64 : 128; }
 template <int T> constexpr int threads() { return Tile<T>::WM * Tile<T>::WN * 64; }
-template <int T> constexpr int lds_bytes() { return Tile<T>::NS * 2 * T * 128; }
+template <int T> constexpr int waves() { return 2; }      // a SIMD: what its registers are shared by
+template <int T> constexpr int lds_bytes() { return Tile<T>::NS * (Tile<T>::BM + Tile<T>::BN) * 128; }
+template <int T> constexpr int slices() { return Tile<T>::BM * Tile<T>::BN / 1024; }     // workgroups that add up a cut tile's parts
 // workgroups of a product
 __host__ __device__ inline int groups(const Gemm& g) { return ((g.full + 7) / 8 + (g.rest * g.splits + 7) / 8) * 8; }
 
@@ -350,14 +362,15 @@ __device__ __forceinline__ void spread() {
 
 template <int T, bool AX, bool BX, int EPI>
 __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* lds) {
-  constexpr int BM = T, BN = T, WM = Tile<T>::WM, WN = Tile<T>::WN, NS = Tile<T>::NS;
+  constexpr int BM = Tile<T>::BM, BN = Tile<T>::BN, WM = Tile<T>::WM, WN = Tile<T>::WN, NS = Tile<T>::NS;
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128, COPIES = (BM + BN) / 8 / NW;
   static_assert((BM / WM) % 64 == 0 || TM == 1, "Reader");
   static_assert((BN / WN) % 64 == 0 || TN == 1, "Reader");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles, and the 32 that it works on at a
-  // time are 8 x 4 neighbours, which go along the reduction together and share 12 operand tiles in its L2 (a column of 32: 33)
+  // time are 4 x 8 neighbours, which go along the reduction together and share 12 operand tiles in its L2 (a column of 32: 33; of
+  // 256 x 128 tiles 2 048 rows of operands, 8 x 4 would be 2 560: 8192 x 1024 x 50001 7.16 -> 7.07 ms)
   const bool whole = block < (g.full + 7) / 8 * 8;
   const int id = whole ? block : block - (g.full + 7) / 8 * 8;
   const int total = whole ? g.full : g.rest * g.splits, per = (total + 7) >> 3;
@@ -371,13 +384,13 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
   const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
   const bool sums = BX && g.colsum && tm == 0 && wm == 0;
 
-  f32x16 acc[TM][TN];
+  f32x16 acc[TM][TN], low[TM][TN];                 // hi hi', and hi lo' + lo hi'
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+      for (int r = 0; r < 16; r++) acc[i][j][r] = low[i][j][r] = 0.0f;
   float col[TN];
 #pragma unroll
   for (int j = 0; j < TN; j++) col[j] = 0.0f;
@@ -404,19 +417,19 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
     for (int i = 0; i < TM; i++) f.ah[i] = ra.get(cur, i, kk, 0);
   };
   auto multiply = [&](const Frag& f) {
-    // (the same accumulator comes up again after TM * TN products)
+    // (the same accumulator comes up again after TM * TN products or more)
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
-      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < TM; i++)
-#pragma unroll
-      for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < TN; j++) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], low[i][j], 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], low[i][j], 0, 0, 0);
   };
   auto add_columns = [&](const Frag& f) {          // (a lane holds eight rows of one column)
     if (BX && sums) {
@@ -424,7 +437,7 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
       for (int j = 0; j < TN; j++) {
         float t = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) t += (float)f.bh[j][k] + (float)f.bl[j][k];
+        for (int k = 0; k < 8; k++) t += fmaf((float)f.bl[j][k], kLow, (float)f.bh[j][k]);
         col[j] += t;
       }
     }
@@ -475,6 +488,12 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
   multiply(f1);
   add_columns(f1);
 
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = fmaf(low[i][j][r], kLow, acc[i][j][r]);
   const int e = exponent(g);
   const float sc = g.scale ? g.scale[0] : 1.0f;
   float* part = whole ? nullptr : g.parts + (int64_t)((tile - g.full) * g.splits + z) * (BM * BN + BN);
@@ -520,7 +539,7 @@ __device__ __forceinline__ void gemm_body(const Gemm& g, const int block, char* 
 }
 
 template <int T, bool AX, bool BX, int EPI>
-__global__ __launch_bounds__(threads<T>()) void k_split_gemm(Gemm g) {
+__global__ __launch_bounds__(threads<T>(), waves<T>()) void k_split_gemm(Gemm g) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   gemm_body<T, AX, BX, EPI>(g, (int)blockIdx.x, lds);
 }
@@ -528,7 +547,7 @@ __global__ __launch_bounds__(threads<T>()) void k_split_gemm(Gemm g) {
 // the parts of the cut tiles added up: 1024 cells of one tile a workgroup, four a thread
 template <int T, int EPI>
 __device__ __forceinline__ void rest_body(const Gemm& g, const int block) {
-  constexpr int BM = T, BN = T, SLICES = BM * BN / 1024, CELLS = BM * BN + BN;
+  constexpr int BM = Tile<T>::BM, BN = Tile<T>::BN, SLICES = slices<T>(), CELLS = BM * BN + BN;
   const int t = block / SLICES, slice = block % SLICES, tile = g.full + t;
   int tm, tn;
   place(g, tile, tm, tn);
@@ -575,10 +594,10 @@ __global__ __launch_bounds__(256) void k_split_rest(Gemm g) { rest_body<T, EPI>(
 // How a product of m x n outputs runs with T x T tiles: which tiles are cut, and into how many parts.
 struct Plan { int tile, tiles_m, tiles_n, full, rest, splits, ksteps, ksteps_split; };
 
-// Microseconds of `items` resident workgroups of one step each, measured (a step: 32 along the reduction): a chip full of 256 x 256
-// tiles (256 workgroups) 2.5, of 128 x 128 (512) 1.42, of 64 x 64 (512) 0.49; few workgroups 1.85, 0.66 and 0.31.
+// Microseconds of `items` resident workgroups of one step each, measured (a step: 32 along the reduction): a chip full of 256 x 128
+// tiles (256 workgroups) 1.4, of 128 x 128 (512) 1.42, of 64 x 64 (512) 0.49; few workgroups 1.0, 0.66 and 0.31.
 inline double step_us(int tile, double items) {
-  if (tile == 256) return items <= 64 ? 1.85 : 1.85 + 0.65 * (items - 64) / 192;
+  if (tile == 256) return items <= 64 ? 1.0 : 1.0 + 0.4 * (items - 64) / 192;
   const double half = items <= 256 ? items / 256 : 1.0, over = items <= 256 ? 0.0 : (items - 256) / 256;
   return tile == 128 ? 0.66 + 0.15 * half + 0.61 * over : 0.31 + 0.03 * half + 0.15 * over;
 }
@@ -588,7 +607,7 @@ inline int64_t slots(int tile) { return (tile == 256 ? 1 : 2) * (int64_t)dfhip::
 inline double cost_us(const Plan* p, int n) {
   const int tile = p[0].tile;
   const int64_t s = slots(tile);
-  const double begin = tile == 256 ? 8.0 : tile == 128 ? 4.5 : 3.5;
+  const double begin = tile == 256 ? 7.0 : tile == 128 ? 4.5 : 3.5;
   int64_t items = 0, parts = 0;
   for (int i = 0; i < n; i++) {
     parts += (int64_t)p[i].rest * p[i].splits;
@@ -629,11 +648,11 @@ inline double cost_us(const Plan* p, int n) {
     }
     for (int k = 0; k < groups; k++) end = std::max(end, free_at[k].t);
   }
-  return end + (parts ? 5.0 + (double)parts * (tile == 256 ? 0.1 : tile == 128 ? 0.025 : 0.00625) : 0.0);
+  return end + (parts ? 5.0 + (double)parts * (tile == 256 ? 0.05 : tile == 128 ? 0.025 : 0.00625) : 0.0);
 }
 // the ways a product may be cut: not at all; what is left over from whole rounds; every tile
 inline int ways(int tile, int64_t m, int64_t n, int steps, Plan* out) {
-  const int64_t tm = (m + tile - 1) / tile, tn = (n + tile - 1) / tile, tiles = tm * tn, s = slots(tile);
+  const int64_t tm = (m + tile - 1) / tile, bn = tile_columns(tile), tn = (n + bn - 1) / bn, tiles = tm * tn, s = slots(tile);
   if (tiles > (1 << 24)) return 0;
   int count = 0;
   out[count++] = Plan{tile, (int)tm, (int)tn, (int)tiles, 0, 1, steps, steps};
@@ -662,7 +681,7 @@ inline void apply(Gemm& g, const Plan& p, int64_t m, int64_t n) {
   g.m = g.c || g.stat ? (int)m : 0;                // (column sums alone: nothing of the product is stored)
   g.n = (int)n;
 }
-inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.tile * p.tile + p.tile); }
+inline int64_t parts_floats(const Plan& p) { return (int64_t)p.rest * p.splits * (p.tile * tile_columns(p.tile) + tile_columns(p.tile)); }
 
 // a kernel's LDS beyond 64 KB has to be asked for once
 inline int allow_lds(const void* kernel, int bytes, bool& done) {

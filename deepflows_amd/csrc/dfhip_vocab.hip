@@ -8,8 +8,9 @@
 // products, so memory does not grow with rows x classes.  The gradients are formed in the forward pass, for an upstream
 // gradient of 1: nothing is computed twice (recomputing the logits in a backward pass would be a third more products).
 //
-// The three products run on the fp16 matrix cores with fp32 accuracy (dfhip_splitgemm.h): x and W are converted once a call,
-// dl where it is formed; for few rows, where W's bytes are what counts, on the fp32 matrix cores (dfhip_fewrows.h, and further
+// The three products run on the fp16 matrix cores with fp32 accuracy (dfhip_splitgemm.h: 23 bits of every element down to 2^-28 of its
+// array's largest, of dl down to 2^-29): x and W are converted once a call, dl where it is formed; for few rows, where W's bytes are
+// what counts, they run on the fp32 matrix cores (dfhip_fewrows.h, and further
 // down).  The launches of a call:
 //   k_lce_scan     the largest magnitudes of x (counted rows) and W, finite elements only
 //   k_lce_split    x, W -> split arrays; the number of counted rows (a large W may need it twice)
@@ -18,11 +19,11 @@
 //   without gradients: the product's epilogue leaves what the softmax needs of every 64 logits and the targets' (none is stored),
 //                  k_few_rows joins them, k_lce_loss
 //
-// Measured.  8192 x 1024 x 50001 with gradients, 6.6 ms: logits 2.08 ms and the pair 3.85 ms, 1.21 and 1.31 PFLOP/s of fp16 (the
+// Measured.  8192 x 1024 x 50001 with gradients, 7.1 ms: logits 2.19 ms and the pair 4.31 ms, 1.15 and 1.17 PFLOP/s of fp16 (the
 // library's 8192^3 fp16 product: 1.18; at that rate the three products alone are 6.42 ms, in fp32 16.4), rows 0.68 ms (3.3 GB, 4.8
-// TB/s), conversion 0.09.  2048 x 768 x 32000: 0.89 ms; 509 x 512 x 10007: 86 us; 1500 x 1024 x 30011, the loss alone: 0.30 ms.
-// Largest error of any result against 64 bits, relative to the result's largest value: 1.8e-6 at 8192 x 1024 x 50001, where the
-// fp32 composition (library products) has 5.4e-6; 7e-7 and 4.3e-6 at 2048 x 768 x 32000.
+// TB/s), conversion 0.10.  2048 x 768 x 32000: 0.95 ms; 509 x 512 x 10007: 89 us; 1500 x 1024 x 30011, the loss alone: 0.32 ms.
+// Largest error of any result against 64 bits, relative to the result's largest value: 2.1e-6 at 8192 x 1024 x 50001, where the
+// fp32 composition (library products) has 5.4e-6; 9e-7 and 4.3e-6 at 2048 x 768 x 32000.
 #include <math.h>
 
 #include <algorithm>
@@ -37,6 +38,7 @@ using namespace dfhip_split;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTopDl = 15;                                 // |dl| <= 1: at most 2^15 as a split array
 constexpr int kScan = 512;                                 // workgroups (= partial maxima) a tensor
 // From this many elements of W on its scale comes from a sample: at 1024 x 16384 the full scan is 11.6 us, the sample 4.6 and the
 // launch that looks whether it was enough 4.8; at 1024 x 50001 41 and 5.4 + 4.9.
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void k_lce_split(const float* __restrict_
 // 2^-k, 2^k >= classes: what the terms of a mean over the classes are scaled by, so that no sum of finite ones passes the largest float
 __device__ __forceinline__ float mean_scale(int classes) { return ldexpf(1.0f, -(32 - __clz(classes - 1))); }
 
-// A workgroup a row: the row's loss, and dl (times 2^kTop) over its logits as a split array.  `cells` is the padded row, a
+// A workgroup a row: the row's loss, and dl (times 2^kTopDl) over its logits as a split array.  `cells` is the padded row, a
 // multiple of 256; a row that is not counted, or lies behind the last one (blockIdx.x >= rows), becomes zeros.
 // U > 0: U groups of eight logits a thread hold the row in registers (T * 8 * U >= cells), one pass over memory each way;
 // U = 0: any length, the row read three times.
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(T) void k_lce_rows(float* __restrict__ logits, cons
     if (smooth > 0.0f) r -= smooth * (s / ((float)classes * down));
     rowloss[blockIdx.x] = ok ? r : NAN;
   }
-  const float top = (float)(1 << kTop), iz = ok ? top / z : NAN, q = top * (smooth / (float)classes), p1 = top * (1.0f - smooth);
+  const float top = (float)(1 << kTopDl), iz = ok ? top / z : NAN, q = top * (smooth / (float)classes), p1 = top * (1.0f - smooth);
   for (int i = 0; i < trips; i++) {
     if (U == 0) {
       load(i);
@@ -405,7 +407,7 @@ struct Pair {
   int64_t rows;
 };
 template <int T, int EPI>
-__global__ __launch_bounds__(threads<T>()) void k_lce_pair(Pair p) {
+__global__ __launch_bounds__(threads<T>(), waves<T>()) void k_lce_pair(Pair p) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int block = (int)blockIdx.x;
   if (block < p.na) gemm_body<T, false, false, EPI_STORE>(p.a, block, lds);
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(threads<T>()) void k_lce_pair(Pair p) {
 }
 template <int T, int EPI>
 __global__ __launch_bounds__(256) void k_lce_pair_rest(Pair p) {
-  constexpr int SLICES = T * T / 1024;
+  constexpr int SLICES = slices<T>();
   const int block = (int)blockIdx.x;
   if (block < p.a.rest * SLICES) rest_body<T, EPI_STORE>(p.a, block);
   else rest_body<T, EPI>(p.b, block - p.a.rest * SLICES);
@@ -615,7 +617,7 @@ int launch_logits(const Gemm& g) {
   DF_LAUNCH((k_split_gemm<T, false, true, EPI>), dim3((unsigned)groups(g)), dim3(threads<T>()), lds_bytes<T>(), stream(), g);
   DF_LAUNCH_CHECK();
   if (g.rest) {
-    DF_LAUNCH((k_split_rest<T, EPI>), dim3((unsigned)g.rest * (T * T / 1024)), dim3(256), 0, stream(), g);
+    DF_LAUNCH((k_split_rest<T, EPI>), dim3((unsigned)g.rest * slices<T>()), dim3(256), 0, stream(), g);
     DF_LAUNCH_CHECK();
   }
   return DFHIP_OK;
@@ -629,7 +631,7 @@ int launch_pair(const Pair& p) {
   DF_LAUNCH((k_lce_pair<T, EPI>), dim3((unsigned)(p.na + p.nb + (p.loss ? 1 : 0))), dim3(threads<T>()), lds_bytes<T>(), stream(), p);
   DF_LAUNCH_CHECK();
   if (p.a.rest + p.b.rest) {
-    DF_LAUNCH((k_lce_pair_rest<T, EPI>), dim3((unsigned)(p.a.rest + p.b.rest) * (T * T / 1024)), dim3(256), 0, stream(), p);
+    DF_LAUNCH((k_lce_pair_rest<T, EPI>), dim3((unsigned)(p.a.rest + p.b.rest) * slices<T>()), dim3(256), 0, stream(), p);
     DF_LAUNCH_CHECK();
   }
   return DFHIP_OK;
@@ -921,7 +923,7 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
                    (float)label_smoothing);
     if (st != DFHIP_OK) return st;
     Pair p = {};
-    p.a.exp_c = p.b.exp_c = -kTop;
+    p.a.exp_c = p.b.exp_c = -kTopDl;
     p.a.scale = p.b.scale = &ctl->scale;
     if (dx) {
       p.a.a = (const char*)logits.p;

@@ -651,3 +651,68 @@ def test_smoothing_over_several_classes_of_the_lowest_value(hip_device, N, V):
     with no_grad():
         loss = F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, w, b, t)], label_smoothing=0.1)
     _within(float(loss.numpy()[0]), want, tol, "loss alone")
+
+
+# ---- small elements beside large ones --------------------------------------------------------------------------------------------
+# The two halves of an operand carry 2^-23 of it down to 2^-28 of the array's largest magnitude A, and an absolute 2^-49 A below
+# (dl, whose scale is fixed: 2^-51).  A product's bound is the one above with those floors, times two:
+#   |error| <= (12 + 6 sqrt(3 K)) u sum|a b| + 2^-48 (A sum|b| + B sum|a|).
+def _fine_product_error(a, b):
+    K = a.shape[1]
+    aa, bb = np.abs(a), np.abs(b)
+    fl = 2.0 ** -48 * (aa.max(initial=0.0) * bb.sum(0)[None, :] + bb.max(initial=0.0) * aa.sum(1)[:, None])
+    return (12 + 6 * np.sqrt(3 * K)) * U * (aa @ bb) + fl
+
+
+def _fine_gradients(x, w, b, t):
+    """the gradients of the mean and their bounds"""
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    N, V = x.shape[0], w.shape[1]
+    l = x @ w + b.astype(np.float64).reshape(1, -1)
+    # (one error of a row's largest logits moves all its probabilities; a logit's own moves its own)
+    E = _fine_product_error(x, w) + U * np.abs(l)
+    p = np.exp(l - l.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    # (the exponential's argument l - m is rounded: u |l - m|)
+    tp = p * (E + (E * p).sum(1, keepdims=True) + U * np.abs(l - l.max(1, keepdims=True)) + (V / 256 + 40) * U)
+    dl = p.copy()
+    dl[np.arange(N), t.astype(int)] -= 1.0
+    td = tp + 2.0 ** -22 * np.abs(dl) + 2.0 ** -50
+    td[np.arange(N), t.astype(int)] += 4 * U
+    dx, dw, db = dl @ w.T / N, x.T @ dl / N, dl.sum(0) / N
+    return ((dx, (_fine_product_error(dl, w.T) + td @ np.abs(w).T) / N + 4 * U * np.abs(dx)),
+            (dw, (_fine_product_error(x.T, dl) + np.abs(x).T @ td) / N + 4 * U * np.abs(dw)),
+            (db, (td.sum(0) + (N / 64 + 30) * U * np.abs(dl).sum(0)) / N + 4 * U * np.abs(db)))
+
+
+@pytest.mark.parametrize("N,D,V", [(100, 24, 700), (300, 130, 4001), (700, 64, 60000)])
+def test_classes_that_are_hardly_ever_likely(hip_device, N, D, V):
+    """probabilities from 1e-2 to 1e-13 side by side: every class's column of dW and element of db is as good as its own magnitude asks"""
+    x, w, b, t = _data(N, D, V, 47)
+    b -= np.array([0.0, 10.0, 16.0, 22.0, 26.0], np.float32)[np.arange(V) % 5]
+    t -= t % 5                                                 # (targets among the likely ones: the others' columns are as small as p)
+    got = _run(hip_device, 0.25 * x, w, b, t)
+    for g, (want, tol), what in zip(got[1:], _fine_gradients(np.float32(0.25) * x, w, b, t), ("dx", "dw", "db")):
+        _within(g, want, tol, what)
+
+
+@pytest.mark.parametrize("small", [2.0 ** -12, 2.0 ** -20, 2.0 ** -26])
+def test_features_of_different_magnitudes(hip_device, small):
+    """columns of x far below the others: their rows of dW; rows of W far below the others: their columns of dx"""
+    x, w, b, t = _data(200, 96, 900, 48)
+    x[:, 1::3] *= np.float32(small)
+    w[2::3] *= np.float32(small)
+    got = _run(hip_device, x, w, b, t)
+    for g, (want, tol), what in zip(got[1:], _fine_gradients(x, w, b, t), ("dx", "dw", "db")):
+        _within(g, want, tol, what)
+
+
+@pytest.mark.parametrize("large", [2.0 ** 10, 2.0 ** 20, 2.0 ** 30])
+def test_a_row_far_above_the_others(hip_device, large):
+    """one row's magnitude does not cost the others their logits: the gradients of the rows of an ordinary batch beside it.  (Its own
+    loss is so large that the mean says nothing of theirs: dx does.)"""
+    x, w, b, t = _data(150, 48, 500, 49)
+    x[17] *= np.float32(large)
+    got = _run(hip_device, x, w, b, t)
+    want, tol = _fine_gradients(x, w, b, t)[0]
+    _within(np.delete(got[1], 17, 0), np.delete(want, 17, 0), np.delete(tol, 17, 0), "dx")
