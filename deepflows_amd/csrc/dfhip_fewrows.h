@@ -1,4 +1,4 @@
-// fp32 products of FEW rows (at most 64) with a large matrix W on the fp32 matrix cores.
+// fp32 products of FEW rows (at most 64 a workgroup) with a large matrix W on the fp32 matrix cores.
 //
 // What bounds them is reading W, or writing a gradient of its size: 32 rows are 64 operations for the 4 bytes of an element, and
 // the fp32 matrix cores form 121 in the time that HBM takes for them (153 TFLOP/s, 5.07 TB/s).  So W is read as it is, once a
@@ -21,7 +21,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));      // rows of any width begin on any element
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kMost = 64;                          // rows
+constexpr int kMost = 64;                          // rows a workgroup; of the gradients, rows in all
 
 // rows x n outputs over kn; `a` (rows, lda), `b` (kn, ldb), along: (n, ldb)
 struct Product {

@@ -447,14 +447,20 @@ struct Few {
 template <int RB, int CF, int NW>
 __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
   __shared__ dfhip_few::f32x4 lds[dfhip_few::lds_pieces<CF, NW>()];
-  const dfhip_few::Product& p = g.logits;
-  const int tile = (int)blockIdx.x, n0 = tile * 32 * CF, i = threadIdx.x & 31;
+  // (64 rows a workgroup; a tile's workgroups eight numbers apart, on the same XCD, where W comes out of the L2 for the second)
+  const int sets = (g.logits.rows + 63) >> 6, block = (int)blockIdx.x;
+  const int tile = (block >> 3) / sets * 8 + (block & 7), row0 = (block >> 3) % sets * 64, n0 = tile * 32 * CF, i = threadIdx.x & 31;
+  if (tile >= g.tiles) return;
+  dfhip_few::Product p = g.logits;
+  p.a += (int64_t)row0 * p.lda;
+  p.rows = min(p.rows - row0, 64);
   const int c = n0 + CF * i, over = c - min(c, p.n - CF);  // columns by which this lane's loads were moved back
   float bias[CF];
 #pragma unroll
   for (int f = 0; f < CF; f++) bias[f] = g.bias && c + f < p.n ? g.bias[c + f] : 0.0f;
   dfhip_few::across<RB, CF, NW>(p, n0, lds, [&](int row, const float* v) {
     if (row >= p.rows) return;                             // (uniform in the half wave)
+    row += row0;
     float w[CF];                                           // -inf behind the last class
 #pragma unroll
     for (int f = 0; f < CF; f++) {
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(NW * 64) void k_few_logits(Few g) {
 #pragma unroll
     for (int f = 0; f < CF; f++) in[f] = c + f < p.n;
     const RowPart part = row_part<CF, 32>(w, in, g.smooth > 0.0f);
-    if (i == 0) store_part(g.stat + (int64_t)row * g.tiles + tile, (int64_t)p.rows * g.tiles, part);
+    if (i == 0) store_part(g.stat + (int64_t)row * g.tiles + tile, (int64_t)g.logits.rows * g.tiles, part);
   });
 }
 
@@ -713,16 +719,18 @@ int rows_pass(float* logits, const float* target, int n, int launch_rows, float*
 //     where W is very large (1024 x 34001 220 / 196, 1024 x 50001 277 / 284, 2048 x 50001 513 / 584), and where the launches are
 //     what counts, four instead of six (100 x 500 22 / 21, 256 x 1000 24.5 / 24, 512 x 2000 28.6 / 29.5, 64 x 50001 52 / 61, but
 //     1024 x 1000 34 / 31, 256 x 16384 47 / 45; the host, where it is slower than the device, saves 5 us of 38)
-//   more rows would be as fast at best (128, the loss alone: 1024 x 34001 119 / 104, 1024 x 50001 151 / 139, 2048 x 99991 496 / 546)
+//   65 to 128 rows: the loss alone over a very large W (128 rows: 1024 x 34001 121 / 106, 1024 x 50001 154 / 139, 2048 x 50001 287 / 278,
+//     1024 x 99991 273 / 282, 2048 x 99991 500 / 551, 4096 x 64000 561 / 668; 65 rows 125 / 108 to 549 / 657)
 inline bool few_rows(int64_t rows, int64_t width, int64_t classes, bool grads) {
-  if (classes < 4 || rows > dfhip_few::kMost) return false;
   const int64_t size = width * classes, M = 1 << 20;
+  if (classes < 4 || rows > (grads ? 1 : 2) * dfhip_few::kMost) return false;
+  if (rows > dfhip_few::kMost) return size >= 128 * M;
   return rows <= 32 || (grads ? size >= 48 * M || (width <= 512 && size <= 7 * M / 2) : size >= 3 * M || width <= 1024);
 }
 
 template <int RB>
 int few_logits(const Few& g) {
-  const dim3 grid((unsigned)g.tiles);
+  const dim3 grid((unsigned)(df_ceil_div(g.tiles, 8) * 8 * df_ceil_div(g.logits.rows, 64)));
   if (g.cols == 32) DF_LAUNCH((k_few_logits<RB, 1, 8>), grid, dim3(512), 0, stream(), g);
   else DF_LAUNCH((k_few_logits<RB, 4, 4>), grid, dim3(256), 0, stream(), g);
   DF_LAUNCH_CHECK();

@@ -716,3 +716,30 @@ def test_a_row_far_above_the_others(hip_device, large):
     got = _run(hip_device, x, w, b, t)
     want, tol = _fine_gradients(x, w, b, t)[0]
     _within(np.delete(got[1], 17, 0), np.delete(want, 17, 0), np.delete(tol, 17, 0), "dx")
+
+
+@pytest.mark.parametrize("N", [65, 100, 128])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_evaluation_of_65_to_128_rows_over_a_very_large_weight(hip_device, N, smoothing):
+    """140 M weights, 1 000 different columns of them with a bias each: the bound of `_reference`"""
+    from deepflows_amd.autograd import no_grad
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    D, V, e = 1401, 100003, smoothing
+    x, w0, _, _ = _data(N, D, 1000, 50)
+    _, _, b, t = _data(N, 1, V, 51, ignored=0.2)
+    wide = lambda a: np.tile(a, (1, V // 1000 + 1))[:, :V]
+    x64, w64 = x.astype(np.float64), w0.astype(np.float64)
+    l = wide(x64 @ w64) + b.astype(np.float64)
+    E = (wide(_product_error(x64, w64)) + U * np.abs(l)).max(1)
+    m = l.max(1)
+    lse = np.log(np.exp(l - m[:, None]).sum(1)) + m
+    counted = t != -100
+    lt = l[np.arange(N), np.where(counted, t, 0).astype(int)]
+    row = lse - (1 - e) * lt - e * l.mean(1)
+    trow = 3 * E + U * (V / 256 + 60) * (1 + np.abs(lse - lt)) + e * U * (V / 256 + 30) * np.abs(l - m[:, None]).mean(1)
+    want, tol = row[counted].mean(), trow[counted].mean() + 14 * U * np.abs(row[counted]).mean()
+    x[~counted] = np.nan
+    with no_grad():
+        loss = F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, wide(w0), b, t)], label_smoothing=e)
+    _within(float(loss.numpy()[0]), want, tol, "loss")
