@@ -501,7 +501,7 @@ def rms_norm(input: Tensor, weight=None, eps: float = 1e-6, residual=None):
     if weight is not None:
         if weight is input:
             raise ValueError("rms_norm: weight and input are one tensor")
-        if weight.size != width or weight.shape[-1] != width:
+        if weight.size != width or tuple(weight.shape)[-1:] != (width,):
             raise ValueError(f"rms_norm: weight of shape {tuple(weight.shape)} for a last axis of {width}")
     if residual is not None and tuple(residual.shape) != shape:
         raise ValueError(f"rms_norm: residual of shape {tuple(residual.shape)} for an input of shape {shape}")
@@ -667,7 +667,7 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     rows, classes = int(xs[0]), int(ws[1])
     if classes < 1 or xs[1] < 1:
         raise ValueError("linear_cross_entropy: at least one class and one input feature are needed")
-    if bias is not None and (bias.size != classes or bias.shape[-1] != classes):
+    if bias is not None and (bias.size != classes or tuple(bias.shape)[-1:] != (classes,)):
         raise ValueError(f"linear_cross_entropy: bias of shape {tuple(bias.shape)} for {classes} classes")
     if tuple(target.shape) != (rows,):
         raise ValueError(f"linear_cross_entropy: target of shape {tuple(target.shape)} for {rows} rows (class indices, one a row)")

@@ -227,3 +227,17 @@ def test_clip_of_magnitudes_whose_squares_no_float_holds(cpu_oracle, magnitude):
     for a, p in zip(arrays, params):
         expected = a.astype(np.float64) * min(1.0, most / (norm + 1e-6))
         assert np.all(np.abs(p.grad.numpy() - expected) <= 2 ** -22 * np.abs(expected) + 2 ** -149)
+
+
+def test_operands_without_an_axis_are_refused(cpu_oracle):
+    from deepflows_amd.nn import functional as F
+    from deepflows_amd.tensor import Tensor
+    new = lambda *s: Tensor(np.zeros(s, np.float32), device=cpu_oracle)
+    with pytest.raises(ValueError):
+        F.rms_norm(new(3, 1), new())
+    with pytest.raises(ValueError):
+        F.rms_norm(new(), None)
+    with pytest.raises(ValueError):
+        F.linear_cross_entropy(new(4, 3), new(3, 1), new(), new(4))
+    with pytest.raises(ValueError):
+        F.linear_cross_entropy(new(4, 3), new(3, 1), None, new())
