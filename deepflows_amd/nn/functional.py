@@ -658,8 +658,13 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     input (N, D), weight (D, V), bias None or V elements, target (N,): class indices as whole numbers (fp32, the device's only
     type, holds them exactly up to 2^24 classes).  Rows whose target is `ignore_index` are not counted; 'mean' divides by the
     number of counted rows, and a batch without one has loss 0 and zero gradients.  What stands in a row of input that is not
-    counted does not matter, NaN and infinities included.  label_smoothing e: the target distribution is (1 - e) onehot + e / V.  On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it
-    in time to raise would stall the device); elsewhere it raises ValueError."""
+    counted does not matter, NaN and infinities included.  label_smoothing e: the target distribution is (1 - e) onehot + e / V.
+
+    On the hip device a target outside [0, V) makes the loss and the gradients it reaches NaN (finding it in time to raise would
+    stall the device); elsewhere it raises ValueError.  There the products of more rows than a few are formed on the fp16 matrix
+    cores from two halves of every operand and added up in fp32: 2^-23 of an element is lost where it is at least 2^-28 of its
+    array's largest magnitude, at most 2^-49 of that below (of the logits' gradient 2^-51).  Large sums come out closer to the exact
+    ones than fp32 products do; what is smaller than that beside the largest element of its array counts as 0."""
     input, weight, bias = realize(input), realize(weight), realize(bias)
     xs, ws, device = tuple(input.shape), tuple(weight.shape), input.device
     if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[0]:

@@ -16,7 +16,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, grad_scale=1.0, error_i
     tensor of shape (1,).
 
     norm_type 2: the square root of the sum of all squares, held in double; norm_type inf: the largest magnitude.  Every
-    gradient is multiplied by min(1, max_norm / (norm + 1e-6)); a NaN or an infinity in one of them shows in the norm and in all.
+    gradient is multiplied by min(1, max_norm / (norm + 1e-6)).  A NaN in one of them makes the norm and all of them NaN; an infinity
+    makes the norm infinite, hence the factor 0: itself NaN, everything finite 0.
     Parameters without a gradient are passed over, one that is listed twice counts once.  `grad_scale` is the factor the
     optimizer applies when it steps (`optimizer.grad_scale`, 1/world behind a gradient exchange): the norm is that of the scaled
     gradients.  error_if_nonfinite reads the norm back and raises RuntimeError instead of scaling, which a captured step cannot.
