@@ -14,19 +14,20 @@
 // STORAGE ("split array"): a padded row-major array of 4-byte cells, columns in blocks of 32: 128 bytes that hold the block's 32
 // hi halves, then its 32 lo halves.  A cell takes as much room as the fp32 value it stands for, so an fp32 array can be converted
 // in place block by block, and ONE copy of an array serves as either operand of a product:
-//   the reduction runs along the rows of the storage ("K along"): a tile is 128-byte pieces of T rows, read as 16-byte fragments;
-//   the reduction runs across them ("K across"): a tile is 32 rows of 4 T bytes, read with the transposing LDS loads
+//   the reduction runs along the rows of the storage ("K along"): a tile is 128-byte pieces of BM (BN) rows, read as 16-byte fragments;
+//   the reduction runs across them ("K across"): a tile is 32 rows of 4 BM (BN) bytes, read with the transposing LDS loads
 //   (ds_read_b64_tr_b16: 16 lanes hand in 4 rows x 16 halves, each lane receives the 4 rows of its column).
 //
 // KERNEL: workgroup tile BM x BN, K step 32, LDS buffers filled by 16-byte global-to-LDS copies issued NS - 1 steps ahead; one
 // barrier a step.  32 x 32 x 16 MFMA.  T = 256: 256 x 128 by eight waves of 64 x 64, two buffers, one workgroup a CU; T = 128:
 // 128 x 128 by four waves of 64 x 64, two buffers, two workgroups a CU; T = 64: 64 x 64 by four waves of 32 x 32, four buffers (short
 // reductions and few tiles wait for memory, not for the matrix cores).
-// The second set of accumulators is what the tiles are small for: one set allowed 256 x 256 by waves of 128 x 64, whose operands cross
-// the LDS two thirds as often (8192 x 1024 x 50001: 6.6 ms against 7.07).  Those waves with both sets, one a SIMD (256 x 128 by four):
-// 110 us where eight waves take 96; a third buffer: 99.  LDS positions are XOR-permuted at 16-byte granularity by the ROW (the copy's source address is permuted,
-// its LDS side is linear): 16 lanes that read the same piece of 16 rows, or 32 lanes that read 4 rows transposed, touch every bank
-// once (SQ_LDS_BANK_CONFLICT reads 0).
+// The second set of accumulators is what the tiles are small for: one set allowed 256 x 256 by waves of 128 x 64, whose operands come
+// out of the LDS three quarters as often (8192 x 1024 x 50001: 6.6 ms against 7.07; the power limit sets the clock).  Those waves with
+// both sets, one a SIMD (256 x 128 by four): 110 us where eight waves take 96; a third buffer: 99 (256 tiles, 64 steps).
+// LDS positions are XOR-permuted at 16-byte granularity by the ROW (the copy's source address is permuted, its LDS side is linear): 16
+// lanes that read the same piece of 16 rows, or 32 lanes that read 4 rows transposed, touch every bank once (SQ_LDS_BANK_CONFLICT
+// reads 0).
 // LDS reads: three products share two fragments a side, so the LDS moves half the bytes an fp16 GEMM of the same rate would.
 #pragma once
 #include <algorithm>

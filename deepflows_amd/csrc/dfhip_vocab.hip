@@ -671,7 +671,9 @@ const Choice* choose(int64_t rows, int64_t width, int64_t classes, bool dx, int6
   double least = 1e300, least_pair = 1e300;
   for (int tile : {256, 128, 64}) {
     Plan l[kWays], a[kWays] = {}, b[kWays] = {};
-    const int nl = ways(tile, rows, classes, (int)df_ceil_div(width, 32), l);
+    // (256 x 128 tiles are for the pair alone: 8192 x 1024 x 50001 7.67 -> 7.16 ms; the logits of 157 x 4274 x 63752 take 847 us with
+    // them and 828 without)
+    const int nl = tile == 256 ? 0 : ways(tile, rows, classes, (int)df_ceil_div(width, 32), l);
     for (int i = 0; i < nl; i++) {
       const double us = cost_us(&l[i], 1);
       if (us < least) { least = us; c.logits = l[i]; }
@@ -897,7 +899,7 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
       g.c = logits.p;
       g.ldc = vp;
     } else {                                       // the softmax's parts instead of the logits
-      g.units = (int)df_ceil_div(classes, how->logits.tile == 64 ? unit<64>() : unit<256>());
+      g.units = (int)df_ceil_div(classes, how->logits.tile == 64 ? unit<64>() : unit<128>());
       g.lt = logits.p;
       g.stat = logits.p + n;
       g.target = target + r0;
@@ -907,16 +909,14 @@ int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, c
     st = room(parts, held, std::max(parts_floats(how->logits), parts_floats(how->a) + parts_floats(how->b)));
     if (st != DFHIP_OK) return st;
     g.parts = parts.p;
-    st = with_tile(how->logits, [&](auto t) {
-      constexpr int T = decltype(t)::value;
-      return grads ? launch_logits<T, EPI_BIAS>(g) : launch_logits<T, EPI_STATS>(g);
-    });
+    if (how->logits.tile == 128) st = grads ? launch_logits<128, EPI_BIAS>(g) : launch_logits<128, EPI_STATS>(g);
+    else st = grads ? launch_logits<64, EPI_BIAS>(g) : launch_logits<64, EPI_STATS>(g);
     if (st != DFHIP_OK) return st;
     if (!grads) {
       Few f = {};
       f.stat = g.stat;
       f.tiles = g.units;
-      f.cols = how->logits.tile == 64 ? unit<64>() : unit<256>();
+      f.cols = how->logits.tile == 64 ? unit<64>() : unit<128>();
       f.lt = g.lt;
       f.ld = classes;
       f.target = g.target;

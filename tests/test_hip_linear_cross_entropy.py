@@ -743,3 +743,33 @@ def test_evaluation_of_65_to_128_rows_over_a_very_large_weight(hip_device, N, sm
     with no_grad():
         loss = F.linear_cross_entropy(*[Tensor(a, device=hip_device) for a in (x, wide(w0), b, t)], label_smoothing=e)
     _within(float(loss.numpy()[0]), want, tol, "loss")
+
+
+@pytest.mark.parametrize("N,D,V", [(8328, 183, 7929), (1858, 1542, 4233), (2239, 438, 14704), (2776, 1197, 5054), (6144, 180, 100003)])
+def test_the_largest_tiles_of_the_gradient_products(hip_device, N, D, V):
+    """Gradient products by 256 x 128 tiles: both with a last round that is cut along the reduction, neither, one each, and two pieces
+    of the logits.  The rows are 60 different ones in any order: their loss, dW and db are theirs times their share.  dW's bound grows
+    with the root of the rows, db's with N / 64 + 30, the loss's not (it is added up in double)."""
+    x, w, b, t = _data(60, D, V, 52, ignored=0.1)
+    order = np.random.default_rng(53).permutation(np.tile(np.arange(60), N // 60 + 1)[:N])
+    share = np.bincount(order, minlength=60).astype(np.float64)
+    got = _run(hip_device, x[order], w, b, t[order], label_smoothing=0.1)
+    counted = t != -100
+    total = share[counted].sum()
+    _, (dx, tdx), (_, tdw), (_, tdb) = _reference(x, w, b, t, mean=False, e=0.1)
+    x64, l = x.astype(np.float64), x.astype(np.float64) @ w.astype(np.float64) + b.astype(np.float64)
+    lse = np.log(np.exp(l - l.max(1, keepdims=True)).sum(1)) + l.max(1)
+    place = np.where(counted, t, 0).astype(int)
+    row = (lse - 0.9 * l[np.arange(60), place] - 0.1 * l.mean(1)) * counted
+    E = (_product_error(x64, w.astype(np.float64)) + U * np.abs(l)).max(1)
+    trow = 3 * E + U * (V / 256 + 60) * (1 + np.abs(lse - l[np.arange(60), place])) \
+        + U * (V / 256 + 30) * np.abs(l - l.max(1, keepdims=True)).mean(1)
+    _within(got[0], (share * row).sum() / total, (share * trow * counted).sum() / total + 14 * U * np.abs(share * row).sum() / total, "loss")
+    _within(got[1], dx[order] / total, tdx[order] / total + 4 * U * np.abs(dx[order]) / total, "dx")
+    dl = np.exp(l - lse[:, None])
+    dl -= 0.1 / V
+    dl[np.arange(60), place] -= 0.9
+    dl *= (counted * share / total)[:, None]
+    most = share.max()                                         # (a row's share differs by one)
+    _within(got[2], x64.T @ dl, np.sqrt(N / 60) * tdw * most / total, "dw")
+    _within(got[3], dl.sum(0, keepdims=True), (N / 64 + 30) / 30 * tdb * most / total, "db")
