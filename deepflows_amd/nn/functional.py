@@ -664,7 +664,8 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, bias, target: Tensor, re
     stall the device); elsewhere it raises ValueError.  There the products of more rows than a few are formed on the fp16 matrix
     cores from two halves of every operand and added up in fp32: 2^-23 of an element is lost where it is at least 2^-28 of its
     array's largest magnitude, at most 2^-49 of that below (of the logits' gradient 2^-51).  Large sums come out closer to the exact
-    ones than fp32 products do; what is smaller than that beside the largest element of its array counts as 0."""
+    ones than fp32 products do; what is smaller than that beside the largest element of its array counts as 0.  Classes are masked by
+    the bias (-inf or the type's lowest value): an infinity in a counted row or in weight makes NaN where fp32 might keep -inf."""
     input, weight, bias = realize(input), realize(weight), realize(bias)
     xs, ws, device = tuple(input.shape), tuple(weight.shape), input.device
     if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[0]:

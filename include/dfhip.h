@@ -504,7 +504,8 @@ int dfhip_mlp2_ce_backward(const float* x, const float* h, const float* dz1, con
  * nothing added to dw and db, whatever their elements are (NaN too).  A target that is neither ignore_index nor a whole number in
  * [0, classes) makes the loss and the gradients it reaches NaN.  At most 2^24 classes.  Without counted rows the loss and the
  * gradients are 0.  Few rows: fp32 products.  More: an element of x, w or dl enters a product with an error of at most 2^-23 of
- * itself plus 2^-49 of its array's largest magnitude (dl: 2^-51); sums are fp32, the loss's over the rows double.
+ * itself plus 2^-49 of its array's largest magnitude (dl: 2^-51); sums are fp32, the loss's over the rows double.  bias may mask classes
+ * (-inf or the lowest float); an infinity in a counted row of x or in w may become NaN where fp32 would keep it.
  * Scratch memory comes from the pool and does not grow with rows x classes.  No output may overlap an input. */
 int dfhip_linear_ce_forward(const float* x, const float* w, const float* bias, const float* target, float* loss, float* dx,
                             float* dw, float* db, int64_t rows, int64_t width, int64_t classes, int64_t ignore_index,
